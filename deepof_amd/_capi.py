@@ -71,6 +71,27 @@ class PreprocDims(C.Structure):
                 ("scale_kind", C.c_int32), ("reserved", C.c_int32), ("col_keep", C.c_void_p), ("video_scaler_in", C.c_void_p)]
 
 
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
+_ST = C.c_int64 * 2   # (row, head) strides
+
+
+class NormRope(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("head_dim", C.c_int32), ("rot_dim", C.c_int32), ("interleaved", C.c_int32),
+                ("q_heads", C.c_int32), ("k_heads", C.c_int32), ("tokens", C.c_int64), ("eps", C.c_float),
+                ("reserved", C.c_int32), ("q_stride", _ST), ("k_stride", _ST), ("q_out_stride", _ST),
+                ("k_out_stride", _ST), ("gq_stride", _ST), ("gk_stride", _ST)]
+
+
+class AttnPlan(C.Structure):
+    _fields_ = [("n_docs", C.c_int32), ("causal", C.c_int32), ("n_tiles", C.c_int64 * 4), ("table_bytes", C.c_int64)]
+
+
+class Attention(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("head_dim", C.c_int32), ("q_heads", C.c_int32), ("k_heads", C.c_int32),
+                ("scale", C.c_float), ("cap", C.c_float), ("q_stride", _ST), ("k_stride", _ST), ("v_stride", _ST),
+                ("o_stride", _ST), ("g_stride", _ST), ("dq_stride", _ST), ("dk_stride", _ST), ("dv_stride", _ST)]
+
+
 PP_KINDS = {"other": 0, "coord": 1, "speed": 2, "dist_inner": 3, "dist_intra": 4, "angle": 5}
 PP_MODES = {None: 0, "per_column": 1, "groupwise": 2}
 PP_INTER_SCALE = {"mean": 0, "geom": 1, "global": 2}
@@ -149,6 +170,14 @@ SIGNATURES = {
     "dof_preprocess_fit_global": (C.c_int, [C.POINTER(PreprocDims), _I32, _P, _P, _P, _P]),
     "dof_preprocess_raw_moments": (C.c_int, [C.POINTER(PreprocDims)] + [_P] * 6),
     "dof_preprocess_order_stats": (C.c_int, [C.POINTER(PreprocDims)] + [_P] * 11),
+    "dof_norm_rope_forward": (C.c_int, [C.POINTER(NormRope)] + [_P] * 9),
+    "dof_norm_rope_workspace_bytes": (_I64, [C.POINTER(NormRope)]),
+    "dof_norm_rope_backward": (C.c_int, [C.POINTER(NormRope)] + [_P] * 14),
+    "dof_attn_plan_size": (C.c_int, [_I32, _P, _P, _I32, C.POINTER(AttnPlan)]),
+    "dof_attn_plan_table": (C.c_int, [C.POINTER(AttnPlan), _P, _P, _P, _P]),
+    "dof_attention_forward": (C.c_int, [C.POINTER(AttnPlan), _P, C.POINTER(Attention)] + [_P] * 7),
+    "dof_attention_workspace_bytes": (_I64, [_I64, _I32]),
+    "dof_attention_backward": (C.c_int, [C.POINTER(AttnPlan), _P, C.POINTER(Attention)] + [_P] * 12),
 }
 
 

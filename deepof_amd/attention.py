@@ -1,0 +1,342 @@
+"""Sequence operators on packed recordings: what a transformer over whole recordings needs next to the windowed family.
+
+The transformer family (/root/reference/deepof/clustering/models_new.py:832-1327) attends inside one window, in fp32, with
+sinusoidal positions added to its input.  These operators take the same mathematics to recordings of any length: ``norm_rope``
+(RMS norm of every query / key head and rotation by its position, one pass), ``attention`` (packed documents, grouped heads,
+causal / prefix masks, tanh cap, distance bias) -- both with their backward pass -- and ``attention_step``, which takes the new
+frames of live streams against a paged key / value cache.  Elements are float32, bfloat16 or float16; sums, norms and softmax
+statistics are fp32.
+
+``AttentionOps`` issues the C-ABI calls (include/deepof_hip.h) on the current HIP stream of its device; product code obtains it
+through :func:`create_attention_ops`, which requires a ROCm device and the compiled library and raises otherwise.  Workspaces and
+outputs come from torch's allocator, one per call, so calls on different streams and captured graphs never share memory.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes as C
+from typing import Optional, Sequence
+
+import numpy as np
+import torch
+
+from . import _capi
+
+DTYPES = {torch.float32: _capi.DTYPE_F32, torch.bfloat16: _capi.DTYPE_BF16, torch.float16: _capi.DTYPE_F16}
+
+
+def rotary_frequencies(rot_dim: int, base: float = 10000.0, scale: float = 1.0, original_length: Optional[float] = None,
+                       low_turns: float = 1.0, high_turns: float = 32.0, device=None) -> torch.Tensor:
+    """Angles per position of the ``rot_dim / 2`` pairs, float64: ``base ** (-2 i / rot_dim)``.
+
+    ``scale`` > 1 stretches the positions for recordings that many times longer than those trained on.  Without
+    ``original_length`` every frequency is divided by it.  With it, only the slow pairs are: a pair that turns fewer than
+    ``low_turns`` times over ``original_length`` positions is divided by ``scale``, one that turns more than ``high_turns`` times
+    stays, and between the two the divisor's reciprocal runs linearly with the number of turns."""
+    if rot_dim < 2 or rot_dim % 2:
+        raise ValueError(f"rot_dim must be an even number from 2, got {rot_dim}")
+    if not (base > 0.0 and scale > 0.0):
+        raise ValueError("base and scale must be positive")
+    f = float(base) ** (-torch.arange(rot_dim // 2, dtype=torch.float64) / (rot_dim // 2))
+    if scale != 1.0:
+        if original_length is None:
+            f = f / scale
+        else:
+            if not 0.0 <= low_turns < high_turns:
+                raise ValueError("need 0 <= low_turns < high_turns")
+            turns = f * (original_length / (2.0 * np.pi))
+            keep = ((turns - low_turns) / (high_turns - low_turns)).clamp(0.0, 1.0)
+            f = f * (keep + (1.0 - keep) / scale)
+    return f.to(device) if device is not None else f
+
+
+def _rows(name: str, t: torch.Tensor, device, dtype=None, ndim: int = 3):
+    """A (..., heads, head_dim) tensor whose heads are runs of memory; raises otherwise."""
+    if not isinstance(t, torch.Tensor) or t.dim() != ndim:
+        raise ValueError(f"{name} must be a tensor of {ndim} dimensions")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, these operators are on {device}")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{name} has dtype {t.dtype}, expected {dtype}")
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"the elements of a head of {name} must lie side by side (stride 1 in the last dimension)")
+    return t
+
+
+def _writable(name: str, t: torch.Tensor):
+    """An output may not address one element twice (an expanded view)."""
+    for n, s in zip(t.shape, t.stride()):
+        if n > 1 and s == 0:
+            raise ValueError(f"{name} is an expanded view; its elements must be distinct")
+    return t
+
+
+def _vector(name: str, t: Optional[torch.Tensor], n: int, dtype, device):
+    if t is None:
+        return 0
+    if t.shape != (n,) or t.dtype != dtype or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of {n} elements on {device}")
+    return t.data_ptr()
+
+
+def _st(t: torch.Tensor):
+    """Row and head strides of a (rows, heads, head_dim) tensor."""
+    s = t.stride()
+    return (s[0], s[1])
+
+
+def _is_wide(t: torch.Tensor) -> bool:
+    """Address and strides are multiples of 16 bytes (what the attention kernels load at once)."""
+    e = t.element_size()
+    return t.data_ptr() % 16 == 0 and all(s * e % 16 == 0 for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n > 1)
+
+
+def _wide(t: torch.Tensor) -> torch.Tensor:
+    """The tensor itself, or a contiguous copy of one whose memory the kernels' 16-byte loads do not fit."""
+    return t if _is_wide(t) else t.clone(memory_format=torch.contiguous_format)
+
+
+class AttentionPlan:
+    """The tiles of one packed batch on the device (:meth:`AttentionOps.attention_plan`): serves any number of heads, head sizes,
+    dtypes and streams, forward and backward; never written after it is made."""
+
+    def __init__(self, ops: "AttentionOps", q_lengths, k_lengths, causal, prefix):
+        ql = self._host("q_lengths", q_lengths)
+        kl = ql if k_lengths is None else self._host("k_lengths", k_lengths)
+        if len(kl) != len(ql):
+            raise ValueError(f"{len(ql)} query lengths and {len(kl)} key lengths")
+        if prefix is not None and not causal:
+            raise ValueError("a prefix is part of a causal mask: pass causal=True")
+        pre = None
+        if prefix is not None:
+            pre = self._host("prefix", prefix)
+            if len(pre) != len(ql):
+                raise ValueError(f"{len(ql)} documents and {len(pre)} prefixes")
+            pre = np.minimum(pre, 2 ** 31 - 1).astype(np.int32)
+        q_off, k_off = (np.concatenate(([0], np.cumsum(x))).astype(np.int64) for x in (ql, kl))
+        self.device, self.causal, self.n_docs = ops.device, bool(causal), len(ql)
+        self.q_rows, self.k_rows = int(q_off[-1]), int(k_off[-1])
+        self.record = _capi.AttnPlan()
+        _capi.check(ops.lib, ops.lib.dof_attn_plan_size(len(ql), q_off.ctypes.data, k_off.ctypes.data, int(self.causal),
+                                                        C.byref(self.record)), "dof_attn_plan_size")
+        host = torch.empty(max(16, self.record.table_bytes), dtype=torch.uint8)
+        _capi.check(ops.lib, ops.lib.dof_attn_plan_table(C.byref(self.record), q_off.ctypes.data, k_off.ctypes.data,
+                                                         pre.ctypes.data if pre is not None else 0, host.data_ptr()),
+                    "dof_attn_plan_table")
+        self.table = host.to(self.device)
+
+    @staticmethod
+    def _host(name, lengths):
+        if isinstance(lengths, torch.Tensor) and lengths.is_cuda:
+            raise ValueError(f"{name} must be host data: the plan is made on the host")
+        a = np.asarray(lengths)
+        if a.ndim != 1 or (a.size and a.dtype.kind not in "iu"):
+            raise ValueError(f"{name} must be a sequence of whole numbers")
+        a = a.astype(np.int64)
+        if a.size and a.min() < 0:
+            raise ValueError(f"{name} must not be negative")
+        return a
+
+
+class AttentionOps:
+    """The operators on one device.  Holds no state between calls; safe to share between streams and captured graphs."""
+
+    def __init__(self, lib, device):
+        self.lib = lib
+        self.device = torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+
+    def _on_device(self):
+        """Launches go to the current device: make it this object's for the call if it is another one."""
+        if self.device.type == "cuda" and torch.cuda.current_device() != self.device.index:
+            return torch.cuda.device(self.device)
+        return contextlib.nullcontext()
+
+    def _stream(self):
+        if self.device.type == "cuda":
+            return torch.cuda.current_stream(self.device).cuda_stream
+        return 0
+
+    def _dtype(self, name, t):
+        if not isinstance(t, torch.Tensor) or t.dtype not in DTYPES:
+            raise ValueError(f"{name} must be a float32, bfloat16 or float16 tensor")
+        return t.dtype
+
+    def _output(self, name, t, like_shape, dtype):
+        if t is None:
+            return torch.empty(like_shape, dtype=dtype, device=self.device)
+        _rows(name, t, self.device, dtype, len(like_shape))
+        if tuple(t.shape) != tuple(like_shape):
+            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(like_shape)}")
+        return _writable(name, t)
+
+    # ---- norm + rotation ------------------------------------------------------------------------------------------
+    def _norm_rope_dims(self, q, k, positions, freqs, eps, interleaved):
+        dt = self._dtype("q", q)
+        _rows("q", q, self.device, dt)
+        _rows("k", k, self.device, dt)
+        if q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+            raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} must have the same rows and head size")
+        pos = _vector("positions", positions, q.shape[0], torch.int32, self.device)
+        if freqs.dim() != 1:
+            raise ValueError("freqs must hold one angle per rotated pair")
+        fr = _vector("freqs", freqs, freqs.shape[0], torch.float64, self.device)
+        if 2 * freqs.shape[0] > q.shape[2]:
+            raise ValueError(f"{freqs.shape[0]} rotated pairs do not fit a head of {q.shape[2]}")
+        if not eps >= 0.0:
+            raise ValueError("eps must not be negative")
+        d = _capi.NormRope()
+        d.dtype, d.head_dim, d.rot_dim, d.interleaved = DTYPES[dt], q.shape[2], 2 * freqs.shape[0], int(bool(interleaved))
+        d.q_heads, d.k_heads, d.tokens, d.eps = q.shape[1], k.shape[1], q.shape[0], eps
+        d.q_stride[:], d.k_stride[:] = _st(q), _st(k)
+        return d, pos, fr
+
+    def norm_rope(self, q, k, positions, freqs, q_weight=None, k_weight=None, eps: float = 1e-6, interleaved: bool = False,
+                  q_out=None, k_out=None):
+        """-> (q', k').  q (rows, query heads, head_dim) and k (rows, key heads, head_dim): every head divided by its root mean
+        square and multiplied by ``q_weight`` / ``k_weight`` (fp32, None: no norm), then its first ``2 len(freqs)`` elements
+        rotated by ``positions[row] * freqs[pair]`` (positions int32; freqs float64, see :func:`rotary_frequencies`).
+        ``interleaved``: neighbouring elements are a pair; otherwise the pairs lie half the rotated part apart.  ``q_out`` /
+        ``k_out`` may be q / k themselves."""
+        d, pos, fr = self._norm_rope_dims(q, k, positions, freqs, eps, interleaved)
+        q_out = self._output("q_out", q_out, q.shape, q.dtype)
+        k_out = self._output("k_out", k_out, k.shape, k.dtype)
+        d.q_out_stride[:], d.k_out_stride[:] = _st(q_out), _st(k_out)
+        wq = _vector("q_weight", q_weight, q.shape[2], torch.float32, self.device)
+        wk = _vector("k_weight", k_weight, q.shape[2], torch.float32, self.device)
+        with self._on_device():
+            rc = self.lib.dof_norm_rope_forward(C.byref(d), q.data_ptr(), k.data_ptr(), pos, fr, wq, wk, q_out.data_ptr(),
+                                                k_out.data_ptr(), self._stream())
+        _capi.check(self.lib, rc, "dof_norm_rope_forward")
+        return q_out, k_out
+
+    def norm_rope_backward(self, dq_out, dk_out, q, k, positions, freqs, q_weight=None, k_weight=None, eps: float = 1e-6,
+                           interleaved: bool = False):
+        """-> (dq, dk, dq_weight, dk_weight) from the gradients at :meth:`norm_rope`'s outputs and its inputs (the weight gradients
+        are None without a weight; they are the same bits on every run)."""
+        d, pos, fr = self._norm_rope_dims(q, k, positions, freqs, eps, interleaved)
+        for name, g, x in (("dq_out", dq_out, q), ("dk_out", dk_out, k)):
+            _rows(name, g, self.device, q.dtype)
+            if g.shape != x.shape:
+                raise ValueError(f"{name} has shape {tuple(g.shape)}, expected {tuple(x.shape)}")
+        d.gq_stride[:], d.gk_stride[:] = _st(dq_out), _st(dk_out)
+        dq = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+        dk = torch.empty(k.shape, dtype=k.dtype, device=self.device)
+        d.q_out_stride[:], d.k_out_stride[:] = _st(dq), _st(dk)
+        wq = _vector("q_weight", q_weight, q.shape[2], torch.float32, self.device)
+        wk = _vector("k_weight", k_weight, q.shape[2], torch.float32, self.device)
+        f32 = dict(dtype=torch.float32, device=self.device)
+        dwq = torch.empty(q.shape[2], **f32) if wq else None
+        dwk = torch.empty(q.shape[2], **f32) if wk else None
+        ws = torch.empty(self._bytes("dof_norm_rope_workspace_bytes", C.byref(d)) if wq or wk else 0, dtype=torch.uint8,
+                         device=self.device)
+        with self._on_device():
+            rc = self.lib.dof_norm_rope_backward(C.byref(d), dq_out.data_ptr(), dk_out.data_ptr(), q.data_ptr(), k.data_ptr(),
+                                                 pos, fr, wq, wk, dq.data_ptr(), dk.data_ptr(),
+                                                 dwq.data_ptr() if wq else 0, dwk.data_ptr() if wk else 0, ws.data_ptr(),
+                                                 self._stream())
+        _capi.check(self.lib, rc, "dof_norm_rope_backward")
+        return dq, dk, dwq, dwk
+
+    # ---- attention over packed documents ----------------------------------------------------------------------------
+    def attention_plan(self, q_lengths: Sequence[int], k_lengths: Optional[Sequence[int]] = None, causal: bool = False,
+                       prefix: Optional[Sequence[int]] = None) -> "AttentionPlan":
+        """The packing of a batch: document d has ``q_lengths[d]`` query rows and ``k_lengths[d]`` key rows (default: the same),
+        one behind the other in the tensors.  ``causal``: the last query row stands at the last key, every row sees the keys up to
+        its own; ``prefix``: the first ``prefix[d]`` keys of a document are visible to all its rows besides.  Lengths are host
+        data (lists, arrays, CPU tensors).  Build it once per batch and use it for every layer, forward and backward."""
+        return AttentionPlan(self, q_lengths, k_lengths, causal, prefix)
+
+    def _attention_dims(self, plan, q, k, v, scale, cap, slopes):
+        if not isinstance(plan, AttentionPlan) or plan.device != self.device:
+            raise ValueError("plan must come from attention_plan() of these operators")
+        dt = self._dtype("q", q)
+        _rows("q", q, self.device, dt)
+        _rows("k", k, self.device, dt)
+        _rows("v", v, self.device, dt)
+        if k.shape != v.shape or q.shape[2] != k.shape[2]:
+            raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: k and v must have one shape and q's head size")
+        if q.shape[0] < plan.q_rows or k.shape[0] < plan.k_rows:
+            raise ValueError(f"the plan covers {plan.q_rows} query and {plan.k_rows} key rows, the tensors have {q.shape[0]} and {k.shape[0]}")
+        if k.shape[1] < 1 or q.shape[1] % k.shape[1] or q.shape[1] < 1:
+            raise ValueError(f"{q.shape[1]} query heads are not a multiple of {k.shape[1]} key heads")
+        d = _capi.Attention()
+        d.dtype, d.head_dim, d.q_heads, d.k_heads = DTYPES[dt], q.shape[2], q.shape[1], k.shape[1]
+        d.scale = q.shape[2] ** -0.5 if scale is None else scale
+        d.cap = cap
+        return d, _vector("slopes", slopes, q.shape[1], torch.float32, self.device)
+
+    def attention(self, plan, q, k, v, scale: Optional[float] = None, cap: float = 0.0, slopes=None, out=None, lse=None):
+        """-> (o, lse).  q (rows, query heads, head_dim), k and v (rows, key heads, head_dim); query head h reads key head
+        ``h // (query heads / key heads)``.  Scores ``scale q.k`` (default ``head_dim ** -0.5``), ``cap``: ``cap tanh(score / cap)``,
+        ``slopes`` (fp32 per query head): minus ``slope * distance``.  lse (rows, query heads), fp32, natural log.  A row that sees no
+        key gives zeros and -inf.  Rows behind the last document are left as they were in ``out`` / ``lse`` and are zeros in tensors
+        allocated here.  head_dim: a multiple of 8 up to 128."""
+        d, sl = self._attention_dims(plan, q, k, v, scale, cap, slopes)
+        tail = q.shape[0] > plan.q_rows
+        new = torch.zeros if tail else torch.empty
+        if out is None:
+            out = new(q.shape, dtype=q.dtype, device=self.device)
+        o = self._output("out", out, q.shape, q.dtype)
+        if lse is None:
+            lse = new(q.shape[:2], dtype=torch.float32, device=self.device)
+        elif lse.shape != q.shape[:2] or lse.dtype != torch.float32 or lse.device != self.device or not lse.is_contiguous():
+            raise ValueError(f"lse must be a contiguous float32 tensor of shape {tuple(q.shape[:2])} on {self.device}")
+        q, k, v = _wide(q), _wide(k), _wide(v)
+        ow = o if _is_wide(o) else torch.empty_like(q, memory_format=torch.contiguous_format)
+        if ow is not o:
+            ow.copy_(o)
+        d.q_stride[:], d.k_stride[:], d.v_stride[:], d.o_stride[:] = _st(q), _st(k), _st(v), _st(ow)
+        with self._on_device():
+            rc = self.lib.dof_attention_forward(C.byref(plan.record), plan.table.data_ptr(), C.byref(d), q.data_ptr(), k.data_ptr(),
+                                                v.data_ptr(), sl, ow.data_ptr(), lse.data_ptr(), self._stream())
+        _capi.check(self.lib, rc, "dof_attention_forward")
+        if ow is not o:
+            o.copy_(ow)
+        return o, lse
+
+    def attention_backward(self, plan, do, q, k, v, o, lse, scale: Optional[float] = None, cap: float = 0.0, slopes=None):
+        """-> (dq, dk, dv) from the gradient at ``o`` and the forward's inputs and results; zeros in rows of no document.  The same
+        bits on every run.  ``slopes`` are constants: they get no gradient.  float16: small gradients keep their precision down to
+        about 1e-6 of the scores' gradient; scale the loss for smaller ones, as in any float16 training."""
+        d, sl = self._attention_dims(plan, q, k, v, scale, cap, slopes)
+        for name, t in (("do", do), ("o", o)):
+            _rows(name, t, self.device, q.dtype)
+            if t.shape != q.shape:
+                raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(q.shape)}")
+        if lse.shape != q.shape[:2] or lse.dtype != torch.float32 or lse.device != self.device or not lse.is_contiguous():
+            raise ValueError(f"lse must be a contiguous float32 tensor of shape {tuple(q.shape[:2])} on {self.device}")
+        new_q = torch.zeros if q.shape[0] > plan.q_rows else torch.empty
+        new_k = torch.zeros if k.shape[0] > plan.k_rows else torch.empty
+        dq = new_q(q.shape, dtype=q.dtype, device=self.device)
+        dk, dv = (new_k(k.shape, dtype=q.dtype, device=self.device) for _ in range(2))
+        q, k, v, do, o = _wide(q), _wide(k), _wide(v), _wide(do), _wide(o)
+        d.q_stride[:], d.k_stride[:], d.v_stride[:], d.o_stride[:], d.g_stride[:] = _st(q), _st(k), _st(v), _st(o), _st(do)
+        d.dq_stride[:], d.dk_stride[:], d.dv_stride[:] = _st(dq), _st(dk), _st(dv)
+        ws = torch.empty(self._bytes("dof_attention_workspace_bytes", plan.q_rows, q.shape[1]), dtype=torch.uint8, device=self.device)
+        with self._on_device():
+            rc = self.lib.dof_attention_backward(C.byref(plan.record), plan.table.data_ptr(), C.byref(d), do.data_ptr(), q.data_ptr(),
+                                                 k.data_ptr(), v.data_ptr(), sl, o.data_ptr(), lse.data_ptr(), dq.data_ptr(),
+                                                 dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), self._stream())
+        _capi.check(self.lib, rc, "dof_attention_backward")
+        return dq, dk, dv
+
+    def _bytes(self, fn: str, *args) -> int:
+        n = getattr(self.lib, fn)(*args)
+        if n < 0:
+            _capi.check(self.lib, -1, fn)
+        return n
+
+
+def create_attention_ops(device=None) -> AttentionOps:
+    """Product entry: requires a ROCm GPU and the compiled HIP library (no fallback)."""
+    from ._lib import load_hip_library
+
+    if not torch.cuda.is_available():
+        raise RuntimeError("deepof_amd needs a ROCm GPU (torch.cuda.is_available() is False); there is no CPU path")
+    lib = load_hip_library()
+    dev = torch.device(device if device is not None else f"cuda:{torch.cuda.current_device()}")
+    if dev.type != "cuda":
+        raise RuntimeError(f"deepof_amd runs on ROCm devices only, got {dev}")
+    return AttentionOps(lib, dev)

@@ -1,0 +1,274 @@
+// Host side of the attention operators: the plan of a packed batch and the C-ABI entry points of the forward and backward passes.
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <new>
+#include <vector>
+
+#include "deepof_hip.h"
+#include "dof_rt.h"
+#include "launchers.h"
+#include "seq_attn_args.h"
+
+namespace {
+
+constexpr int64_t kMaxRows = 1 << 30;  // of one document
+
+int check_plan_args(int32_t n_docs, const int64_t* q_off, const int64_t* k_off, const void* out) {
+  if (n_docs < 0 || (n_docs > 0 && (!q_off || !k_off)) || !out) {
+    dof_set_error("dof_attn_plan: bad argument (n_docs %d)", (int)n_docs);
+    return DOF_ERR_ARG;
+  }
+  for (int32_t i = 0; i < n_docs; ++i) {
+    const int64_t lq = q_off[i + 1] - q_off[i], lk = k_off[i + 1] - k_off[i];
+    if (q_off[i] < 0 || k_off[i] < 0 || lq < 0 || lk < 0 || lq > kMaxRows || lk > kMaxRows) {
+      dof_set_error("dof_attn_plan: the offsets of document %d do not rise (or it has more than 2^30 rows)", (int)i);
+      return DOF_ERR_ARG;
+    }
+  }
+  return DOF_OK;
+}
+
+struct Listed {
+  DofAttnTile tile;
+  int64_t work;
+};
+
+// keys visible to row i, as dof_attn_kend
+int64_t kend(int64_t lq, int64_t lk, int64_t prefix, int causal, int64_t i) {
+  if (!causal) return lk;
+  return std::max<int64_t>(0, std::min(lk, std::max(prefix, i + lk - lq + 1)));
+}
+
+void list_tiles(const DofAttnPlan* p, const int64_t* q_off, const int64_t* k_off, const int32_t* prefix, bool keys, int rows,
+                std::vector<Listed>* out) {
+  for (int32_t d = 0; d < p->n_docs; ++d) {
+    const int64_t lq = q_off[d + 1] - q_off[d], lk = k_off[d + 1] - k_off[d];
+    const int64_t pre = prefix ? std::max(0, prefix[d]) : 0;
+    for (int64_t r = 0; r < (keys ? lk : lq); r += rows) {
+      Listed e;
+      e.tile.q0 = q_off[d];
+      e.tile.k0 = k_off[d];
+      e.tile.lq = (int32_t)lq;
+      e.tile.lk = (int32_t)lk;
+      e.tile.prefix = (int32_t)std::min(pre, lk);
+      e.tile.row0 = (int32_t)r;
+      if (keys) e.work = !p->causal || r < pre ? lq : lq - std::min(lq, std::max<int64_t>(0, r - (lk - lq)));
+      else e.work = kend(lq, lk, pre, p->causal, std::min(r + rows, lq) - 1);
+      out->push_back(e);
+    }
+  }
+  std::stable_sort(out->begin(), out->end(), [](const Listed& a, const Listed& b) { return a.work > b.work; });
+}
+
+int64_t count_tiles(int32_t n_docs, const int64_t* off, int rows) {
+  int64_t n = 0;
+  for (int32_t i = 0; i < n_docs; ++i) n += (off[i + 1] - off[i] + rows - 1) / rows;
+  return n;
+}
+
+bool aligned(const void* p, const int64_t* s, int size) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && s[0] * size % 16 == 0 && s[1] * size % 16 == 0;
+}
+
+int check(const DofAttnPlan* p, const void* table, const DofAttention* d, const char* who) {
+  if (!p || !d || (!table && p->table_bytes > 0)) {
+    dof_set_error("%s: null plan, table or descriptor", who);
+    return DOF_ERR_ARG;
+  }
+  if (d->dtype < DOF_DTYPE_F32 || d->dtype > DOF_DTYPE_F16) {
+    dof_set_error("%s: unknown dtype %d", who, (int)d->dtype);
+    return DOF_ERR_ARG;
+  }
+  if (d->head_dim < 8 || d->head_dim > 128 || d->head_dim % 8) {
+    dof_set_error("%s: head_dim %d (multiples of 8 from 8 to 128 are supported)", who, (int)d->head_dim);
+    return DOF_ERR_UNSUPPORTED;
+  }
+  if (d->k_heads < 1 || d->q_heads < d->k_heads || d->q_heads % d->k_heads) {
+    dof_set_error("%s: %d query heads are not a multiple of %d key heads", who, (int)d->q_heads, (int)d->k_heads);
+    return DOF_ERR_ARG;
+  }
+  if (!std::isfinite(d->scale) || !std::isfinite(d->cap) || d->cap < 0.0f) {
+    dof_set_error("%s: scale and cap must be finite, cap not negative", who);
+    return DOF_ERR_ARG;
+  }
+  for (int i = 0; i < 4; ++i)
+    if (p->n_tiles[i] < 0 || p->n_tiles[i] * d->q_heads > 0x7FFFFFFF) {
+      dof_set_error("%s: too many tiles for one launch (%lld tiles, %d heads)", who, (long long)p->n_tiles[i], (int)d->q_heads);
+      return DOF_ERR_UNSUPPORTED;
+    }
+  return DOF_OK;
+}
+
+// list 0: query tiles of 128 rows, 1: of 32; 2, 3: key tiles
+const DofAttnTile* list_at(const DofAttnPlan* p, const void* table, int list) {
+  const DofAttnTile* t = static_cast<const DofAttnTile*>(table);
+  for (int i = 0; i < list; ++i) t += p->n_tiles[i];
+  return t;
+}
+
+// Tiles of 128 rows (four wavefronts share the staged keys) unless the documents are so short that most of such a tile is empty, or
+// there are so few of them that most CUs would go without work.
+int flat_tiles(const DofAttnPlan* p, int which, int heads) {
+  const int64_t tall = p->n_tiles[which], flat = p->n_tiles[which + 1];
+  return flat * 2 < tall * 5 || (tall * heads < 256 && flat > tall);
+}
+
+DofAttnFwd forward_args(const DofAttention* d, const void* q, const void* k, const void* v, const float* slopes, void* o, float* lse) {
+  DofAttnFwd A;
+  memset(&A, 0, sizeof(A));
+  A.q_heads = d->q_heads;
+  A.k_heads = d->k_heads;
+  A.dim = d->head_dim;
+  A.slopes = slopes;
+  if (d->cap > 0.0f) {
+    A.score.mul = d->scale / d->cap;
+    A.score.cap_l2 = d->cap * kLog2e;
+  } else {
+    A.score.mul = d->scale * kLog2e;
+  }
+  A.q = q;
+  A.k = k;
+  A.v = v;
+  A.o = o;
+  A.lse = lse;
+  for (int i = 0; i < 2; ++i) {
+    A.qs[i] = d->q_stride[i];
+    A.ks[i] = d->k_stride[i];
+    A.vs[i] = d->v_stride[i];
+    A.os[i] = d->o_stride[i];
+  }
+  return A;
+}
+
+int set_tiles(DofAttnFwd* A, const DofAttnPlan* p, const void* table, int which, int flat) {
+  A->causal = p->causal;
+  A->n_tiles = (int32_t)p->n_tiles[which + flat];
+  A->tiles = list_at(p, table, which + flat);
+  return A->n_tiles;
+}
+
+}  // namespace
+
+extern "C" int dof_attn_plan_size(int32_t n_docs, const int64_t* q_off, const int64_t* k_off, int32_t causal, DofAttnPlan* plan) {
+  const int rc = check_plan_args(n_docs, q_off, k_off, plan);
+  if (rc != DOF_OK) return rc;
+  plan->n_docs = n_docs;
+  plan->causal = causal != 0;
+  plan->n_tiles[0] = count_tiles(n_docs, q_off, kAttnTall);
+  plan->n_tiles[1] = count_tiles(n_docs, q_off, kAttnFlat);
+  plan->n_tiles[2] = count_tiles(n_docs, k_off, kAttnTall);
+  plan->n_tiles[3] = count_tiles(n_docs, k_off, kAttnFlat);
+  plan->table_bytes = 0;
+  for (int i = 0; i < 4; ++i) plan->table_bytes += plan->n_tiles[i] * (int64_t)sizeof(DofAttnTile);
+  return DOF_OK;
+}
+
+extern "C" int dof_attn_plan_table(const DofAttnPlan* plan, const int64_t* q_off, const int64_t* k_off, const int32_t* prefix,
+                                   void* table) {
+  if (!plan) {
+    dof_set_error("dof_attn_plan_table: null plan");
+    return DOF_ERR_ARG;
+  }
+  DofAttnPlan again;
+  const int rc = dof_attn_plan_size(plan->n_docs, q_off, k_off, plan->causal, &again);
+  if (rc != DOF_OK) return rc;
+  if (memcmp(again.n_tiles, plan->n_tiles, sizeof(again.n_tiles)) || again.table_bytes != plan->table_bytes) {
+    dof_set_error("dof_attn_plan_table: the offsets are not those the plan was sized for");
+    return DOF_ERR_ARG;
+  }
+  if (plan->table_bytes == 0) return DOF_OK;
+  if (!table) {
+    dof_set_error("dof_attn_plan_table: null table");
+    return DOF_ERR_ARG;
+  }
+  try {
+    DofAttnTile* out = static_cast<DofAttnTile*>(table);
+    for (int i = 0; i < 4; ++i) {
+      std::vector<Listed> list;
+      list.reserve((size_t)plan->n_tiles[i]);
+      list_tiles(plan, q_off, k_off, prefix, i >= 2, i % 2 ? kAttnFlat : kAttnTall, &list);
+      for (const Listed& e : list) *out++ = e.tile;
+    }
+  } catch (const std::bad_alloc&) {
+    dof_set_error("dof_attn_plan_table: out of host memory");
+    return DOF_ERR_STATE;
+  }
+  return DOF_OK;
+}
+
+extern "C" int dof_attention_forward(const DofAttnPlan* plan, const void* table, const DofAttention* d, const void* q, const void* k,
+                                     const void* v, const float* slopes, void* o, float* lse, void* stream) {
+  int rc = check(plan, table, d, "dof_attention_forward");
+  if (rc != DOF_OK) return rc;
+  if (plan->n_tiles[0] == 0) return DOF_OK;
+  const bool keys = plan->n_tiles[2] > 0;  // documents without any key need no k and v
+  if (!q || !o || !lse || (keys && (!k || !v))) {
+    dof_set_error("dof_attention_forward: null tensor");
+    return DOF_ERR_ARG;
+  }
+  const int size = d->dtype == DOF_DTYPE_F32 ? 4 : 2;
+  if (!aligned(q, d->q_stride, size) || !aligned(k, d->k_stride, size) || !aligned(v, d->v_stride, size) || !aligned(o, d->o_stride, size)) {
+    dof_set_error("dof_attention_forward: tensors and strides must be multiples of 16 bytes");
+    return DOF_ERR_UNSUPPORTED;
+  }
+  DofAttnFwd A = forward_args(d, q, k, v, slopes, o, lse);
+  const int flat = flat_tiles(plan, 0, d->q_heads);
+  set_tiles(&A, plan, table, 0, flat);
+  return dof_launch_attn_fwd(A, d->dtype, flat, (hipStream_t)stream);
+}
+
+extern "C" int64_t dof_attention_workspace_bytes(int64_t query_rows, int32_t q_heads) {
+  if (query_rows < 0 || q_heads < 1) {
+    dof_set_error("dof_attention_workspace_bytes: bad sizes");
+    return -1;
+  }
+  return query_rows * q_heads * 4;
+}
+
+extern "C" int dof_attention_backward(const DofAttnPlan* plan, const void* table, const DofAttention* d, const void* g, const void* q,
+                                      const void* k, const void* v, const float* slopes, const void* o, const float* lse, void* dq,
+                                      void* dk, void* dv, void* workspace, void* stream) {
+  int rc = check(plan, table, d, "dof_attention_backward");
+  if (rc != DOF_OK) return rc;
+  const bool rows = plan->n_tiles[0] > 0, keys = plan->n_tiles[2] > 0;
+  if (!rows && !keys) return DOF_OK;
+  if ((rows && (!g || !q || !o || !lse || !dq || !workspace)) || (keys && (!k || !v || !dk || !dv))) {
+    dof_set_error("dof_attention_backward: null tensor");
+    return DOF_ERR_ARG;
+  }
+  const int size = d->dtype == DOF_DTYPE_F32 ? 4 : 2;
+  if (!aligned(q, d->q_stride, size) || !aligned(k, d->k_stride, size) || !aligned(v, d->v_stride, size) || !aligned(o, d->o_stride, size) ||
+      !aligned(g, d->g_stride, size) || !aligned(dq, d->dq_stride, size) || !aligned(dk, d->dk_stride, size) ||
+      !aligned(dv, d->dv_stride, size)) {
+    dof_set_error("dof_attention_backward: tensors and strides must be multiples of 16 bytes");
+    return DOF_ERR_UNSUPPORTED;
+  }
+  DofAttnBwd B;
+  memset(&B, 0, sizeof(B));
+  B.f = forward_args(d, q, k, v, slopes, const_cast<void*>(o), const_cast<float*>(lse));
+  B.g = g;
+  B.delta = static_cast<float*>(workspace);
+  B.scale = d->scale;
+  B.dq = dq;
+  B.dk = dk;
+  B.dv = dv;
+  for (int i = 0; i < 2; ++i) {
+    B.gs[i] = d->g_stride[i];
+    B.dqs[i] = d->dq_stride[i];
+    B.dks[i] = d->dk_stride[i];
+    B.dvs[i] = d->dv_stride[i];
+  }
+  if (rows) {
+    const int flat = flat_tiles(plan, 0, d->q_heads);
+    set_tiles(&B.f, plan, table, 0, flat);
+    rc = dof_launch_attn_dq(B, d->dtype, flat, (hipStream_t)stream);
+    if (rc != DOF_OK) return rc;
+  }
+  if (keys) {
+    const int flat = flat_tiles(plan, 2, d->k_heads);
+    set_tiles(&B.f, plan, table, 2, flat);
+    rc = dof_launch_attn_dkv(B, d->dtype, flat, (hipStream_t)stream);
+  }
+  return rc;
+}

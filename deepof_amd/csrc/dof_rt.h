@@ -102,6 +102,59 @@ __device__ __forceinline__ void dof_split3x4(const float (&v)[4], uint32_t (&out
   out[2][0] = dof_pack_hi16(r2[0], r2[1]); out[2][1] = dof_pack_hi16(r2[2], r2[3]);
 }
 
+// ---- 16-bit element types of the sequence operators (norm_rope, attention, attention_step) --------------------------
+// v_mfma_f32_32x32x16_f16 / v_mfma_f32_16x16x32_f16 have the operand and result layouts of their bf16 forms above.
+// v_mfma_f32_32x32x2_f32: operand of lane l = row / column l & 31, k = l >> 5; result layout of the 32x32x16 form.
+#ifdef DOF_EMU
+#define DOF_MFMA_32x32x16_F16(a, b, c) emu_mfma_32x32x16_f16((a), (b), (c))
+#define DOF_MFMA_16x16x32_F16(a, b, c) emu_mfma_16x16x32_f16((a), (b), (c))
+#define DOF_MFMA_32x32x2_F32(a, b, c) emu_mfma_32x32x2((a), (b), (c))
+typedef emu_bf16x8 dof_f16x8;  // eight raw 16-bit values
+#else
+typedef _Float16 dof_f16x8 __attribute__((ext_vector_type(8)));
+#define DOF_MFMA_32x32x16_F16(a, b, c) __builtin_amdgcn_mfma_f32_32x32x16_f16((a), (b), (c), 0, 0, 0)
+#define DOF_MFMA_16x16x32_F16(a, b, c) __builtin_amdgcn_mfma_f32_16x16x32_f16((a), (b), (c), 0, 0, 0)
+#define DOF_MFMA_32x32x2_F32(a, b, c) __builtin_amdgcn_mfma_f32_32x32x2f32((a), (b), (c), 0, 0, 0)
+#endif
+__device__ __forceinline__ float dof_bf16_to_f32(uint32_t lo16) { return __builtin_bit_cast(float, lo16 << 16); }
+// two fp32 values rounded to nearest even as packed 16-bit words (first argument in the low half)
+#ifdef DOF_EMU
+__device__ __forceinline__ uint32_t dof_pack_bf16(float a, float b) { return emu_f32_to_bf16(a) | ((uint32_t)emu_f32_to_bf16(b) << 16); }
+__device__ __forceinline__ uint32_t dof_pack_f16(float a, float b) { return emu_f32_to_f16(a) | ((uint32_t)emu_f32_to_f16(b) << 16); }
+__device__ __forceinline__ float dof_f16_to_f32(uint32_t lo16) { return emu_f16_to_f32((uint16_t)lo16); }
+__device__ __forceinline__ float dof_exp2(float x) { return exp2f(x); }
+__device__ __forceinline__ float dof_log2(float x) { return log2f(x); }
+// value of lane ^ 32 (the other half of the wavefront)
+__device__ __forceinline__ float dof_swap32(float v) { return __shfl_xor(v, 32); }
+__device__ __forceinline__ bool dof_wave_any(bool p) { return emu_any(p); }
+__device__ __forceinline__ void dof_sincos_turns(double turns, float* s, float* c) {
+  const double r = (turns - rint(turns)) * 6.283185307179586477;
+  *s = (float)sin(r);
+  *c = (float)cos(r);
+}
+#else
+__device__ __forceinline__ uint32_t dof_pack_bf16(float a, float b) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const bf16x2 v = {(__bf16)a, (__bf16)b};
+  return __builtin_bit_cast(uint32_t, v);
+}
+__device__ __forceinline__ uint32_t dof_pack_f16(float a, float b) {
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  const f16x2 v = {(_Float16)a, (_Float16)b};
+  return __builtin_bit_cast(uint32_t, v);
+}
+__device__ __forceinline__ float dof_f16_to_f32(uint32_t lo16) { return (float)__builtin_bit_cast(_Float16, (uint16_t)lo16); }
+__device__ __forceinline__ float dof_exp2(float x) { return __builtin_amdgcn_exp2f(x); }  // v_exp_f32, 1 ulp, denormals to 0
+__device__ __forceinline__ float dof_log2(float x) { return __builtin_amdgcn_logf(x); }   // v_log_f32, 1 ulp
+__device__ __forceinline__ float dof_swap32(float v) { return __shfl_xor(v, 32); }
+__device__ __forceinline__ bool dof_wave_any(bool p) { return __any(p); }
+// sin and cos of `turns` revolutions: the reduction to half a turn is exact enough in 64 bits for any 32-bit position, what is
+// left (at most half a turn) is a 32-bit argument in units of pi
+__device__ __forceinline__ void dof_sincos_turns(double turns, float* s, float* c) {
+  sincospif((float)((turns - rint(turns)) * 2.0), s, c);
+}
+#endif
+
 // 1: the HIP runtime is underneath (RCCL can be opened); 0: the host-only emulation build
 #ifdef DOF_EMU
 #define DOF_HAS_DEVICE_RUNTIME 0

@@ -1,0 +1,335 @@
+// Attention over packed documents, backward: two kernels that recompute the probabilities from the forward's log-sum-exp.
+//
+//   p = exp(s - lse) ; dp_ij = g_i.v_j ; ds = p (dp - delta_i) c_ij, delta_i = sum_d g_id o_id, c = 1 - tanh^2 under a cap, else 1
+//   dq_i = scale sum_j ds_ij k_j        (k_attn_dq:  a workgroup per query tile, walks the keys as the forward does)
+//   dv_j = sum_i p_ij g_i, dk_j = scale sum_i ds_ij q_i   (k_attn_dkv: a workgroup per key tile, walks the query rows that see it,
+//                                                          through all query heads of its group)
+//
+// Every gradient element is summed by one workgroup in a fixed order: no atomics, the same bits on every run.  The price is that S
+// and dP are computed twice (seven products of the size of S instead of five).  Both kernels keep their own rows' operands in
+// registers and stream the other side through LDS (two images); the second products take P and dS straight from the registers the
+// first ones left them in, as in the forward.  P and dS are rounded to the elements' type for their products; everything that is
+// summed is fp32.  fp16 has 5 exponent bits: there P is carried as 2^12 P and dS as 2^6 dS (exact factors, taken out at the end), so
+// that weights of long documents and small gradients stay out of its subnormals.
+#include <cmath>
+
+#include "deepof_hip.h"
+#include "dof_rt.h"
+#include "launchers.h"
+#include "seq_attn.h"
+#include "seq_attn_args.h"
+
+namespace {
+
+constexpr int kRows = 32;  // query rows per step of the dk / dv kernel
+
+template <class T> struct Lift {
+  static constexpr float p2 = 0.0f, p = 1.0f, ds = 1.0f;  // log2 of P's factor, P's factor, dS's factor
+};
+template <> struct Lift<DofF16> {
+  static constexpr float p2 = 12.0f, p = 4096.0f, ds = 64.0f;
+};
+
+template <class T, int DP, int NW>
+__global__ void __launch_bounds__(64 * NW) k_attn_dq(DofAttnBwd B) {
+  const DofAttnFwd& A = B.f;
+  constexpr int KU = NW == 1 ? 1 : 2, kKeys = 32 * KU;  // keys per step, as in the forward
+  using Tile = DofTile<T, kKeys, DP>;
+  using Stage = DofStage<T, kKeys, DP, 64 * NW>;
+  __shared__ Tile sk[2], sv[2];
+  constexpr int KS = DP / 16, DT = DP / 32;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+  const int64_t item = dof_xcd_item(blockIdx.x, (int64_t)A.n_tiles * A.q_heads);
+  const int h = (int)(item / A.n_tiles);
+  const DofAttnTile t = A.tiles[item - (int64_t)h * A.n_tiles];
+  const int hk = h / (A.q_heads / A.k_heads);
+
+  const int first = t.row0 + 32 * wave, row = first + col;
+  const bool live = row < t.lq;
+  const int last_wg = (t.row0 + 32 * NW < t.lq ? t.row0 + 32 * NW : t.lq) - 1;
+  const int last = (first + 32 < t.lq ? first + 32 : t.lq) - 1;
+  const int kmax = dof_attn_kend(t, A.causal, last_wg);
+  const int wmax = first < t.lq ? dof_attn_kend(t, A.causal, last) : 0;
+  const int wmin = first < t.lq ? dof_attn_kend(t, A.causal, first) : 0;
+  const int kend = live ? dof_attn_kend(t, A.causal, row) : 0;
+  const int pos = row + t.lk - t.lq;
+  DofScore sc = A.score;
+  if (A.slopes) sc.slope_l2 = A.slopes[h] * kLog2e;
+
+  DofFrag<T> q[KS], g[KS];
+  const T* qp = static_cast<const T*>(A.q) + (t.q0 + row) * A.qs[0] + h * A.qs[1];
+  const T* gp = static_cast<const T*>(B.g) + (t.q0 + row) * B.gs[0] + h * B.gs[1];
+  const T* op = static_cast<const T*>(A.o) + (t.q0 + row) * A.os[0] + h * A.os[1];
+  float delta = 0.0f;
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int e = 16 * s + 8 * half;
+    q[s] = g[s] = dof_frag_zero<T>();
+    if (live && e < A.dim) {
+      q[s] = dof_frag_load<T>(qp + e);
+      g[s] = dof_frag_load<T>(gp + e);
+      float a[8], b[8];
+      dof_frag_unpack<T>(g[s], a);
+      dof_frag_unpack<T>(dof_frag_load<T>(op + e), b);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) delta = fmaf(a[i], b[i], delta);
+    }
+  }
+  delta += dof_swap32(delta);
+  const int64_t srow = (t.q0 + row) * A.q_heads + h;
+  if (live && half == 0) B.delta[srow] = delta;
+  float lse2 = live ? A.lse[srow] * kLog2e : 0.0f;
+  if (lse2 == -INFINITY) lse2 = 0.0f;  // a row without keys: every score is masked below
+  lse2 -= Lift<T>::p2;
+  const T* kp = static_cast<const T*>(A.k) + t.k0 * A.ks[0] + hk * A.ks[1];
+  const T* vp = static_cast<const T*>(A.v) + t.k0 * A.vs[0] + hk * A.vs[1];
+
+  dof_f32x16 dq[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d) dq[d] = dof_zero16();
+  Stage rk, rv;
+  if (kmax > 0) {
+    rk.load(kp, A.ks[0], t.lk, A.dim, tid);
+    rv.load(vp, A.vs[0], t.lk, A.dim, tid);
+    rk.store(sk[0], tid);
+    rv.store(sv[0], tid);
+  }
+  for (int j0 = 0, buf = 0; j0 < kmax; j0 += kKeys, buf ^= 1) {
+    __syncthreads();
+    const int next = j0 + kKeys;
+    if (next < kmax) {
+      rk.load(kp + next * A.ks[0], A.ks[0], t.lk - next, A.dim, tid);
+      rv.load(vp + next * A.vs[0], A.vs[0], t.lk - next, A.dim, tid);
+    }
+    if (j0 < wmax) {
+      const bool partial = j0 + kKeys > wmin;
+#pragma unroll
+      for (int u = 0; u < KU; ++u) {
+        dof_f32x16 x = dof_zero16(), y = dof_zero16();
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          x = dof_mma32<T>(sk[buf].rowfrag(32 * u + col, 2 * s + half), q[s], x);
+          y = dof_mma32<T>(sv[buf].rowfrag(32 * u + col, 2 * s + half), g[s], y);
+        }
+        float ds[16];
+        const float base = (float)(pos - j0 - 32 * u - 4 * half);
+        const int left = kend - j0 - 32 * u - 4 * half;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const int r = 8 * (v / 4) + v % 4;
+          float c = Lift<T>::ds / Lift<T>::p, w;
+          if (sc.cap_l2 != 0.0f) {
+            const float th = dof_cap_tanh<T>(x[v] * sc.mul);
+            w = sc.cap_l2 * th;
+            c *= 1.0f - th * th;
+          } else {
+            w = x[v] * sc.mul;
+          }
+          if (A.slopes) w -= sc.slope_l2 * fabsf(base - (float)r);
+          float p = dof_exp2(w - lse2);
+          if (partial && r >= left) p = 0.0f;
+          ds[v] = p * c * (y[v] - delta);
+          if (partial && r >= left) ds[v] = 0.0f;  // not 0 x (what a masked key holds)
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const DofFrag<T> f = dof_frag_pack<T>(ds + 8 * s);
+          const int r = 32 * u + 16 * s + 4 * half;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) dq[d] = dof_mma32<T>(sk[buf].colfrag(r, r + 8, 32 * d + col), f, dq[d]);
+        }
+      }
+    }
+    if (next < kmax) {
+      rk.store(sk[buf ^ 1], tid);
+      rv.store(sv[buf ^ 1], tid);
+    }
+  }
+  if (!live) return;
+  const float out = B.scale / Lift<T>::ds;
+  T* dqp = static_cast<T*>(B.dq) + (t.q0 + row) * B.dqs[0] + h * B.dqs[1];
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int v = 0; v < 16; v += 4) {
+      const int e = 32 * d + 2 * v + 4 * half;
+      if (e < A.dim) {
+        const float r[4] = {dq[d][v] * out, dq[d][v + 1] * out, dq[d][v + 2] * out, dq[d][v + 3] * out};
+        dof_store_vec<T, 4>(dqp + e, r);
+      }
+    }
+}
+
+template <class T, int DP, int NW>
+__global__ void __launch_bounds__(64 * NW) k_attn_dkv(DofAttnBwd B) {
+  const DofAttnFwd& A = B.f;
+  using Tile = DofTile<T, kRows, DP>;
+  using Stage = DofStage<T, kRows, DP, 64 * NW>;
+  __shared__ Tile sq[2], sg[2];
+  __shared__ float sl[2][kRows], sd[2][kRows];  // log-sum-exp in units of log 2 (+inf: the row takes no part), delta
+  constexpr int KS = DP / 16, DT = DP / 32;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+  const int64_t item = dof_xcd_item(blockIdx.x, (int64_t)A.n_tiles * A.k_heads);
+  const int hk = (int)(item / A.n_tiles);
+  const DofAttnTile t = A.tiles[item - (int64_t)hk * A.n_tiles];
+  const int group = A.q_heads / A.k_heads;
+  const int off = t.lk - t.lq;
+
+  const int first = t.row0 + 32 * wave, key = first + col;
+  const bool live = key < t.lk;
+  // the first query row that sees any key of the workgroup (of the wavefront): keys below the prefix are seen by all, key j by the
+  // rows from j - off on
+  auto row_from = [&](int j) {
+    if (!A.causal || j < t.prefix) return 0;
+    return j - off > 0 ? j - off : 0;
+  };
+  const int i_lo = row_from(t.row0) & ~(kRows - 1);
+  const int w_lo = first < t.lk ? row_from(first) : t.lq;
+  // from this row on, every row sees every key of the wavefront
+  const int last_key = first + 31 < t.lk ? first + 31 : t.lk - 1;
+  const int w_full = row_from(last_key);
+
+  DofFrag<T> kf[KS], vf[KS];
+  const T* kp = static_cast<const T*>(A.k) + (t.k0 + key) * A.ks[0] + hk * A.ks[1];
+  const T* vp = static_cast<const T*>(A.v) + (t.k0 + key) * A.vs[0] + hk * A.vs[1];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int e = 16 * s + 8 * half;
+    kf[s] = vf[s] = dof_frag_zero<T>();
+    if (live && e < A.dim) {
+      kf[s] = dof_frag_load<T>(kp + e);
+      vf[s] = dof_frag_load<T>(vp + e);
+    }
+  }
+  dof_f32x16 dk[DT], dv[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d) dk[d] = dv[d] = dof_zero16();
+
+  Stage rq, rg;
+  float rl = 0.0f, rd = 0.0f;
+  const int per_head = t.lq > i_lo ? (t.lq - i_lo + kRows - 1) / kRows : 0;
+  const int steps = per_head * group;
+  auto load = [&](int step) {
+    const int h = hk * group + step / per_head, i0 = i_lo + (step % per_head) * kRows;
+    rq.load(static_cast<const T*>(A.q) + (t.q0 + i0) * A.qs[0] + h * A.qs[1], A.qs[0], t.lq - i0, A.dim, tid);
+    rg.load(static_cast<const T*>(B.g) + (t.q0 + i0) * B.gs[0] + h * B.gs[1], B.gs[0], t.lq - i0, A.dim, tid);
+    if (tid < kRows) {
+      rl = INFINITY;
+      rd = 0.0f;
+      if (i0 + tid < t.lq) {
+        const int64_t srow = (t.q0 + i0 + tid) * A.q_heads + h;
+        rl = A.lse[srow] * kLog2e;
+        rd = B.delta[srow];
+        rl = rl == -INFINITY ? INFINITY : rl - Lift<T>::p2;
+      }
+    }
+  };
+  auto store = [&](int buf) {
+    rq.store(sq[buf], tid);
+    rg.store(sg[buf], tid);
+    if (tid < kRows) {
+      sl[buf][tid] = rl;
+      sd[buf][tid] = rd;
+    }
+  };
+  if (steps > 0) {
+    load(0);
+    store(0);
+  }
+  for (int step = 0, buf = 0; step < steps; ++step, buf ^= 1) {
+    __syncthreads();
+    if (step + 1 < steps) load(step + 1);
+    const int i0 = i_lo + (step % per_head) * kRows;
+    if (i0 + kRows > w_lo) {
+      DofScore sc = A.score;
+      if (A.slopes) sc.slope_l2 = A.slopes[hk * group + step / per_head] * kLog2e;
+      dof_f32x16 x = dof_zero16(), y = dof_zero16();
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        x = dof_mma32<T>(sq[buf].rowfrag(col, 2 * s + half), kf[s], x);
+        y = dof_mma32<T>(sg[buf].rowfrag(col, 2 * s + half), vf[s], y);
+      }
+      float p[16], ds[16];
+      const bool partial = i0 < w_full;
+      const float base = (float)(i0 + off + 4 * half - key);
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        const int r = 8 * (v / 4) + v % 4;
+        float c = Lift<T>::ds / Lift<T>::p, w;
+        if (sc.cap_l2 != 0.0f) {
+          const float th = dof_cap_tanh<T>(x[v] * sc.mul);
+          w = sc.cap_l2 * th;
+          c *= 1.0f - th * th;
+        } else {
+          w = x[v] * sc.mul;
+        }
+        if (A.slopes) w -= sc.slope_l2 * fabsf(base + (float)r);
+        p[v] = dof_exp2(w - sl[buf][r + 4 * half]);
+        ds[v] = p[v] * c * (y[v] - sd[buf][r + 4 * half]);
+        if (partial && key >= dof_attn_kend(t, A.causal, i0 + r + 4 * half)) p[v] = ds[v] = 0.0f;
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const DofFrag<T> pf = dof_frag_pack<T>(p + 8 * s), df = dof_frag_pack<T>(ds + 8 * s);
+        const int r = 16 * s + 4 * half;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          dv[d] = dof_mma32<T>(sg[buf].colfrag(r, r + 8, 32 * d + col), pf, dv[d]);
+          dk[d] = dof_mma32<T>(sq[buf].colfrag(r, r + 8, 32 * d + col), df, dk[d]);
+        }
+      }
+    }
+    if (step + 1 < steps) store(buf ^ 1);
+  }
+  if (!live) return;
+  T* dkp = static_cast<T*>(B.dk) + (t.k0 + key) * B.dks[0] + hk * B.dks[1];
+  T* dvp = static_cast<T*>(B.dv) + (t.k0 + key) * B.dvs[0] + hk * B.dvs[1];
+  const float ok = B.scale / Lift<T>::ds, ov = 1.0f / Lift<T>::p;
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int v = 0; v < 16; v += 4) {
+      const int e = 32 * d + 2 * v + 4 * half;
+      if (e < A.dim) {
+        const float a[4] = {dk[d][v] * ok, dk[d][v + 1] * ok, dk[d][v + 2] * ok, dk[d][v + 3] * ok};
+        const float b[4] = {dv[d][v] * ov, dv[d][v + 1] * ov, dv[d][v + 2] * ov, dv[d][v + 3] * ov};
+        dof_store_vec<T, 4>(dkp + e, a);
+        dof_store_vec<T, 4>(dvp + e, b);
+      }
+    }
+}
+
+template <class T, int DP>
+void launch_dq(const DofAttnBwd& B, int flat, hipStream_t stream) {
+  const unsigned blocks = (unsigned)((int64_t)B.f.n_tiles * B.f.q_heads);
+  if (flat) DOF_LAUNCH((k_attn_dq<T, DP, 1>), (blocks, 1, 1), (64, 1, 1), stream, B);
+  else DOF_LAUNCH((k_attn_dq<T, DP, 4>), (blocks, 1, 1), (256, 1, 1), stream, B);
+}
+template <class T, int DP>
+void launch_dkv(const DofAttnBwd& B, int flat, hipStream_t stream) {
+  const unsigned blocks = (unsigned)((int64_t)B.f.n_tiles * B.f.k_heads);
+  if (flat) DOF_LAUNCH((k_attn_dkv<T, DP, 1>), (blocks, 1, 1), (64, 1, 1), stream, B);
+  else DOF_LAUNCH((k_attn_dkv<T, DP, 4>), (blocks, 1, 1), (256, 1, 1), stream, B);
+}
+
+}  // namespace
+
+int dof_launch_attn_dq(const DofAttnBwd& B, int dtype, int flat, hipStream_t stream) {
+  DOF_SEQ_DISPATCH(dtype, T, {
+    if (B.f.dim <= 32) launch_dq<T, 32>(B, flat, stream);
+    else if (B.f.dim <= 64) launch_dq<T, 64>(B, flat, stream);
+    else if (B.f.dim <= 96) launch_dq<T, 96>(B, flat, stream);
+    else launch_dq<T, 128>(B, flat, stream);
+  });
+  return dof_check_launch("k_attn_dq");
+}
+
+int dof_launch_attn_dkv(const DofAttnBwd& B, int dtype, int flat, hipStream_t stream) {
+  DOF_SEQ_DISPATCH(dtype, T, {
+    if (B.f.dim <= 32) launch_dkv<T, 32>(B, flat, stream);
+    else if (B.f.dim <= 64) launch_dkv<T, 64>(B, flat, stream);
+    else if (B.f.dim <= 96) launch_dkv<T, 96>(B, flat, stream);
+    else launch_dkv<T, 128>(B, flat, stream);
+  });
+  return dof_check_launch("k_attn_dkv");
+}

@@ -1,0 +1,218 @@
+// Attention over packed documents, forward.
+//
+//   s_ij = scale q_i.k_j ; s = cap tanh(s / cap) ; s -= slope |pos_i - j| ; softmax over the visible keys ; o_i = sum_j p_ij v_j
+//
+// A workgroup owns a tile of query rows of one document and head (32 rows per wavefront) and walks the document's visible keys, 64
+// at a time, with a running maximum and sum; K and V pass through LDS (two images, the next one's loads in flight under the present
+// one's products).  The products are transposed -- S^T = K Q^T, O^T = V^T P^T -- so that a lane owns one query: its maximum, sum and
+// rescaling are lane-local but for one exchange with the other half-wavefront, and P^T leaves the first product in just the registers
+// the second one wants it in (the key order inside a fragment is permuted, the same on both operands).  V^T is read from row-major
+// LDS by the transposing LDS read.  Statistics and accumulators are fp32; P is rounded to the elements' type for its product (relative
+// half a step per weight, as the inputs' own), the sum l is taken of the unrounded weights.
+#include <cmath>
+
+#include "deepof_hip.h"
+#include "dof_rt.h"
+#include "launchers.h"
+#include "seq_attn.h"
+#include "seq_attn_args.h"
+
+namespace {
+
+// keys per step: 64; a single wavefront stages a tile alone and takes 32, which fit its registers
+template <class T, int DP, int NW>
+__global__ void __launch_bounds__(64 * NW) k_attn_fwd(DofAttnFwd A) {
+  constexpr int KU = NW == 1 ? 1 : 2, kKeys = 32 * KU;
+  using Tile = DofTile<T, kKeys, DP>;
+  using Stage = DofStage<T, kKeys, DP, 64 * NW>;
+  __shared__ Tile sk[2], sv[2];
+  constexpr int KS = DP / 16, DT = DP / 32;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+  const int64_t item = dof_xcd_item(blockIdx.x, (int64_t)A.n_tiles * A.q_heads);
+  const int h = (int)(item / A.n_tiles);
+  const DofAttnTile t = A.tiles[item - (int64_t)h * A.n_tiles];
+  const int hk = h / (A.q_heads / A.k_heads);
+
+  const int first = t.row0 + 32 * wave, row = first + col;
+  const bool live = row < t.lq;
+  const int last_wg = (t.row0 + 32 * NW < t.lq ? t.row0 + 32 * NW : t.lq) - 1;
+  const int last = (first + 32 < t.lq ? first + 32 : t.lq) - 1;
+  const int kmax = dof_attn_kend(t, A.causal, last_wg);                          // of the workgroup
+  const int wmax = first < t.lq ? dof_attn_kend(t, A.causal, last) : 0;          // of the wavefront
+  const int wmin = first < t.lq ? dof_attn_kend(t, A.causal, first) : 0;         // keys that all its rows see
+  const int kend = live ? dof_attn_kend(t, A.causal, row) : 0;
+  const int pos = row + t.lk - t.lq;
+  DofScore sc = A.score;
+  if (A.slopes) sc.slope_l2 = A.slopes[h] * kLog2e;
+
+  DofFrag<T> q[KS];
+  const T* qp = static_cast<const T*>(A.q) + (t.q0 + row) * A.qs[0] + h * A.qs[1];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int e = 16 * s + 8 * half;
+    q[s] = dof_frag_zero<T>();
+    if (live && e < A.dim) q[s] = dof_frag_load<T>(qp + e);
+  }
+  const T* kp = static_cast<const T*>(A.k) + t.k0 * A.ks[0] + hk * A.ks[1];
+  const T* vp = static_cast<const T*>(A.v) + t.k0 * A.vs[0] + hk * A.vs[1];
+
+  dof_f32x16 o[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d) o[d] = dof_zero16();
+  float m = -INFINITY, l = 0.0f;
+
+  Stage rk, rv;
+  if (kmax > 0) {
+    rk.load(kp, A.ks[0], t.lk, A.dim, tid);
+    rv.load(vp, A.vs[0], t.lk, A.dim, tid);
+    rk.store(sk[0], tid);
+    rv.store(sv[0], tid);
+  }
+  for (int j0 = 0, buf = 0; j0 < kmax; j0 += kKeys, buf ^= 1) {
+    __syncthreads();
+    const int next = j0 + kKeys;
+    if (next < kmax) {
+      rk.load(kp + next * A.ks[0], A.ks[0], t.lk - next, A.dim, tid);
+      rv.load(vp + next * A.vs[0], A.vs[0], t.lk - next, A.dim, tid);
+    }
+    if (j0 < wmax) {
+      dof_f32x16 x[KU];
+#pragma unroll
+      for (int u = 0; u < KU; ++u) {
+        x[u] = dof_zero16();
+#pragma unroll
+        for (int s = 0; s < KS; ++s) x[u] = dof_mma32<T>(sk[buf].rowfrag(32 * u + col, 2 * s + half), q[s], x[u]);
+      }
+      if (sc.cap_l2 != 0.0f) {
+#pragma unroll
+        for (int u = 0; u < KU; ++u)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) x[u][v] = sc.cap_l2 * dof_cap_tanh<T>(x[u][v] * sc.mul);
+      } else {
+#pragma unroll
+        for (int u = 0; u < KU; ++u)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) x[u][v] *= sc.mul;
+      }
+      if (A.slopes) {
+        const float base = (float)(pos - j0 - 4 * half);
+#pragma unroll
+        for (int u = 0; u < KU; ++u)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) x[u][v] -= sc.slope_l2 * fabsf(base - (float)(32 * u + 8 * (v / 4) + v % 4));
+      }
+      if (j0 + kKeys > wmin) {
+        const int left = kend - j0 - 4 * half;
+#pragma unroll
+        for (int u = 0; u < KU; ++u)
+#pragma unroll
+          for (int v = 0; v < 16; ++v)
+            if (32 * u + 8 * (v / 4) + v % 4 >= left) x[u][v] = -INFINITY;
+      }
+      float mt = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < KU; ++u)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) mt = fmaxf(mt, x[u][v]);
+      mt = fmaxf(mt, dof_swap32(mt));
+      // The running maximum follows only when a tile's exceeds it by 2^8: until then the weights stay below 256, which costs the
+      // fp32 sums nothing, and the accumulators need no rescaling pass.
+      if (dof_wave_any(mt > m + 8.0f)) {
+        const float mn = fmaxf(m, mt);
+        const float a = mn == -INFINITY ? 1.0f : dof_exp2(m - mn);
+        m = mn;
+        l *= a;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) o[d][v] *= a;
+      }
+      const float mm = m == -INFINITY ? 0.0f : m;
+      // In a tile that some rows see only in part, a hidden key's weight is zero, but zero times an infinity or NaN in V is not:
+      // such values (rare, so looked for in these tiles only) are taken out of the product and put where they are seen.
+      bool careful = false;
+      if ((j0 > wmin ? j0 : wmin) < (next < t.lk ? next : t.lk)) {
+        bool bad = false;
+#pragma unroll
+        for (int r = 0; r < kKeys; r += 16)
+#pragma unroll
+          for (int d = 0; d < DT; ++d) bad |= dof_frag_nonfinite<T>(sv[buf].colfrag(r + 4 * half, r + 8 + 4 * half, 32 * d + col));
+        careful = dof_wave_any(bad);
+      }
+#pragma unroll
+      for (int u = 0; u < KU; ++u) {
+        float p[16];
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          p[v] = dof_exp2(x[u][v] - mm);
+          l += p[v];
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const DofFrag<T> pf = dof_frag_pack<T>(p + 8 * s);
+          const int r = 32 * u + 16 * s + 4 * half;
+          if (!careful) {
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[d] = dof_mma32<T>(sv[buf].colfrag(r, r + 8, 32 * d + col), pf, o[d]);
+          } else {
+            float seen[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) seen[e] = j0 + r + e + (e < 4 ? 0 : 4) < kend ? 1.0f : 0.0f;
+            const DofFrag<T> sf = dof_frag_pack<T>(seen);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+              DofFrag<T> f = sv[buf].colfrag(r, r + 8, 32 * d + col), pos_f, neg_f;
+              dof_frag_split<T>(f, pos_f, neg_f);
+              o[d] = dof_mma32<T>(f, pf, o[d]);
+              const dof_f32x16 up = dof_mma32<T>(pos_f, sf, dof_zero16()), down = dof_mma32<T>(neg_f, sf, dof_zero16());
+#pragma unroll
+              for (int v = 0; v < 16; ++v) {
+                if (up[v] > 0.0f) o[d][v] += INFINITY;
+                if (down[v] > 0.0f) o[d][v] -= INFINITY;
+              }
+            }
+          }
+        }
+      }
+    }
+    if (next < kmax) {
+      rk.store(sk[buf ^ 1], tid);
+      rv.store(sv[buf ^ 1], tid);
+    }
+  }
+
+  l += dof_swap32(l);
+  if (!live) return;
+  const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // no visible key: zeros; NaN stays NaN
+  T* op = static_cast<T*>(A.o) + (t.q0 + row) * A.os[0] + h * A.os[1];
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int v = 0; v < 16; v += 4) {
+      const int e = 32 * d + 2 * v + 4 * half;
+      if (e < A.dim) {
+        const float r[4] = {o[d][v] * inv, o[d][v + 1] * inv, o[d][v + 2] * inv, o[d][v + 3] * inv};
+        dof_store_vec<T, 4>(op + e, r);
+      }
+    }
+  if (half == 0) A.lse[(t.q0 + row) * A.q_heads + h] = l == 0.0f ? -INFINITY : (m + dof_log2(l)) * kLn2;
+}
+
+template <class T, int DP>
+void launch(const DofAttnFwd& A, int flat, hipStream_t stream) {
+  const unsigned blocks = (unsigned)((int64_t)A.n_tiles * A.q_heads);
+  if (flat) DOF_LAUNCH((k_attn_fwd<T, DP, 1>), (blocks, 1, 1), (64, 1, 1), stream, A);
+  else DOF_LAUNCH((k_attn_fwd<T, DP, 4>), (blocks, 1, 1), (256, 1, 1), stream, A);
+}
+
+}  // namespace
+
+int dof_launch_attn_fwd(const DofAttnFwd& A, int dtype, int flat, hipStream_t stream) {
+  DOF_SEQ_DISPATCH(dtype, T, {
+    if (A.dim <= 32) launch<T, 32>(A, flat, stream);
+    else if (A.dim <= 64) launch<T, 64>(A, flat, stream);
+    else if (A.dim <= 96) launch<T, 96>(A, flat, stream);
+    else launch<T, 128>(A, flat, stream);
+  });
+  return dof_check_launch("k_attn_fwd");
+}

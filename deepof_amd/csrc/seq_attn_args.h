@@ -1,0 +1,27 @@
+// Arguments of the attention kernels' launchers (k_attn_fwd.hip, k_attn_bwd.hip), filled by attention.hip.
+#pragma once
+#include "seq_attn.h"
+
+struct DofAttnFwd {
+  const DofAttnTile* tiles;
+  int32_t n_tiles, q_heads, k_heads, dim, causal;
+  DofScore score;
+  const float* slopes;  // per query head, NULL: no bias
+  const void *q, *k, *v;
+  void* o;
+  float* lse;           // (query rows, q_heads)
+  int64_t qs[2], ks[2], vs[2], os[2];  // row and head strides
+};
+
+struct DofAttnBwd {
+  DofAttnFwd f;          // f.tiles: query tiles (dq kernel) or key tiles (dk / dv kernel); f.o and f.lse are read
+  const void* g;         // gradient at o
+  float* delta;          // (query rows, q_heads): sum of g o over a row, written by the dq kernel, read by the dk / dv kernel
+  float scale;           // d(score) / d(q.k) without the cap
+  void *dq, *dk, *dv;
+  int64_t gs[2], dqs[2], dks[2], dvs[2];
+};
+
+int dof_launch_attn_fwd(const DofAttnFwd& A, int dtype, int flat, hipStream_t stream);
+int dof_launch_attn_dq(const DofAttnBwd& A, int dtype, int flat, hipStream_t stream);
+int dof_launch_attn_dkv(const DofAttnBwd& A, int dtype, int flat, hipStream_t stream);

@@ -1,0 +1,204 @@
+// Matrix fragments and LDS tiles of the attention kernels (see seq_types.h for the element types).
+#pragma once
+#include "seq_types.h"
+
+// Eight k values of one row, as a lane supplies them to a 32x32x16 or 16x16x32 product.
+template <class T> struct DofFrag { uint32_t w[4]; };
+template <> struct DofFrag<float> { float v[8]; };
+
+template <class T> __device__ __forceinline__ DofFrag<T> dof_frag_zero() {
+  DofFrag<T> f;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f.v[i] = 0.0f;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f.w[i] = 0u;
+  }
+  return f;
+}
+// eight elements at a 16-byte aligned address
+template <class T> __device__ __forceinline__ DofFrag<T> dof_frag_load(const T* p) {
+  DofFrag<T> f;
+  if constexpr (sizeof(T) == 4) {
+    const DofWords<4> a = *reinterpret_cast<const DofWords<4>*>(p), b = *reinterpret_cast<const DofWords<4>*>(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f.v[i] = __builtin_bit_cast(float, a.w[i]);
+      f.v[4 + i] = __builtin_bit_cast(float, b.w[i]);
+    }
+  } else {
+    const DofWords<4> a = *reinterpret_cast<const DofWords<4>*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f.w[i] = a.w[i];
+  }
+  return f;
+}
+// eight fp32 values as a fragment; 16-bit types: rounded to nearest even
+template <class T> __device__ __forceinline__ DofFrag<T> dof_frag_pack(const float* v) {
+  DofFrag<T> f;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f.v[i] = v[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f.w[i] = DofElem<T>::pack2(v[2 * i], v[2 * i + 1]);
+  }
+  return f;
+}
+template <class T> __device__ __forceinline__ void dof_frag_unpack(const DofFrag<T>& f, float* v) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = f.v[i];
+  } else {
+    DofWords<4> w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w.w[i] = f.w[i];
+    DofElem<T>::unpack(w, v);
+  }
+}
+
+// Infinities and NaN inside a fragment.  any: is there one; split: the fragment with zeros in their places, and two fragments of ones
+// where +inf or NaN (pos) and where -inf or NaN (neg) stood.
+template <class T> __device__ __forceinline__ bool dof_frag_nonfinite(const DofFrag<T>& f) {
+  bool bad = false;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) bad |= (__builtin_bit_cast(uint32_t, f.v[i]) & 0x7F800000u) == 0x7F800000u;
+  } else {
+    constexpr uint32_t e = std::is_same<T, DofBf16>::value ? 0x7F80u : 0x7C00u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bad |= (f.w[i] & e) == e || (f.w[i] & (e << 16)) == (e << 16);
+  }
+  return bad;
+}
+template <class T> __device__ __forceinline__ void dof_frag_split(DofFrag<T>& f, DofFrag<T>& pos, DofFrag<T>& neg) {
+  float v[8], a[8], b[8];
+  dof_frag_unpack<T>(f, v);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const bool bad = !(fabsf(v[i]) < INFINITY);
+    a[i] = bad && !(v[i] < 0.0f) ? 1.0f : 0.0f;
+    b[i] = bad && !(v[i] > 0.0f) ? 1.0f : 0.0f;
+    v[i] = bad ? 0.0f : v[i];
+  }
+  f = dof_frag_pack<T>(v);
+  pos = dof_frag_pack<T>(a);
+  neg = dof_frag_pack<T>(b);
+}
+
+// c (32 x 32) += a (32 x 16) b (16 x 32); register v of lane l: row 8 (v / 4) + 4 (l >> 5) + v % 4, column l & 31
+template <class T> __device__ __forceinline__ dof_f32x16 dof_mma32(const DofFrag<T>& a, const DofFrag<T>& b, dof_f32x16 c) {
+  if constexpr (std::is_same<T, DofBf16>::value) {
+    return DOF_MFMA_32x32x16_BF16(__builtin_bit_cast(dof_bf16x8, a), __builtin_bit_cast(dof_bf16x8, b), c);
+  } else if constexpr (std::is_same<T, DofF16>::value) {
+    return DOF_MFMA_32x32x16_F16(__builtin_bit_cast(dof_f16x8, a), __builtin_bit_cast(dof_f16x8, b), c);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c = DOF_MFMA_32x32x2_F32(a.v[e], b.v[e], c);
+    return c;
+  }
+}
+// c (16 x 16) += a (16 x 32) b (32 x 16); register r of lane l: row 4 (l >> 4) + r, column l & 15
+template <class T> __device__ __forceinline__ dof_f32x4 dof_mma16(const DofFrag<T>& a, const DofFrag<T>& b, dof_f32x4 c) {
+  if constexpr (std::is_same<T, DofBf16>::value) {
+    return DOF_MFMA_16x16x32_BF16(__builtin_bit_cast(dof_bf16x8, a), __builtin_bit_cast(dof_bf16x8, b), c);
+  } else if constexpr (std::is_same<T, DofF16>::value) {
+    return DOF_MFMA_16x16x32_F16(__builtin_bit_cast(dof_f16x8, a), __builtin_bit_cast(dof_f16x8, b), c);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[e], b.v[e], c, 0, 0, 0);
+    return c;
+  }
+}
+__device__ __forceinline__ dof_f32x16 dof_zero16() {
+  dof_f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.0f;
+  return z;
+}
+__device__ __forceinline__ dof_f32x4 dof_zero4() {
+  dof_f32x4 z;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) z[i] = 0.0f;
+  return z;
+}
+
+// An LDS image of ROWS rows x DP elements, read both ways: eight consecutive elements of a row (rowfrag, the operand whose k runs
+// along the row) and eight rows of one column (colfrag, the operand whose k runs down the rows).
+//
+// 16-bit elements: unpadded rows of CH = DP / 8 chunks of 16 bytes, the chunk index XORed with a function of the row, so that both
+// readings are free of bank conflicts: sixteen consecutive rows of one chunk (ds_read_b128) and the four rows x four chunks of a
+// transposing read (ds_read_b64_tr_b16) each fall into sixteen different 16-byte slots of the 256-byte bank line.
+// fp32: rows padded by 16 bytes, columns read as single words.
+template <class T, int ROWS, int DP> struct DofTile {
+  static constexpr int EPC = 16 / (int)sizeof(T);  // elements per chunk
+  static constexpr int CH = DP / EPC;              // chunks per row
+  static constexpr int kStride = sizeof(T) == 4 ? DP + 4 : DP;  // elements per row in LDS
+  alignas(16) unsigned char mem[ROWS * kStride * (int)sizeof(T)];
+
+  __device__ __forceinline__ static int offset(int row, int chunk) {  // bytes
+    if constexpr (sizeof(T) == 4) return (row * kStride + chunk * EPC) * 4;
+    int x = (row >> 2) & 3;
+    if constexpr (CH % 16 == 0) x |= (row & 3) << 2;
+    else if constexpr (CH % 8 == 0) x |= ((row >> 1) & 1) << 2;
+    return (row * CH + (chunk ^ x)) * 16;
+  }
+  __device__ __forceinline__ void put(int row, int chunk, const DofWords<4>& v) {
+    *reinterpret_cast<DofWords<4>*>(mem + offset(row, chunk)) = v;
+  }
+  // elements 8 k8 .. 8 k8 + 7 of a row
+  __device__ __forceinline__ DofFrag<T> rowfrag(int row, int k8) const {
+    DofFrag<T> f;
+    if constexpr (sizeof(T) == 4) {
+      return dof_frag_load<T>(reinterpret_cast<const T*>(mem + offset(row, 2 * k8)));
+    } else {
+      const DofWords<4> v = *reinterpret_cast<const DofWords<4>*>(mem + offset(row, k8));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f.w[i] = v.w[i];
+      return f;
+    }
+  }
+  // column `col` (16-bit: all 16 lanes of an aligned group read the 16 columns of one aligned block) of the rows ra .. ra + 3 and
+  // rb .. rb + 3 (multiples of 4, the same over the group)
+  __device__ __forceinline__ DofFrag<T> colfrag(int ra, int rb, int col) const {
+    DofFrag<T> f;
+    if constexpr (sizeof(T) == 4) {
+      const float* m = reinterpret_cast<const float*>(mem);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f.v[i] = m[(ra + i) * kStride + col];
+        f.v[4 + i] = m[(rb + i) * kStride + col];
+      }
+    } else {
+      const int q = (int)(threadIdx.x & 15), r = q >> 2, c = (col >> 4) * 2 + ((q & 3) >> 1), b = (q & 1) * 8;
+      dof_lds_tr16(reinterpret_cast<const uint16_t*>(mem + offset(ra + r, c) + b), f.w[0], f.w[1]);
+      dof_lds_tr16(reinterpret_cast<const uint16_t*>(mem + offset(rb + r, c) + b), f.w[2], f.w[3]);
+    }
+    return f;
+  }
+};
+
+// Rows of a tensor on their way into a tile: load() issues the global loads into registers, store() puts them into LDS, so the
+// loads of the next tile run under the products of the present one.  Rows from `rows` and elements from `dim` on are zeros.
+template <class T, int ROWS, int DP, int NT> struct DofStage {
+  using Tile = DofTile<T, ROWS, DP>;
+  static constexpr int N = (ROWS * Tile::CH + NT - 1) / NT;
+  DofWords<4> reg[N];
+  __device__ __forceinline__ void load(const T* base, int64_t stride, int rows, int dim, int tid) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int e = tid + i * NT, r = e / Tile::CH, c = e - r * Tile::CH;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) reg[i].w[k] = 0u;
+      if (r < rows && c * Tile::EPC < dim) reg[i] = *reinterpret_cast<const DofWords<4>*>(base + r * stride + c * Tile::EPC);
+    }
+  }
+  __device__ __forceinline__ void store(Tile& t, int tid) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int e = tid + i * NT, r = e / Tile::CH, c = e - r * Tile::CH;
+      if ((ROWS * Tile::CH) % NT == 0 || r < ROWS) t.put(r, c, reg[i]);
+    }
+  }
+};

@@ -480,6 +480,69 @@ int dof_comm_abort(DofComm* comm);
 int dof_flat_allreduce(DofComm* comm, float* buf, int64_t n, void* stream);
 int dof_comm_broadcast(DofComm* comm, float* buf, int64_t n, int32_t root, void* stream);
 
+/* ---- sequence operators: what a transformer over recordings is made of ------------------------------------------
+ * Stand-alone operators next to the transformer family's plans: fp32, bf16 or fp16 elements, ordinary head sizes, packed
+ * recordings of any length.  Tensors are (rows, heads, head_dim) with the elements of a head side by side and the row and head
+ * strides given in elements; nothing is allocated or synchronised.  Where a call takes a workspace, its memory is the call's own
+ * until the stream has passed it: calls that may run at the same time (two streams, two captured graphs) need one each. */
+enum { DOF_DTYPE_F32 = 0, DOF_DTYPE_BF16 = 1, DOF_DTYPE_F16 = 2 };
+
+/* RMS norm of every query / key head (weights fp32, NULL = no norm) and rotation by its position, in one pass.
+ * head_dim even, at most 256; the first rot_dim elements (even, 0 = none) are rotated: pair p by positions[row] * freqs[p] radians
+ * (freqs: rot_dim / 2 float64 on the device).  interleaved 0: the pairs lie rot_dim / 2 apart, 1: side by side.  The outputs may be
+ * the inputs' own memory (same strides).  Backward: gq / gk are the gradients at the outputs, q / k the forward's inputs (their
+ * values are read only where a norm needs them); q_out_stride / k_out_stride are dq's / dk's strides; dq_weight / dk_weight
+ * (head_dim fp32, overwritten, NULL with the weight) sum over all rows and heads in a fixed order. */
+typedef struct {
+  int32_t dtype, head_dim, rot_dim, interleaved;
+  int32_t q_heads, k_heads;
+  int64_t tokens;
+  float eps;
+  int32_t reserved;
+  int64_t q_stride[2], k_stride[2];          /* (row, head) strides of q and k */
+  int64_t q_out_stride[2], k_out_stride[2];  /* of the outputs (backward: of dq and dk) */
+  int64_t gq_stride[2], gk_stride[2];        /* backward: of gq and gk */
+} DofNormRope;
+int dof_norm_rope_forward(const DofNormRope* dims, const void* q, const void* k, const int32_t* positions, const double* freqs,
+                          const float* q_weight, const float* k_weight, void* q_out, void* k_out, void* stream);
+int64_t dof_norm_rope_workspace_bytes(const DofNormRope* dims); /* of the backward call; -1: bad dims */
+int dof_norm_rope_backward(const DofNormRope* dims, const void* gq, const void* gk, const void* q, const void* k,
+                           const int32_t* positions, const double* freqs, const float* q_weight, const float* k_weight, void* dq,
+                           void* dk, float* dq_weight, float* dk_weight, void* workspace, void* stream);
+
+/* Attention over packed documents.  Document d owns the query rows q_off[d] .. q_off[d + 1] - 1 and the key rows k_off[d] ..; its
+ * rows see its own keys only.  causal: query row i of a document with lq rows and lk keys stands at key position i + lk - lq and
+ * sees the keys up to it; with a prefix (per document, NULL = none) every row also sees the keys below prefix[d].  A row without a
+ * visible key gives zeros and a log-sum-exp of -inf; rows of no document are neither read nor written.
+ * Scores: scale q.k; cap > 0: cap tanh(score / cap); then minus slopes[head] |i + lk - lq - j| (slopes: q_heads fp32 on the device,
+ * NULL = none; they are constants, no gradient).  Query head h reads key head h / (q_heads / k_heads).
+ *
+ * The plan is host work, once per batch shape: dof_attn_plan_size checks the offsets (host memory, n_docs + 1 each) and fills the
+ * record, dof_attn_plan_table writes table_bytes of tiles into host memory, the caller copies them to the device (16-byte
+ * aligned) and passes both to the calls.  A plan serves any head count, head size and dtype. */
+typedef struct {
+  int32_t n_docs, causal;
+  int64_t n_tiles[4];
+  int64_t table_bytes;
+} DofAttnPlan;
+int dof_attn_plan_size(int32_t n_docs, const int64_t* q_off, const int64_t* k_off, int32_t causal, DofAttnPlan* plan);
+int dof_attn_plan_table(const DofAttnPlan* plan, const int64_t* q_off, const int64_t* k_off, const int32_t* prefix, void* table);
+/* head_dim: multiples of 8 from 8 to 128; every tensor and stride a multiple of 16 bytes.  lse (fp32): (query rows, q_heads),
+ * natural log.  Backward: g is the gradient at o; o and lse are the forward's; the workspace holds
+ * dof_attention_workspace_bytes(highest query row + 1, q_heads).  Every gradient is summed in a fixed order (no atomics). */
+typedef struct {
+  int32_t dtype, head_dim, q_heads, k_heads;
+  float scale, cap;
+  int64_t q_stride[2], k_stride[2], v_stride[2], o_stride[2];     /* (row, head) strides */
+  int64_t g_stride[2], dq_stride[2], dk_stride[2], dv_stride[2];  /* backward */
+} DofAttention;
+int dof_attention_forward(const DofAttnPlan* plan, const void* table, const DofAttention* dims, const void* q, const void* k,
+                          const void* v, const float* slopes, void* o, float* lse, void* stream);
+int64_t dof_attention_workspace_bytes(int64_t query_rows, int32_t q_heads);
+int dof_attention_backward(const DofAttnPlan* plan, const void* table, const DofAttention* dims, const void* g, const void* q,
+                           const void* k, const void* v, const float* slopes, const void* o, const float* lse, void* dq, void* dk,
+                           void* dv, void* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -207,6 +207,105 @@ emu_f32x4 emu_mfma_16x16x32_bf16(emu_bf16x8 a, emu_bf16x8 b, emu_f32x4 c) {
   return c;
 }
 
+uint16_t emu_f32_to_bf16(float f) {
+  uint32_t u;
+  memcpy(&u, &f, 4);
+  if ((u & 0x7FFFFFFFu) > 0x7F800000u) return (uint16_t)((u >> 16) | 0x40);
+  return (uint16_t)((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);
+}
+
+float emu_f16_to_f32(uint16_t h) {
+  const int e = (h >> 10) & 31, m = h & 1023;
+  float v;
+  if (e == 31) v = m ? NAN : INFINITY;
+  else if (e == 0) v = ldexpf((float)m, -24);
+  else v = ldexpf((float)(m | 1024), e - 25);
+  return (h & 0x8000) ? -v : v;
+}
+
+uint16_t emu_f32_to_f16(float f) {
+  uint32_t u;
+  memcpy(&u, &f, 4);
+  const uint16_t sign = (uint16_t)((u >> 16) & 0x8000);
+  const float a = fabsf(f);
+  if (std::isnan(f)) return sign | 0x7E00;
+  if (a == 0.0f) return sign;
+  if (a >= 65520.0f) return sign | 0x7C00;  // halfway to 2^16 and above
+  int e;
+  frexpf(a, &e);                            // a = m 2^e, m in [0.5, 1)
+  const int q = (e < -13 ? -13 : e) - 11;   // weight of the last kept bit: 2^q
+  const long long n = llrintf(ldexpf(a, -q));  // ties to even; exact scaling
+  if (q == -24 && n < 1024) return sign | (uint16_t)n;
+  const long long m = n == 2048 ? 1024 : n;
+  const int ex = (n == 2048 ? q + 1 : q) + 25;
+  return sign | (uint16_t)((ex << 10) + (int)(m - 1024));
+}
+
+bool emu_any(bool p) {
+  int me = g_cur;
+  int lane = me & 63, base = me - lane;
+  g_xchg[me * 2] = p ? 1.0f : 0.0f;
+  yield_as(WAIT_WAVE);
+  bool any = false;
+  for (int i = 0; i < 64; ++i)
+    if (base + i < (int)(blockDim.x * blockDim.y * blockDim.z) && g_fibers[base + i].st != DONE) any |= g_xchg[(base + i) * 2] != 0.0f;
+  yield_as(WAIT_WAVE);
+  return any;
+}
+
+namespace {
+template <int M, int K>
+float emu_f16_dot(int row_lane_base, int row, int col, float acc) {
+  for (int k = 0; k < K; ++k)
+    acc = fmaf(emu_f16_to_f32(g_xchg16[row_lane_base + (k / 8) * M + row][k % 8]),
+               emu_f16_to_f32(g_xchg16[row_lane_base + (k / 8) * M + col][8 + k % 8]), acc);
+  return acc;
+}
+}  // namespace
+
+emu_f32x16 emu_mfma_32x32x16_f16(emu_bf16x8 a, emu_bf16x8 b, emu_f32x16 c) {
+  int me = g_cur;
+  int lane = me & 63, base = me - lane;
+  for (int e = 0; e < 8; ++e) {
+    g_xchg16[me][e] = a.v[e];
+    g_xchg16[me][8 + e] = b.v[e];
+  }
+  yield_as(WAIT_WAVE);
+  for (int v = 0; v < 16; ++v) c[v] = emu_f16_dot<32, 16>(base, 8 * (v / 4) + 4 * (lane >> 5) + v % 4, lane & 31, c[v]);
+  yield_as(WAIT_WAVE);
+  return c;
+}
+
+emu_f32x4 emu_mfma_16x16x32_f16(emu_bf16x8 a, emu_bf16x8 b, emu_f32x4 c) {
+  int me = g_cur;
+  int lane = me & 63, base = me - lane;
+  for (int e = 0; e < 8; ++e) {
+    g_xchg16[me][e] = a.v[e];
+    g_xchg16[me][8 + e] = b.v[e];
+  }
+  yield_as(WAIT_WAVE);
+  for (int r = 0; r < 4; ++r) c[r] = emu_f16_dot<16, 32>(base, 4 * (lane >> 4) + r, lane & 15, c[r]);
+  yield_as(WAIT_WAVE);
+  return c;
+}
+
+emu_f32x16 emu_mfma_32x32x2(float a, float b, emu_f32x16 c) {
+  // A[m][k]: lane k*32+m ; B[k][n]: lane k*32+n ; D as 32x32x16
+  int me = g_cur;
+  int lane = me & 63, base = me - lane;
+  g_xchg[me * 2] = a;
+  g_xchg[me * 2 + 1] = b;
+  yield_as(WAIT_WAVE);
+  for (int v = 0; v < 16; ++v) {
+    const int row = 8 * (v / 4) + 4 * (lane >> 5) + v % 4, col = lane & 31;
+    float acc = c[v];
+    for (int k = 0; k < 2; ++k) acc = fmaf(g_xchg[(base + 32 * k + row) * 2], g_xchg[(base + 32 * k + col) * 2 + 1], acc);
+    c[v] = acc;
+  }
+  yield_as(WAIT_WAVE);
+  return c;
+}
+
 namespace {
 const uint16_t* g_trp[1024];  // per-thread run addresses of a transposing read
 }

@@ -1,0 +1,291 @@
+"""attention over packed documents, forward and backward, against the formulas in 64 bits; masks, orders, refusals, graphs."""
+import math
+
+import pytest
+import torch
+
+from sequence_common import DEVICES, DTYPES, TINY, U, U32, assert_within, draw, make_ops, strided
+
+
+def reference(q, k, v, g, q_lens, k_lens, causal, prefix, scale, cap, slopes, dtype):
+    """64-bit results and elementwise error bounds of o, lse, dq, dk, dv.
+
+    u = half a step of the element type.  Forward: a score is a chain of head_dim products in fp32 (error e_s below), a weight carries
+    that error relatively plus its rounding u, so o differs by at most sum_j p_j |v_j| (2 u + 2 e_s + 64 U32) plus its own rounding.
+    Backward: p and ds are rounded once for their products (u each), delta is taken from the rounded o (u |g||o|)."""
+    u = U[dtype]
+    low = u if dtype != torch.float32 else 0.0  # P and dS are rounded to the type; fp32 keeps them
+    hq, hk, d = q.shape[1], k.shape[1], q.shape[2]
+    grp = hq // hk
+    out = {n: torch.zeros_like(t) for n, t in (("o", q), ("dq", q), ("dk", k), ("dv", k))}
+    bound = {n: torch.zeros_like(t) for n, t in out.items()}
+    out["lse"] = torch.full(q.shape[:2], float("-inf"), dtype=torch.float64)
+    bound["lse"] = torch.zeros(q.shape[:2], dtype=torch.float64)
+    qa = ka = 0
+    for doc, (lq, lk) in enumerate(zip(q_lens, k_lens)):
+        i = torch.arange(lq).unsqueeze(1) + lk - lq
+        j = torch.arange(lk).unsqueeze(0)
+        vis = torch.ones(lq, lk, dtype=torch.bool)
+        if causal:
+            vis = j <= i
+            if prefix is not None:
+                vis = vis | (j < prefix[doc])
+        empty = ~vis.any(1) if lk else torch.ones(lq, dtype=torch.bool)
+        for h in range(hq):
+            Q, K, V, G = q[qa:qa + lq, h], k[ka:ka + lk, h // grp], v[ka:ka + lk, h // grp], g[qa:qa + lq, h]
+            if lk == 0 or lq == 0:
+                continue
+            raw = Q @ K.T * scale
+            es = (Q.abs() @ K.abs().T) * abs(scale) * (d / 8 + 8) * U32
+            c = torch.ones_like(raw)
+            s = raw
+            if cap:
+                t = torch.tanh(raw / cap)
+                c, s = 1 - t * t, cap * t
+                es = es + cap * 2.0 ** -21
+            if slopes is not None:
+                dist = slopes[h].double() * (i - j).abs()
+                s = s - dist
+                es = es + dist * 2 * U32
+            es = es + 4 * U32 * s.abs() + 8 * U32
+            s = s.masked_fill(~vis, float("-inf"))
+            m = s.amax(1, keepdim=True)
+            m = torch.where(m == float("-inf"), torch.zeros_like(m), m)
+            e = torch.exp(s - m)
+            l = e.sum(1, keepdim=True)
+            P = torch.where(empty[:, None], torch.zeros_like(e), e / l.clamp(min=1e-300))
+            es = torch.where(vis, es, torch.zeros_like(es)).amax(1, keepdim=True)  # of any score of the row
+            O = P @ V
+            rel = low + 2 * es + 64 * U32
+            sl = slice(qa, qa + lq)
+            out["o"][sl, h] = O
+            bound["o"][sl, h] = u * O.abs() + (1 + u) * rel * (P @ V.abs()) + TINY[dtype]
+            out["lse"][sl, h] = torch.where(empty, torch.full((lq,), -math.inf, dtype=torch.float64), (m + torch.log(l)).squeeze(1))
+            bound["lse"][sl, h] = (es + 64 * U32 + 4 * U32 * m.abs()).squeeze(1)
+            dP = G @ V.T
+            delta = (G * O).sum(1, keepdim=True)
+            dS = P * (dP - delta) * c
+            # errors of dS's factors: P (relative 3 es: through s and lse), dP and delta (fp32 chains; delta from the rounded o)
+            ddp = (G.abs() @ V.abs().T) * (d / 8 + 8) * U32
+            ddel = (G.abs() * (bound["o"][sl, h] + O.abs() * (d / 8) * U32)).sum(1, keepdim=True)
+            edS = P * c * (ddp + ddel) + (3 * es + 64 * U32) * dS.abs() + low * dS.abs()
+            if cap:  # 1 - tanh^2 carries an absolute error of 2 |tanh| (error of tanh)
+                edS = edS + P * (dP - delta).abs() * (2.0 ** -20 + 2 * es / cap)
+            if dtype == torch.float16:
+                edS = edS + 2.0 ** -25 / 64
+            dq, bq = dS @ K * scale, edS @ K.abs() * abs(scale)
+            out["dq"][sl, h] = dq
+            bound["dq"][sl, h] = u * dq.abs() + (1 + u) * bq + (dS.abs() @ K.abs()) * abs(scale) * (lk / 16 + 16) * U32 + TINY[dtype]
+            kl = slice(ka, ka + lk)
+            out["dk"][kl, h // grp] += dS.T @ Q * scale
+            bound["dk"][kl, h // grp] += edS.T @ Q.abs() * abs(scale) + (dS.abs().T @ Q.abs()) * abs(scale) * (grp * lq / 16 + 16) * U32
+            eP = (low + 3 * es + 64 * U32) * P + (2.0 ** -25 / 4096 if dtype == torch.float16 else 0.0)
+            out["dv"][kl, h // grp] += P.T @ G
+            bound["dv"][kl, h // grp] += eP.T @ G.abs() + (P.T @ G.abs()) * (grp * lq / 16 + 16) * U32
+        qa, ka = qa + lq, ka + lk
+    for n in ("dk", "dv"):
+        bound[n] = bound[n] * (1 + u) + u * out[n].abs() + TINY[dtype]
+    return out, bound
+
+
+# query lengths, key lengths (None: the same), query heads, key heads, head size, causal, prefix, cap, bias, memory order
+CASES = [
+    ([1], None, 1, 1, 8, False, None, 0.0, False, "plain"),
+    ([1], None, 4, 2, 64, True, None, 0.0, False, "plain"),
+    ([25, 25, 25], None, 4, 4, 16, False, None, 0.0, False, "packed"),
+    ([33, 1, 64, 31], None, 2, 1, 32, True, None, 0.0, True, "packed"),
+    ([70], None, 2, 2, 80, True, [20], 5.0, False, "head_major"),
+    ([40, 90], None, 3, 1, 128, True, [200, 0], 0.0, True, "plain"),
+    ([65, 130], None, 2, 2, 48, False, None, 8.0, True, "plain"),
+    ([5, 17], [70, 17], 2, 1, 24, True, None, 0.0, True, "plain"),     # more keys than rows: rows at the end
+    ([70, 9], [5, 0], 2, 1, 40, True, None, 0.0, False, "plain"),      # fewer keys than rows, and none: rows without any key
+    ([70], [5], 2, 2, 16, True, [3], 0.0, False, "plain"),             # ... whose prefix gives them some
+    ([0, 6, 0], [3, 6, 0], 1, 1, 16, False, None, 0.0, False, "plain"),  # keys without rows
+    ([130, 35], None, 2, 1, 96, True, None, 0.0, False, "odd"),
+]
+
+
+def build(case, dtype, device, seed=0, extra=0):
+    ql, kl, hq, hk, d, causal, prefix, cap, bias, how = case
+    kl = ql if kl is None else kl
+    gen = torch.Generator().manual_seed(seed)
+    nq, nk = sum(ql) + extra, sum(kl) + extra
+    t = dict(q=draw((nq, hq, d), dtype, gen), k=draw((nk, hk, d), dtype, gen), v=draw((nk, hk, d), dtype, gen), g=draw((nq, hq, d), dtype, gen))
+    slopes = torch.rand(hq, generator=gen) * 0.3 if bias else None
+    dev = {n: strided(x, device, how) for n, x in t.items()}
+    return t, dev, kl, slopes
+
+
+def run(ops, case, dev, kl, slopes, device):
+    ql, _, hq, hk, d, causal, prefix, cap, bias, how = case
+    plan = ops.attention_plan(ql, kl, causal=causal, prefix=prefix)
+    kw = dict(cap=cap, slopes=slopes.to(device) if slopes is not None else None)
+    o, lse = ops.attention(plan, dev["q"], dev["k"], dev["v"], **kw)
+    dq, dk, dv = ops.attention_backward(plan, dev["g"], dev["q"], dev["k"], dev["v"], o, lse, **kw)
+    return dict(o=o, lse=lse, dq=dq, dk=dk, dv=dv)
+
+
+def check(got, t, case, kl, slopes, dtype):
+    ql, _, hq, hk, d, causal, prefix, cap, bias, how = case
+    want, bound = reference(*(t[n].double() for n in "qkvg"), ql, kl, causal, prefix, d ** -0.5, cap, slopes, dtype)
+    empty = want["lse"] == -math.inf
+    assert torch.equal(got["lse"].cpu() == -math.inf, empty)
+    got, want = dict(got), dict(want)
+    got["lse"], want["lse"] = got["lse"].cpu().masked_fill(empty, 0.0), want["lse"].masked_fill(empty, 0.0)
+    for n in ("o", "lse", "dq", "dk", "dv"):
+        assert_within(n, got[n], want[n], bound[n])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("case", CASES, ids=str)
+def test_forward_and_backward(device, dtype, case):
+    ops = make_ops(device)
+    t, dev, kl, slopes = build(case, dtype, device)
+    check(run(ops, case, dev, kl, slopes, device), t, case, kl, slopes, dtype)
+
+
+LARGE = [
+    ([1500, 3, 700], None, 4, 2, 64, True, None, 0.0, True, "packed"),
+    ([2049], None, 3, 3, 128, True, [300], 20.0, False, "packed"),
+    ([25] * 300, None, 4, 4, 16, False, None, 0.0, False, "packed"),
+    ([600, 900], [1300, 40], 8, 1, 96, True, None, 0.0, False, "plain"),
+    ([1000], [1000], 8, 2, 72, False, None, 0.0, True, "plain"),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("case", LARGE, ids=lambda c: f"{len(c[0])}docs-{c[2]}x{c[3]}x{c[4]}")
+def test_long_documents(dtype, case):
+    ops = make_ops("cuda:0")
+    t, dev, kl, slopes = build(case, dtype, "cuda:0", seed=7)
+    got = run(ops, case, dev, kl, slopes, "cuda:0")
+    check(got, t, case, kl, slopes, dtype)
+    again = run(ops, case, dev, kl, slopes, "cuda:0")
+    assert all(torch.equal(got[n], again[n]) for n in got)  # a fixed order of every sum
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_rows_behind_the_last_document_stay(device):
+    """They are neither read (NaN there reaches nothing) nor written."""
+    ops = make_ops(device)
+    case = ([40, 21], None, 2, 1, 32, True, None, 0.0, False, "plain")
+    t, dev, kl, slopes = build(case, torch.bfloat16, device, extra=9)
+    for x in dev.values():
+        x[61:] = float("nan")
+    plan = ops.attention_plan([40, 21], causal=True)
+    out, lse = torch.full((70, 2, 32), 7.0, dtype=torch.bfloat16, device=device), torch.full((70, 2), 7.0, device=device)
+    o, l = ops.attention(plan, dev["q"], dev["k"], dev["v"], out=out, lse=lse)
+    assert o is out and l is lse and bool((out[61:] == 7).all()) and bool((lse[61:] == 7).all()) and bool(torch.isfinite(out.float()).all())
+    dq, dk, dv = ops.attention_backward(plan, dev["g"], dev["q"], dev["k"], dev["v"], out, lse)
+    for x in (dq, dk, dv):
+        assert bool((x[61:] == 0).all()) and bool(torch.isfinite(x.float()).all())
+    o2, l2 = ops.attention(plan, dev["q"], dev["k"], dev["v"])
+    assert torch.equal(o2[:61], out[:61]) and bool((o2[61:] == 0).all()) and bool((l2[61:] == 0).all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -3.0e38])
+def test_masked_places_reach_nothing(device, bad):
+    """Non-finite or huge values at keys that a row does not see -- later frames, other documents -- leave it as it was."""
+    ops = make_ops(device)
+    case = ([50, 90], None, 2, 1, 32, True, None, 0.0, False, "plain")
+    t, dev, kl, slopes = build(case, torch.float32, device)
+    plan = ops.attention_plan([50, 90], causal=True)
+    want, wl = ops.attention(plan, dev["q"], dev["k"], dev["v"])
+    k2, v2 = dev["k"].clone(), dev["v"].clone()
+    k2[30], v2[30] = bad, bad  # frame 30 of the first document
+    got, gl = ops.attention(plan, dev["q"], k2, v2)
+    for a, b in ((got, want), (gl, wl)):
+        assert torch.equal(a[:30], b[:30]) and torch.equal(a[50:], b[50:])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_gradient_against_differences(device):
+    ops = make_ops(device)
+    case = ([9, 6], None, 2, 1, 8, True, [2, 0], 3.0, True, "plain")
+    t, dev, kl, slopes = build(case, torch.float32, device, seed=5)
+    got = run(ops, case, dev, kl, slopes, device)
+    for name, grad in (("q", "dq"), ("k", "dk"), ("v", "dv")):
+        for e in ((0, 0, 0), (5, 0, 3), (12, 0, 7)):
+            vals = []
+            for h in (1e-5, -1e-5):
+                x = {n: a.double().clone() for n, a in t.items()}
+                x[name][e] += h
+                o = reference(x["q"], x["k"], x["v"], x["g"], case[0], kl, True, case[6], 8 ** -0.5, 3.0, slopes, torch.float32)[0]["o"]
+                vals.append(float((o * x["g"]).sum()))
+            num = (vals[0] - vals[1]) / 2e-5
+            assert abs(num - float(got[grad][e])) < 1e-4 * max(1.0, abs(num))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_refusals(device):
+    from deepof_amd._capi import DofError
+    ops = make_ops(device)
+    case = ([8, 4], None, 4, 2, 16, True, None, 0.0, False, "plain")
+    t, dev, kl, slopes = build(case, torch.float32, device)
+    plan = ops.attention_plan([8, 4], causal=True)
+    q, k, v, g = (dev[n] for n in "qkvg")
+    bad = [(plan, q.double(), k, v), (plan, q, k.half(), v), (plan, q, k, v[:, :1]), (plan, q[:11], k, v), (plan, q, k[:11], v[:11]),
+           (plan, q[:, :3], k, v), (plan, q.flatten(1), k, v), (None, q, k, v), (plan, q, k[..., :8], v[..., :8])]
+    for args in bad:
+        with pytest.raises(ValueError):
+            ops.attention(*args)
+    for kw in (dict(slopes=torch.zeros(3, device=device)), dict(out=torch.zeros(12, 4, 8, device=device)),
+               dict(lse=torch.zeros(12, 4, dtype=torch.float64, device=device)), dict(out=q[:1].expand(12, 4, 16))):
+        with pytest.raises(ValueError):
+            ops.attention(plan, q, k, v, **kw)
+    for kw in (dict(cap=-1.0), dict(cap=float("nan")), dict(scale=float("inf"))):
+        with pytest.raises(DofError):
+            ops.attention(plan, q, k, v, **kw)
+    for dim in (12, 136, 4):
+        z = torch.zeros(12, 2, dim, device=device)
+        with pytest.raises(DofError, match="head_dim"):
+            ops.attention(plan, z, z, z)
+    o, lse = ops.attention(plan, q, k, v)
+    for args in ((plan, g[:5], q, k, v, o, lse), (plan, g, q, k, v, o.half(), lse), (plan, g, q, k, v, o, lse[:5])):
+        with pytest.raises(ValueError):
+            ops.attention_backward(*args)
+    for args, kw in ((([-1],), {}), (([1.5],), {}), (([2, 3], [2]), {}), (([2],), dict(prefix=[1])), (([2],), dict(causal=True, prefix=[1, 1])),
+                     (([2],), dict(causal=True, prefix=[-1])), (([[2]],), {})):
+        with pytest.raises(ValueError):
+            ops.attention_plan(*args, **kw)
+    with pytest.raises(DofError, match="2\\^30"):
+        ops.attention_plan([2 ** 30 + 1])
+    none = ops.attention_plan([])
+    o, lse = ops.attention(none, q[:0], k[:0], v[:0])
+    assert o.shape == (0, 4, 16) and lse.shape == (0, 4)
+
+
+@pytest.mark.gpu
+def test_graph_replays_and_streams():
+    """Two captured graphs and an eager call on a third stream: no memory is shared, every replay gives the eager bits."""
+    ops = make_ops("cuda:0")
+    case = ([300, 77], None, 4, 2, 64, True, None, 0.0, False, "packed")
+    t, dev, kl, slopes = build(case, torch.bfloat16, "cuda:0")
+    t2, dev2, _, _ = build(case, torch.bfloat16, "cuda:0", seed=9)
+    plan = ops.attention_plan([300, 77], causal=True)
+
+    def step(x):
+        o, lse = ops.attention(plan, x["q"], x["k"], x["v"])
+        return (o, lse) + ops.attention_backward(plan, x["g"], x["q"], x["k"], x["v"], o, lse)
+
+    want = [[y.clone() for y in step(x)] for x in (dev, dev2)]
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    graphs, outs = [], []
+    for x in (dev, dev2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step(x))
+        graphs.append(graph)
+    for _ in range(3):
+        torch.cuda.synchronize()
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+        with torch.cuda.stream(streams[2]):
+            eager = step(dev2)
+        torch.cuda.synchronize()
+        for got, ref in zip(outs + [eager], want + [want[1]]):
+            assert all(torch.equal(a, b) for a, b in zip(got, ref))
