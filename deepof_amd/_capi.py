@@ -92,6 +92,17 @@ class Attention(C.Structure):
                 ("o_stride", _ST), ("g_stride", _ST), ("dq_stride", _ST), ("dk_stride", _ST), ("dv_stride", _ST)]
 
 
+_ST3 = C.c_int64 * 3
+
+
+class AttnStep(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("head_dim", C.c_int32), ("q_heads", C.c_int32), ("k_heads", C.c_int32),
+                ("streams", C.c_int32), ("new_frames", C.c_int32), ("n_pages", C.c_int32), ("page_size", C.c_int32),
+                ("max_pages", C.c_int32), ("reserved", C.c_int32), ("scale", C.c_float), ("cap", C.c_float),
+                ("q_stride", _ST3), ("k_stride", _ST3), ("v_stride", _ST3), ("o_stride", _ST3), ("kc_stride", _ST3),
+                ("vc_stride", _ST3)]
+
+
 PP_KINDS = {"other": 0, "coord": 1, "speed": 2, "dist_inner": 3, "dist_intra": 4, "angle": 5}
 PP_MODES = {None: 0, "per_column": 1, "groupwise": 2}
 PP_INTER_SCALE = {"mean": 0, "geom": 1, "global": 2}
@@ -178,6 +189,8 @@ SIGNATURES = {
     "dof_attention_forward": (C.c_int, [C.POINTER(AttnPlan), _P, C.POINTER(Attention)] + [_P] * 7),
     "dof_attention_workspace_bytes": (_I64, [_I64, _I32]),
     "dof_attention_backward": (C.c_int, [C.POINTER(AttnPlan), _P, C.POINTER(Attention)] + [_P] * 12),
+    "dof_attention_step_workspace_bytes": (_I64, [C.POINTER(AttnStep)]),
+    "dof_attention_step": (C.c_int, [C.POINTER(AttnStep)] + [_P] * 11),
 }
 
 

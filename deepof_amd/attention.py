@@ -284,9 +284,7 @@ class AttentionOps:
         elif lse.shape != q.shape[:2] or lse.dtype != torch.float32 or lse.device != self.device or not lse.is_contiguous():
             raise ValueError(f"lse must be a contiguous float32 tensor of shape {tuple(q.shape[:2])} on {self.device}")
         q, k, v = _wide(q), _wide(k), _wide(v)
-        ow = o if _is_wide(o) else torch.empty_like(q, memory_format=torch.contiguous_format)
-        if ow is not o:
-            ow.copy_(o)
+        ow = o if _is_wide(o) else o.clone(memory_format=torch.contiguous_format)
         d.q_stride[:], d.k_stride[:], d.v_stride[:], d.o_stride[:] = _st(q), _st(k), _st(v), _st(ow)
         with self._on_device():
             rc = self.lib.dof_attention_forward(C.byref(plan.record), plan.table.data_ptr(), C.byref(d), q.data_ptr(), k.data_ptr(),
@@ -322,10 +320,66 @@ class AttentionOps:
         _capi.check(self.lib, rc, "dof_attention_backward")
         return dq, dk, dv
 
+    # ---- the new frames of live streams ------------------------------------------------------------------------------
+    def attention_step(self, q, k, v, k_cache, v_cache, page_table, lengths, scale: Optional[float] = None, cap: float = 0.0,
+                       slopes=None, out=None):
+        """-> o (streams, new, query heads, head_dim).  q (streams, new, query heads, head_dim), k and v (streams, new, key heads,
+        head_dim): 1 to 16 new frames of every stream.  They are stored in ``k_cache`` / ``v_cache`` (pages, page size, key heads,
+        head_dim) behind the ``lengths`` (streams, int32) frames already there, on the pages that ``page_table`` (streams, pages,
+        int32) lists for the stream, and attend to everything up to themselves; the caller advances ``lengths``.  ``scale``, ``cap``
+        and ``slopes`` as in :meth:`attention`.
+
+        Streams may share pages that are full.  A negative length marks an idle stream: nothing of it is read or written (its rows
+        of ``out`` stay; allocated here they are undefined).  Frames behind the table's last page and frames on a page index that the
+        cache does not have are neither stored nor seen."""
+        dt = self._dtype("q", q)
+        _rows("q", q, self.device, dt, 4)
+        _rows("k", k, self.device, dt, 4)
+        _rows("v", v, self.device, dt, 4)
+        _writable("k_cache", _rows("k_cache", k_cache, self.device, dt, 4))
+        _writable("v_cache", _rows("v_cache", v_cache, self.device, dt, 4))
+        b, new, hq, dim = q.shape
+        hk = k.shape[2]
+        if k.shape != v.shape or k.shape[:2] != q.shape[:2] or k.shape[3] != dim:
+            raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not go together")
+        if k_cache.shape != v_cache.shape or k_cache.shape[2:] != (hk, dim):
+            raise ValueError(f"caches {tuple(k_cache.shape)} / {tuple(v_cache.shape)} must be (pages, page size, {hk}, {dim})")
+        if hk < 1 or hq % hk or hq < 1:
+            raise ValueError(f"{hq} query heads are not a multiple of {hk} key heads")
+        if not (_is_wide(k_cache) and _is_wide(v_cache)):
+            raise ValueError("the caches' address and strides must be multiples of 16 bytes")
+        if page_table.dim() != 2 or page_table.shape[0] != b or page_table.dtype != torch.int32 or page_table.device != self.device \
+                or not page_table.is_contiguous():
+            raise ValueError(f"page_table must be a contiguous int32 tensor ({b}, pages of a stream) on {self.device}")
+        ln = _vector("lengths", lengths, b, torch.int32, self.device)
+        d = _capi.AttnStep()
+        d.dtype, d.head_dim, d.q_heads, d.k_heads = DTYPES[dt], dim, hq, hk
+        d.streams, d.new_frames, d.n_pages, d.page_size, d.max_pages = b, new, k_cache.shape[0], k_cache.shape[1], page_table.shape[1]
+        d.scale = dim ** -0.5 if scale is None else scale
+        d.cap = cap
+        o = self._output("out", out, q.shape, dt)
+        ow = o
+        if not _is_wide(o):
+            ow = o.clone(memory_format=torch.contiguous_format)
+        q, k, v = _wide(q), _wide(k), _wide(v)
+        d.q_stride[:], d.k_stride[:], d.v_stride[:], d.o_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3], ow.stride()[:3]
+        d.kc_stride[:], d.vc_stride[:] = k_cache.stride()[:3], v_cache.stride()[:3]
+        sl = _vector("slopes", slopes, hq, torch.float32, self.device)
+        need = self._bytes("dof_attention_step_workspace_bytes", C.byref(d))
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        with self._on_device():
+            rc = self.lib.dof_attention_step(C.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(),
+                                             v_cache.data_ptr(), page_table.data_ptr(), ln, sl, ow.data_ptr(),
+                                             ws.data_ptr() if need else 0, self._stream())
+        _capi.check(self.lib, rc, "dof_attention_step")
+        if ow is not o:
+            o.copy_(ow)
+        return o
+
     def _bytes(self, fn: str, *args) -> int:
         n = getattr(self.lib, fn)(*args)
         if n < 0:
-            _capi.check(self.lib, -1, fn)
+            _capi.check(self.lib, n, fn)
         return n
 
 

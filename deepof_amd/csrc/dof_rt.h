@@ -116,6 +116,9 @@ typedef _Float16 dof_f16x8 __attribute__((ext_vector_type(8)));
 #define DOF_MFMA_16x16x32_F16(a, b, c) __builtin_amdgcn_mfma_f32_16x16x32_f16((a), (b), (c), 0, 0, 0)
 #define DOF_MFMA_32x32x2_F32(a, b, c) __builtin_amdgcn_mfma_f32_32x32x2f32((a), (b), (c), 0, 0, 0)
 #endif
+__device__ __forceinline__ int dof_shfl_int(int v, int lane) {
+  return __builtin_bit_cast(int, __shfl(__builtin_bit_cast(float, v), lane));
+}
 __device__ __forceinline__ float dof_bf16_to_f32(uint32_t lo16) { return __builtin_bit_cast(float, lo16 << 16); }
 // two fp32 values rounded to nearest even as packed 16-bit words (first argument in the low half)
 #ifdef DOF_EMU
@@ -127,6 +130,7 @@ __device__ __forceinline__ float dof_log2(float x) { return log2f(x); }
 // value of lane ^ 32 (the other half of the wavefront)
 __device__ __forceinline__ float dof_swap32(float v) { return __shfl_xor(v, 32); }
 __device__ __forceinline__ bool dof_wave_any(bool p) { return emu_any(p); }
+__device__ __forceinline__ uint64_t dof_ballot(bool p) { return emu_ballot(p); }
 __device__ __forceinline__ void dof_sincos_turns(double turns, float* s, float* c) {
   const double r = (turns - rint(turns)) * 6.283185307179586477;
   *s = (float)sin(r);
@@ -148,6 +152,7 @@ __device__ __forceinline__ float dof_exp2(float x) { return __builtin_amdgcn_exp
 __device__ __forceinline__ float dof_log2(float x) { return __builtin_amdgcn_logf(x); }   // v_log_f32, 1 ulp
 __device__ __forceinline__ float dof_swap32(float v) { return __shfl_xor(v, 32); }
 __device__ __forceinline__ bool dof_wave_any(bool p) { return __any(p); }
+__device__ __forceinline__ uint64_t dof_ballot(bool p) { return __ballot(p); }
 // sin and cos of `turns` revolutions: the reduction to half a turn is exact enough in 64 bits for any 32-bit position, what is
 // left (at most half a turn) is a 32-bit argument in units of pi
 __device__ __forceinline__ void dof_sincos_turns(double turns, float* s, float* c) {

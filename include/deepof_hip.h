@@ -543,6 +543,26 @@ int dof_attention_backward(const DofAttnPlan* plan, const void* table, const Dof
                            const void* k, const void* v, const float* slopes, const void* o, const float* lse, void* dq, void* dk,
                            void* dv, void* workspace, void* stream);
 
+/* The new frames of live streams against a paged key / value cache: stores k and v of the new frames in the cache and attends over
+ * it, in one call.  q (streams, new, q_heads, head_dim), k and v (streams, new, k_heads, head_dim), caches (pages, page_size,
+ * k_heads, head_dim); strides are given for the three outer dimensions.  page_table (streams, max_pages) int32: the pages of a stream
+ * in order; lengths (streams) int32: its frames in the cache before the call (the caller advances them).  New frame t stands at
+ * position lengths + t and sees every position up to its own; cap and slopes as in dof_attention_forward.  Different streams may
+ * share pages that are full; the pages that the new frames go to belong to one stream alone.
+ * Device data is not trusted: a length below 0 marks an idle stream (nothing of it is read or written), positions behind
+ * max_pages * page_size are neither stored nor seen, and so are those on a page index outside 0 .. n_pages - 1.
+ * new: 1 .. 16; head_dim: multiples of 8 from 8 to 128; tensors and strides multiples of 16 bytes; n_pages * page_size < 2^31. */
+typedef struct {
+  int32_t dtype, head_dim, q_heads, k_heads;
+  int32_t streams, new_frames, n_pages, page_size, max_pages, reserved;
+  float scale, cap;
+  int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3]; /* (stream, new frame, head) */
+  int64_t kc_stride[3], vc_stride[3];                         /* (page, slot, head) */
+} DofAttnStep;
+int64_t dof_attention_step_workspace_bytes(const DofAttnStep* dims); /* 0: none needed; -1: bad dims */
+int dof_attention_step(const DofAttnStep* dims, const void* q, const void* k, const void* v, void* k_cache, void* v_cache,
+                       const int32_t* page_table, const int32_t* lengths, const float* slopes, void* o, void* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -241,16 +241,17 @@ uint16_t emu_f32_to_f16(float f) {
   return sign | (uint16_t)((ex << 10) + (int)(m - 1024));
 }
 
-bool emu_any(bool p) {
+uint64_t emu_ballot(bool p) {
   int me = g_cur;
   int lane = me & 63, base = me - lane;
   g_xchg[me * 2] = p ? 1.0f : 0.0f;
   yield_as(WAIT_WAVE);
-  bool any = false;
+  uint64_t all = 0;
   for (int i = 0; i < 64; ++i)
-    if (base + i < (int)(blockDim.x * blockDim.y * blockDim.z) && g_fibers[base + i].st != DONE) any |= g_xchg[(base + i) * 2] != 0.0f;
+    if (base + i < (int)(blockDim.x * blockDim.y * blockDim.z) && g_fibers[base + i].st != DONE && g_xchg[(base + i) * 2] != 0.0f)
+      all |= 1ull << i;
   yield_as(WAIT_WAVE);
-  return any;
+  return all;
 }
 
 namespace {

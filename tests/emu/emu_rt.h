@@ -56,7 +56,8 @@ emu_f32x16 emu_mfma_32x32x2(float a, float b, emu_f32x16 c);
 uint16_t emu_f32_to_bf16(float f);  // round to nearest even
 uint16_t emu_f32_to_f16(float f);   // round to nearest even
 float emu_f16_to_f32(uint16_t h);
-bool emu_any(bool p);               // __any over the wavefront's live lanes
+uint64_t emu_ballot(bool p);        // __ballot over the wavefront's live lanes
+static inline bool emu_any(bool p) { return emu_ballot(p) != 0; }
 void emu_lds_tr16(const uint16_t* p, uint16_t out[4]);  // ds_read_b64_tr_b16 (see dof_lds_tr16)
 
 static inline void __syncthreads() { emu_sync_block(); }
