@@ -21,8 +21,6 @@
 
 namespace {
 
-constexpr int kRows = 32;  // query rows per step of the dk / dv kernel
-
 template <class T> struct Lift {
   static constexpr float p2 = 0.0f, p = 1.0f, ds = 1.0f;  // log2 of P's factor, P's factor, dS's factor
 };
@@ -31,7 +29,7 @@ template <> struct Lift<DofF16> {
 };
 
 template <class T, int DP, int NW>
-__global__ void __launch_bounds__(64 * NW) k_attn_dq(DofAttnBwd B) {
+__global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_attn_dq(DofAttnBwd B) {
   const DofAttnFwd& A = B.f;
   constexpr int KU = NW == 1 ? 1 : 2, kKeys = 32 * KU;  // keys per step, as in the forward
   using Tile = DofTile<T, kKeys, DP>;
@@ -39,9 +37,9 @@ __global__ void __launch_bounds__(64 * NW) k_attn_dq(DofAttnBwd B) {
   __shared__ Tile sk[2], sv[2];
   constexpr int KS = DP / 16, DT = DP / 32;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
-  const int64_t item = dof_xcd_item(blockIdx.x, (int64_t)A.n_tiles * A.q_heads);
-  const int h = (int)(item / A.n_tiles);
-  const DofAttnTile t = A.tiles[item - (int64_t)h * A.n_tiles];
+  int tile, h;
+  dof_attn_item(blockIdx.x, A.n_tiles, A.q_heads, &tile, &h);
+  const DofAttnTile t = A.tiles[tile];
   const int hk = h / (A.q_heads / A.k_heads);
 
   const int first = t.row0 + 32 * wave, row = first + col;
@@ -163,15 +161,16 @@ __global__ void __launch_bounds__(64 * NW) k_attn_dq(DofAttnBwd B) {
 template <class T, int DP, int NW>
 __global__ void __launch_bounds__(64 * NW) k_attn_dkv(DofAttnBwd B) {
   const DofAttnFwd& A = B.f;
+  constexpr int RU = NW == 1 ? 1 : 2, kRows = 32 * RU;  // query rows per step
   using Tile = DofTile<T, kRows, DP>;
   using Stage = DofStage<T, kRows, DP, 64 * NW>;
   __shared__ Tile sq[2], sg[2];
   __shared__ float sl[2][kRows], sd[2][kRows];  // log-sum-exp in units of log 2 (+inf: the row takes no part), delta
   constexpr int KS = DP / 16, DT = DP / 32;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
-  const int64_t item = dof_xcd_item(blockIdx.x, (int64_t)A.n_tiles * A.k_heads);
-  const int hk = (int)(item / A.n_tiles);
-  const DofAttnTile t = A.tiles[item - (int64_t)hk * A.n_tiles];
+  int tile, hk;
+  dof_attn_item(blockIdx.x, A.n_tiles, A.k_heads, &tile, &hk);
+  const DofAttnTile t = A.tiles[tile];
   const int group = A.q_heads / A.k_heads;
   const int off = t.lk - t.lq;
 
@@ -243,39 +242,46 @@ __global__ void __launch_bounds__(64 * NW) k_attn_dkv(DofAttnBwd B) {
     if (i0 + kRows > w_lo) {
       DofScore sc = A.score;
       if (A.slopes) sc.slope_l2 = A.slopes[hk * group + step / per_head] * kLog2e;
-      dof_f32x16 x = dof_zero16(), y = dof_zero16();
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        x = dof_mma32<T>(sq[buf].rowfrag(col, 2 * s + half), kf[s], x);
-        y = dof_mma32<T>(sg[buf].rowfrag(col, 2 * s + half), vf[s], y);
-      }
-      float p[16], ds[16];
       const bool partial = i0 < w_full;
-      const float base = (float)(i0 + off + 4 * half - key);
+      dof_f32x16 x[RU], y[RU];
 #pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        const int r = 8 * (v / 4) + v % 4;
-        float c = Lift<T>::ds / Lift<T>::p, w;
-        if (sc.cap_l2 != 0.0f) {
-          const float th = dof_cap_tanh<T>(x[v] * sc.mul);
-          w = sc.cap_l2 * th;
-          c *= 1.0f - th * th;
-        } else {
-          w = x[v] * sc.mul;
+      for (int u = 0; u < RU; ++u) {
+        x[u] = y[u] = dof_zero16();
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          x[u] = dof_mma32<T>(sq[buf].rowfrag(32 * u + col, 2 * s + half), kf[s], x[u]);
+          y[u] = dof_mma32<T>(sg[buf].rowfrag(32 * u + col, 2 * s + half), vf[s], y[u]);
         }
-        if (A.slopes) w -= sc.slope_l2 * fabsf(base + (float)r);
-        p[v] = dof_exp2(w - sl[buf][r + 4 * half]);
-        ds[v] = p[v] * c * (y[v] - sd[buf][r + 4 * half]);
-        if (partial && key >= dof_attn_kend(t, A.causal, i0 + r + 4 * half)) p[v] = ds[v] = 0.0f;
       }
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const DofFrag<T> pf = dof_frag_pack<T>(p + 8 * s), df = dof_frag_pack<T>(ds + 8 * s);
-        const int r = 16 * s + 4 * half;
+      for (int u = 0; u < RU; ++u) {
+        float p[16], ds[16];
+        const float base = (float)(i0 + 32 * u + off + 4 * half - key);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          dv[d] = dof_mma32<T>(sg[buf].colfrag(r, r + 8, 32 * d + col), pf, dv[d]);
-          dk[d] = dof_mma32<T>(sq[buf].colfrag(r, r + 8, 32 * d + col), df, dk[d]);
+        for (int v = 0; v < 16; ++v) {
+          const int r = 8 * (v / 4) + v % 4, at = 32 * u + r + 4 * half;
+          float c = Lift<T>::ds / Lift<T>::p, w;
+          if (sc.cap_l2 != 0.0f) {
+            const float th = dof_cap_tanh<T>(x[u][v] * sc.mul);
+            w = sc.cap_l2 * th;
+            c *= 1.0f - th * th;
+          } else {
+            w = x[u][v] * sc.mul;
+          }
+          if (A.slopes) w -= sc.slope_l2 * fabsf(base + (float)r);
+          p[v] = dof_exp2(w - sl[buf][at]);
+          ds[v] = p[v] * c * (y[u][v] - sd[buf][at]);
+          if (partial && key >= dof_attn_kend(t, A.causal, i0 + at)) p[v] = ds[v] = 0.0f;
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const DofFrag<T> pf = dof_frag_pack<T>(p + 8 * s), df = dof_frag_pack<T>(ds + 8 * s);
+          const int r = 32 * u + 16 * s + 4 * half;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            dv[d] = dof_mma32<T>(sg[buf].colfrag(r, r + 8, 32 * d + col), pf, dv[d]);
+            dk[d] = dof_mma32<T>(sq[buf].colfrag(r, r + 8, 32 * d + col), df, dk[d]);
+          }
         }
       }
     }

@@ -21,16 +21,16 @@ namespace {
 
 // keys per step: 64; a single wavefront stages a tile alone and takes 32, which fit its registers
 template <class T, int DP, int NW>
-__global__ void __launch_bounds__(64 * NW) k_attn_fwd(DofAttnFwd A) {
+__global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 64 ? 1 : 2) k_attn_fwd(DofAttnFwd A) {
   constexpr int KU = NW == 1 ? 1 : 2, kKeys = 32 * KU;
   using Tile = DofTile<T, kKeys, DP>;
   using Stage = DofStage<T, kKeys, DP, 64 * NW>;
   __shared__ Tile sk[2], sv[2];
   constexpr int KS = DP / 16, DT = DP / 32;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
-  const int64_t item = dof_xcd_item(blockIdx.x, (int64_t)A.n_tiles * A.q_heads);
-  const int h = (int)(item / A.n_tiles);
-  const DofAttnTile t = A.tiles[item - (int64_t)h * A.n_tiles];
+  int tile, h;
+  dof_attn_item(blockIdx.x, A.n_tiles, A.q_heads, &tile, &h);
+  const DofAttnTile t = A.tiles[tile];
   const int hk = h / (A.q_heads / A.k_heads);
 
   const int first = t.row0 + 32 * wave, row = first + col;
@@ -61,12 +61,22 @@ __global__ void __launch_bounds__(64 * NW) k_attn_fwd(DofAttnFwd A) {
   for (int d = 0; d < DT; ++d) o[d] = dof_zero16();
   float m = -INFINITY, l = 0.0f;
 
+  // In a step that some rows see only in part a hidden key's weight is zero, but zero times an infinity or NaN in V is not: such
+  // values are left out of the products there (rare, and looked for in these steps only) and put where they are seen at the end.
+  __shared__ int found;
+  const int kmin = dof_attn_kend(t, A.causal, t.row0);
+  if (tid == 0) found = 0;
+  __syncthreads();
   Stage rk, rv;
+  auto store_v = [&](int b, int j) {
+    if ((j + kKeys < t.lk ? j + kKeys : t.lk) > kmin) rv.store_finite(sv[b], tid, &found);
+    else rv.store(sv[b], tid);
+  };
   if (kmax > 0) {
     rk.load(kp, A.ks[0], t.lk, A.dim, tid);
     rv.load(vp, A.vs[0], t.lk, A.dim, tid);
     rk.store(sk[0], tid);
-    rv.store(sv[0], tid);
+    store_v(0, 0);
   }
   for (int j0 = 0, buf = 0; j0 < kmax; j0 += kKeys, buf ^= 1) {
     __syncthreads();
@@ -83,16 +93,19 @@ __global__ void __launch_bounds__(64 * NW) k_attn_fwd(DofAttnFwd A) {
 #pragma unroll
         for (int s = 0; s < KS; ++s) x[u] = dof_mma32<T>(sk[buf].rowfrag(32 * u + col, 2 * s + half), q[s], x[u]);
       }
+      float unit = 1.0f;  // of x, in log 2: the scale of plain scores is folded into the exponent's argument
       if (sc.cap_l2 != 0.0f) {
 #pragma unroll
         for (int u = 0; u < KU; ++u)
 #pragma unroll
           for (int v = 0; v < 16; ++v) x[u][v] = sc.cap_l2 * dof_cap_tanh<T>(x[u][v] * sc.mul);
-      } else {
+      } else if (A.slopes || !(sc.mul > 0.0f)) {
 #pragma unroll
         for (int u = 0; u < KU; ++u)
 #pragma unroll
           for (int v = 0; v < 16; ++v) x[u][v] *= sc.mul;
+      } else {
+        unit = sc.mul;
       }
       if (A.slopes) {
         const float base = (float)(pos - j0 - 4 * half);
@@ -114,7 +127,7 @@ __global__ void __launch_bounds__(64 * NW) k_attn_fwd(DofAttnFwd A) {
       for (int u = 0; u < KU; ++u)
 #pragma unroll
         for (int v = 0; v < 16; ++v) mt = fmaxf(mt, x[u][v]);
-      mt = fmaxf(mt, dof_swap32(mt));
+      mt = fmaxf(mt, dof_swap32(mt)) * unit;
       // The running maximum follows only when a tile's exceeds it by 2^8: until then the weights stay below 256, which costs the
       // fp32 sums nothing, and the accumulators need no rescaling pass.
       if (dof_wave_any(mt > m + 8.0f)) {
@@ -128,61 +141,43 @@ __global__ void __launch_bounds__(64 * NW) k_attn_fwd(DofAttnFwd A) {
           for (int v = 0; v < 16; ++v) o[d][v] *= a;
       }
       const float mm = m == -INFINITY ? 0.0f : m;
-      // In a tile that some rows see only in part, a hidden key's weight is zero, but zero times an infinity or NaN in V is not:
-      // such values (rare, so looked for in these tiles only) are taken out of the product and put where they are seen.
-      bool careful = false;
-      if ((j0 > wmin ? j0 : wmin) < (next < t.lk ? next : t.lk)) {
-        bool bad = false;
-#pragma unroll
-        for (int r = 0; r < kKeys; r += 16)
-#pragma unroll
-          for (int d = 0; d < DT; ++d) bad |= dof_frag_nonfinite<T>(sv[buf].colfrag(r + 4 * half, r + 8 + 4 * half, 32 * d + col));
-        careful = dof_wave_any(bad);
-      }
 #pragma unroll
       for (int u = 0; u < KU; ++u) {
         float p[16];
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
-          p[v] = dof_exp2(x[u][v] - mm);
+          p[v] = dof_exp2(fmaf(x[u][v], unit, -mm));
           l += p[v];
         }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           const DofFrag<T> pf = dof_frag_pack<T>(p + 8 * s);
           const int r = 32 * u + 16 * s + 4 * half;
-          if (!careful) {
 #pragma unroll
-            for (int d = 0; d < DT; ++d) o[d] = dof_mma32<T>(sv[buf].colfrag(r, r + 8, 32 * d + col), pf, o[d]);
-          } else {
-            float seen[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) seen[e] = j0 + r + e + (e < 4 ? 0 : 4) < kend ? 1.0f : 0.0f;
-            const DofFrag<T> sf = dof_frag_pack<T>(seen);
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-              DofFrag<T> f = sv[buf].colfrag(r, r + 8, 32 * d + col), pos_f, neg_f;
-              dof_frag_split<T>(f, pos_f, neg_f);
-              o[d] = dof_mma32<T>(f, pf, o[d]);
-              const dof_f32x16 up = dof_mma32<T>(pos_f, sf, dof_zero16()), down = dof_mma32<T>(neg_f, sf, dof_zero16());
-#pragma unroll
-              for (int v = 0; v < 16; ++v) {
-                if (up[v] > 0.0f) o[d][v] += INFINITY;
-                if (down[v] > 0.0f) o[d][v] -= INFINITY;
-              }
-            }
-          }
+          for (int d = 0; d < DT; ++d) o[d] = dof_mma32<T>(sv[buf].colfrag(r, r + 8, 32 * d + col), pf, o[d]);
         }
       }
     }
     if (next < kmax) {
       rk.store(sk[buf ^ 1], tid);
-      rv.store(sv[buf ^ 1], tid);
+      store_v(buf ^ 1, next);
     }
   }
 
   l += dof_swap32(l);
+  __syncthreads();
   if (!live) return;
+  if (found) {
+    for (int j = kmin / kKeys * kKeys; j < kend; ++j)
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const int e = 32 * d + 8 * (v / 4) + 4 * half + v % 4;
+          const float x = e < A.dim ? DofElem<T>::get(vp + j * A.vs[0] + e) : 0.0f;
+          if (!(fabsf(x) < INFINITY)) o[d][v] += x;
+        }
+  }
   const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // no visible key: zeros; NaN stays NaN
   T* op = static_cast<T*>(A.o) + (t.q0 + row) * A.os[0] + h * A.os[1];
 #pragma unroll

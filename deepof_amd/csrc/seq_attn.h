@@ -37,9 +37,21 @@ template <class T> __device__ __forceinline__ float dof_cap_tanh(float x) {
   else return dof_tanh(x);
 }
 
-// Blocks are dealt to the eight XCDs in turn; block -> work item such that each XCD gets a contiguous run of items (heads of one
-// group read the same keys and values: they meet in that XCD's L2)
-__device__ __forceinline__ int64_t dof_xcd_item(int64_t block, int64_t total) {
-  const int64_t per = total / 8, rem = total - per * 8, c = block % 8, n = block / 8;
-  return c * per + (c < rem ? c : rem) + n;
+// Blocks are dealt to the eight XCDs in turn, each with an L2 of its own.  Where the heads divide over the XCDs (or the XCDs over the
+// heads), a head's tiles go to as few XCDs as that allows -- its keys and values, and those of its group's neighbours, then come from
+// that L2 -- and in every case the tiles keep their order, longest first, on each XCD.
+__device__ __forceinline__ void dof_attn_item(int block, int n_tiles, int heads, int* tile, int* head) {
+  const int c = block & 7, n = block >> 3;
+  if (heads % 8 == 0) {
+    const int per = heads >> 3;
+    *tile = n / per;
+    *head = c * per + n - *tile * per;
+  } else if (8 % heads == 0 && n_tiles % (8 / heads) == 0) {
+    const int share = 8 / heads;
+    *head = c / share;
+    *tile = n * share + c % share;
+  } else {
+    *tile = block / heads;
+    *head = block - *tile * heads;
+  }
 }

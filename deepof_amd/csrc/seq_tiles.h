@@ -201,4 +201,28 @@ template <class T, int ROWS, int DP, int NT> struct DofStage {
       if ((ROWS * Tile::CH) % NT == 0 || r < ROWS) t.put(r, c, reg[i]);
     }
   }
+  // store() with zeros in the place of infinities and NaN; *found is set if there were any
+  __device__ __forceinline__ void store_finite(Tile& t, int tid, int* found) const {
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int e = tid + i * NT, r = e / Tile::CH, c = e - r * Tile::CH;
+      DofWords<4> v = reg[i];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (sizeof(T) == 4) {
+          const bool bad = (v.w[k] & 0x7F800000u) == 0x7F800000u;
+          any |= bad;
+          if (bad) v.w[k] = 0u;
+        } else {
+          constexpr uint32_t m = std::is_same<T, DofBf16>::value ? 0x7F80u : 0x7C00u;
+          const bool lo = (v.w[k] & m) == m, hi = (v.w[k] & (m << 16)) == (m << 16);
+          any |= lo || hi;
+          v.w[k] &= (lo ? 0xFFFF0000u : 0xFFFFFFFFu) & (hi ? 0x0000FFFFu : 0xFFFFFFFFu);
+        }
+      }
+      if ((ROWS * Tile::CH) % NT == 0 || r < ROWS) t.put(r, c, v);
+    }
+    if (any) *found = 1;
+  }
 };
