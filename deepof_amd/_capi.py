@@ -83,7 +83,7 @@ class NormRope(C.Structure):
 
 
 class AttnPlan(C.Structure):
-    _fields_ = [("n_docs", C.c_int32), ("causal", C.c_int32), ("n_tiles", C.c_int64 * 4), ("table_bytes", C.c_int64)]
+    _fields_ = [("n_docs", C.c_int32), ("causal", C.c_int32), ("q_rows", C.c_int64), ("k_rows", C.c_int64), ("n_tiles", C.c_int64 * 4), ("table_bytes", C.c_int64)]
 
 
 class Attention(C.Structure):
@@ -187,7 +187,7 @@ SIGNATURES = {
     "dof_attn_plan_size": (C.c_int, [_I32, _P, _P, _I32, C.POINTER(AttnPlan)]),
     "dof_attn_plan_table": (C.c_int, [C.POINTER(AttnPlan), _P, _P, _P, _P]),
     "dof_attention_forward": (C.c_int, [C.POINTER(AttnPlan), _P, C.POINTER(Attention)] + [_P] * 7),
-    "dof_attention_workspace_bytes": (_I64, [_I64, _I32]),
+    "dof_attention_workspace_bytes": (_I64, [C.POINTER(AttnPlan), C.POINTER(Attention)]),
     "dof_attention_backward": (C.c_int, [C.POINTER(AttnPlan), _P, C.POINTER(Attention)] + [_P] * 12),
     "dof_attention_step_workspace_bytes": (_I64, [C.POINTER(AttnStep)]),
     "dof_attention_step": (C.c_int, [C.POINTER(AttnStep)] + [_P] * 11),

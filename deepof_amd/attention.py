@@ -312,7 +312,7 @@ class AttentionOps:
         q, k, v, do, o = _wide(q), _wide(k), _wide(v), _wide(do), _wide(o)
         d.q_stride[:], d.k_stride[:], d.v_stride[:], d.o_stride[:], d.g_stride[:] = _st(q), _st(k), _st(v), _st(o), _st(do)
         d.dq_stride[:], d.dk_stride[:], d.dv_stride[:] = _st(dq), _st(dk), _st(dv)
-        ws = torch.empty(self._bytes("dof_attention_workspace_bytes", plan.q_rows, q.shape[1]), dtype=torch.uint8, device=self.device)
+        ws = torch.empty(self._bytes("dof_attention_workspace_bytes", C.byref(plan.record), C.byref(d)), dtype=torch.uint8, device=self.device)
         with self._on_device():
             rc = self.lib.dof_attention_backward(C.byref(plan.record), plan.table.data_ptr(), C.byref(d), do.data_ptr(), q.data_ptr(),
                                                  k.data_ptr(), v.data_ptr(), sl, o.data_ptr(), lse.data_ptr(), dq.data_ptr(),

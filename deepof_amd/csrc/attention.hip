@@ -100,19 +100,37 @@ int check(const DofAttnPlan* p, const void* table, const DofAttention* d, const 
   return DOF_OK;
 }
 
-// list 0: query tiles of 128 rows, 1: of 32; 2, 3: key tiles
+// list 0: query tiles of 128 rows, 1: of 32; 2: key tiles of 64, 3: of 32
 const DofAttnTile* list_at(const DofAttnPlan* p, const void* table, int list) {
   const DofAttnTile* t = static_cast<const DofAttnTile*>(table);
   for (int i = 0; i < list; ++i) t += p->n_tiles[i];
   return t;
 }
 
-// Tiles of 128 rows (four wavefronts share the staged keys) unless the documents are so short that most of such a tile is empty, or
+// Tiles of 128 rows (four wavefronts share what is staged) unless the documents are so short that most of such a tile is empty, or
 // there are so few of them that most CUs would go without work.
 int flat_tiles(const DofAttnPlan* p, int which, int heads) {
   const int64_t tall = p->n_tiles[which], flat = p->n_tiles[which + 1];
   return flat * 2 < tall * 5 || (tall * heads < 256 && flat > tall);
 }
+
+// dk / dv: a workgroup per key tile and key head goes through all query heads of the group.  Where those are too few to fill the chip
+// evenly (a causal tile's work ranges from nothing to all rows), the group's heads are shared out; the fp32 parts cost a write and a
+// read of the key rows per share.
+struct Shares { int flat, splits, heads_per; };
+Shares shares_of(const DofAttnPlan* p, const DofAttention* d) {
+  const int group = d->q_heads / d->k_heads;
+  Shares s;
+  s.flat = flat_tiles(p, 2, d->q_heads);
+  const int64_t items = p->n_tiles[2 + s.flat] * d->k_heads;
+  int64_t want = items > 0 ? (2048 + items - 1) / items : 1;
+  if (want > group) want = group;
+  s.heads_per = (int)((group + want - 1) / want);
+  s.splits = (group + s.heads_per - 1) / s.heads_per;
+  return s;
+}
+
+int64_t delta_bytes(const DofAttnPlan* p, const DofAttention* d) { return (p->q_rows * d->q_heads * 4 + 15) / 16 * 16; }
 
 DofAttnFwd forward_args(const DofAttention* d, const void* q, const void* k, const void* v, const float* slopes, void* o, float* lse) {
   DofAttnFwd A;
@@ -155,6 +173,8 @@ extern "C" int dof_attn_plan_size(int32_t n_docs, const int64_t* q_off, const in
   if (rc != DOF_OK) return rc;
   plan->n_docs = n_docs;
   plan->causal = causal != 0;
+  plan->q_rows = n_docs ? q_off[n_docs] : 0;
+  plan->k_rows = n_docs ? k_off[n_docs] : 0;
   plan->n_tiles[0] = count_tiles(n_docs, q_off, kAttnTall);
   plan->n_tiles[1] = count_tiles(n_docs, q_off, kAttnFlat);
   plan->n_tiles[2] = count_tiles(n_docs, k_off, kAttnTall);
@@ -218,12 +238,11 @@ extern "C" int dof_attention_forward(const DofAttnPlan* plan, const void* table,
   return dof_launch_attn_fwd(A, d->dtype, flat, (hipStream_t)stream);
 }
 
-extern "C" int64_t dof_attention_workspace_bytes(int64_t query_rows, int32_t q_heads) {
-  if (query_rows < 0 || q_heads < 1) {
-    dof_set_error("dof_attention_workspace_bytes: bad sizes");
-    return -1;
-  }
-  return query_rows * q_heads * 4;
+extern "C" int64_t dof_attention_workspace_bytes(const DofAttnPlan* plan, const DofAttention* d) {
+  static const char none = 0;
+  if (check(plan, &none, d, "dof_attention_workspace_bytes") != DOF_OK) return -1;
+  const Shares s = shares_of(plan, d);
+  return delta_bytes(plan, d) + (s.splits > 1 ? 2 * s.splits * plan->k_rows * d->k_heads * d->head_dim * 4 : 0);
 }
 
 extern "C" int dof_attention_backward(const DofAttnPlan* plan, const void* table, const DofAttention* d, const void* g, const void* q,
@@ -233,7 +252,7 @@ extern "C" int dof_attention_backward(const DofAttnPlan* plan, const void* table
   if (rc != DOF_OK) return rc;
   const bool rows = plan->n_tiles[0] > 0, keys = plan->n_tiles[2] > 0;
   if (!rows && !keys) return DOF_OK;
-  if ((rows && (!g || !q || !o || !lse || !dq || !workspace)) || (keys && (!k || !v || !dk || !dv))) {
+  if (!workspace || (rows && (!g || !q || !o || !lse || !dq)) || (keys && (!k || !v || !dk || !dv))) {
     dof_set_error("dof_attention_backward: null tensor");
     return DOF_ERR_ARG;
   }
@@ -266,9 +285,13 @@ extern "C" int dof_attention_backward(const DofAttnPlan* plan, const void* table
     if (rc != DOF_OK) return rc;
   }
   if (keys) {
-    const int flat = flat_tiles(plan, 2, d->k_heads);
-    set_tiles(&B.f, plan, table, 2, flat);
-    rc = dof_launch_attn_dkv(B, d->dtype, flat, (hipStream_t)stream);
+    const Shares s = shares_of(plan, d);
+    B.splits = s.splits;
+    B.heads_per = s.heads_per;
+    B.k_rows = plan->k_rows;
+    B.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + delta_bytes(plan, d));
+    set_tiles(&B.f, plan, table, 2, s.flat);
+    rc = dof_launch_attn_dkv(B, d->dtype, s.flat, (hipStream_t)stream);
   }
   return rc;
 }

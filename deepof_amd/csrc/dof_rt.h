@@ -150,7 +150,13 @@ __device__ __forceinline__ uint32_t dof_pack_f16(float a, float b) {
 __device__ __forceinline__ float dof_f16_to_f32(uint32_t lo16) { return (float)__builtin_bit_cast(_Float16, (uint16_t)lo16); }
 __device__ __forceinline__ float dof_exp2(float x) { return __builtin_amdgcn_exp2f(x); }  // v_exp_f32, 1 ulp, denormals to 0
 __device__ __forceinline__ float dof_log2(float x) { return __builtin_amdgcn_logf(x); }   // v_log_f32, 1 ulp
-__device__ __forceinline__ float dof_swap32(float v) { return __shfl_xor(v, 32); }
+// v_permlane32_swap_b32: a VALU exchange of the half-wavefronts (a shuffle would go through the LDS pipe)
+__device__ __forceinline__ float dof_swap32(float v) {
+  typedef unsigned dof_u32x2 __attribute__((ext_vector_type(2)));
+  const unsigned u = __builtin_bit_cast(unsigned, v);
+  const dof_u32x2 r = __builtin_bit_cast(dof_u32x2, __builtin_amdgcn_permlane32_swap(u, u, false, false));
+  return __builtin_bit_cast(float, (threadIdx.x & 32) ? r[0] : r[1]);
+}
 __device__ __forceinline__ bool dof_wave_any(bool p) { return __any(p); }
 __device__ __forceinline__ uint64_t dof_ballot(bool p) { return __ballot(p); }
 // sin and cos of `turns` revolutions: the reduction to half a turn is exact enough in 64 bits for any 32-bit position, what is

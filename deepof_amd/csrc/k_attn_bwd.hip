@@ -28,7 +28,8 @@ template <> struct Lift<DofF16> {
   static constexpr float p2 = 12.0f, p = 4096.0f, ds = 64.0f;
 };
 
-template <class T, int DP, int NW>
+// PLAIN: neither cap nor bias (as in the forward)
+template <class T, int DP, int NW, bool PLAIN>
 __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_attn_dq(DofAttnBwd B) {
   const DofAttnFwd& A = B.f;
   constexpr int KU = NW == 1 ? 1 : 2, kKeys = 32 * KU;  // keys per step, as in the forward
@@ -115,17 +116,19 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
           const int r = 8 * (v / 4) + v % 4;
-          float c = Lift<T>::ds / Lift<T>::p, w;
-          if (sc.cap_l2 != 0.0f) {
-            const float th = dof_cap_tanh<T>(x[v] * sc.mul);
-            w = sc.cap_l2 * th;
-            c *= 1.0f - th * th;
+          float c = Lift<T>::ds / Lift<T>::p, p;
+          if constexpr (PLAIN) {
+            p = dof_exp2(fmaf(x[v], sc.mul, -lse2));
           } else {
-            w = x[v] * sc.mul;
+            float w = x[v] * sc.mul;
+            if (sc.cap_l2 != 0.0f) {
+              const float th = dof_cap_tanh<T>(w);
+              w = sc.cap_l2 * th;
+              c *= 1.0f - th * th;
+            }
+            if (A.slopes) w -= sc.slope_l2 * fabsf(base - (float)r);
+            p = dof_exp2(w - lse2);
           }
-          if (A.slopes) w -= sc.slope_l2 * fabsf(base - (float)r);
-          float p = dof_exp2(w - lse2);
-          if (partial && r >= left) p = 0.0f;
           ds[v] = p * c * (y[v] - delta);
           if (partial && r >= left) ds[v] = 0.0f;  // not 0 x (what a masked key holds)
         }
@@ -158,58 +161,66 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_
     }
 }
 
-template <class T, int DP, int NW>
-__global__ void __launch_bounds__(64 * NW) k_attn_dkv(DofAttnBwd B) {
+// WANT: 1 = dv, 2 = dk, 3 = both in one pass.  Heads over 64 take two passes: with both accumulators (and their operands) in
+// registers only one wavefront fits a SIMD, and one alone does not hide its own latencies (16384 frames, heads of 128: 6.4 ms in one
+// pass, 4 products; the two passes run 5).
+// A workgroup takes `heads_per` query heads of the group; several workgroups of one key tile leave fp32 parts for k_attn_join.
+template <class T, int DP, int NW, bool PLAIN, int WANT>
+__global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_attn_dkv(DofAttnBwd B) {
   const DofAttnFwd& A = B.f;
-  constexpr int RU = NW == 1 ? 1 : 2, kRows = 32 * RU;  // query rows per step
+  constexpr bool DV = (WANT & 1) != 0, DK = (WANT & 2) != 0;
+  constexpr int kRows = 32;  // query rows per step
   using Tile = DofTile<T, kRows, DP>;
   using Stage = DofStage<T, kRows, DP, 64 * NW>;
   __shared__ Tile sq[2], sg[2];
-  __shared__ float sl[2][kRows], sd[2][kRows];  // log-sum-exp in units of log 2 (+inf: the row takes no part), delta
+  alignas(16) __shared__ float sl[2][kRows];  // log-sum-exp in units of log 2 (+inf: the row takes no part)
+  alignas(16) __shared__ float sd[2][kRows];  // delta
   constexpr int KS = DP / 16, DT = DP / 32;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
-  int tile, hk;
-  dof_attn_item(blockIdx.x, A.n_tiles, A.k_heads, &tile, &hk);
-  const DofAttnTile t = A.tiles[tile];
   const int group = A.q_heads / A.k_heads;
+  int tile, unit;
+  dof_attn_item(blockIdx.x, A.n_tiles, A.k_heads * B.splits, &tile, &unit);
+  const DofAttnTile t = A.tiles[tile];
+  const int hk = unit / B.splits, split = unit - hk * B.splits;
+  const int h_lo = hk * group + split * B.heads_per;
+  const int heads = split * B.heads_per + B.heads_per < group ? B.heads_per : group - split * B.heads_per;
   const int off = t.lk - t.lq;
 
   const int first = t.row0 + 32 * wave, key = first + col;
   const bool live = key < t.lk;
-  // the first query row that sees any key of the workgroup (of the wavefront): keys below the prefix are seen by all, key j by the
-  // rows from j - off on
+  // the first query row that sees key j: keys below the prefix are seen by all, key j by the rows from j - off on
   auto row_from = [&](int j) {
     if (!A.causal || j < t.prefix) return 0;
     return j - off > 0 ? j - off : 0;
   };
   const int i_lo = row_from(t.row0) & ~(kRows - 1);
   const int w_lo = first < t.lk ? row_from(first) : t.lq;
-  // from this row on, every row sees every key of the wavefront
-  const int last_key = first + 31 < t.lk ? first + 31 : t.lk - 1;
-  const int w_full = row_from(last_key);
+  const int w_full = row_from(first + 31 < t.lk ? first + 31 : t.lk - 1);  // from here on every row sees every key of the wavefront
+  const int mine = row_from(key);
 
-  DofFrag<T> kf[KS], vf[KS];
+  DofFrag<T> kf[KS], vf[DK ? KS : 1];
   const T* kp = static_cast<const T*>(A.k) + (t.k0 + key) * A.ks[0] + hk * A.ks[1];
   const T* vp = static_cast<const T*>(A.v) + (t.k0 + key) * A.vs[0] + hk * A.vs[1];
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
     const int e = 16 * s + 8 * half;
-    kf[s] = vf[s] = dof_frag_zero<T>();
-    if (live && e < A.dim) {
-      kf[s] = dof_frag_load<T>(kp + e);
-      vf[s] = dof_frag_load<T>(vp + e);
+    kf[s] = dof_frag_zero<T>();
+    if (live && e < A.dim) kf[s] = dof_frag_load<T>(kp + e);
+    if constexpr (DK) {
+      vf[s] = dof_frag_zero<T>();
+      if (live && e < A.dim) vf[s] = dof_frag_load<T>(vp + e);
     }
   }
-  dof_f32x16 dk[DT], dv[DT];
+  dof_f32x16 dk[DK ? DT : 1], dv[DV ? DT : 1];
 #pragma unroll
-  for (int d = 0; d < DT; ++d) dk[d] = dv[d] = dof_zero16();
+  for (int d = 0; d < DT; ++d) {
+    if constexpr (DK) dk[d] = dof_zero16();
+    if constexpr (DV) dv[d] = dof_zero16();
+  }
 
   Stage rq, rg;
   float rl = 0.0f, rd = 0.0f;
-  const int per_head = t.lq > i_lo ? (t.lq - i_lo + kRows - 1) / kRows : 0;
-  const int steps = per_head * group;
-  auto load = [&](int step) {
-    const int h = hk * group + step / per_head, i0 = i_lo + (step % per_head) * kRows;
+  auto load = [&](int h, int i0) {
     rq.load(static_cast<const T*>(A.q) + (t.q0 + i0) * A.qs[0] + h * A.qs[1], A.qs[0], t.lq - i0, A.dim, tid);
     rg.load(static_cast<const T*>(B.g) + (t.q0 + i0) * B.gs[0] + h * B.gs[1], B.gs[0], t.lq - i0, A.dim, tid);
     if (tid < kRows) {
@@ -231,91 +242,144 @@ __global__ void __launch_bounds__(64 * NW) k_attn_dkv(DofAttnBwd B) {
       sd[buf][tid] = rd;
     }
   };
-  if (steps > 0) {
-    load(0);
+  const bool any = t.lq > i_lo && heads > 0;
+  if (any) {
+    load(h_lo, i_lo);
     store(0);
   }
-  for (int step = 0, buf = 0; step < steps; ++step, buf ^= 1) {
+  int buf = 0;
+  for (int h = h_lo, i0 = i_lo; any && h < h_lo + heads; buf ^= 1) {
     __syncthreads();
-    if (step + 1 < steps) load(step + 1);
-    const int i0 = i_lo + (step % per_head) * kRows;
+    const bool wrap = i0 + kRows >= t.lq;
+    const int next_h = wrap ? h + 1 : h, next_i = wrap ? i_lo : i0 + kRows;
+    if (next_h < h_lo + heads) load(next_h, next_i);
     if (i0 + kRows > w_lo) {
-      DofScore sc = A.score;
-      if (A.slopes) sc.slope_l2 = A.slopes[hk * group + step / per_head] * kLog2e;
-      const bool partial = i0 < w_full;
-      dof_f32x16 x[RU], y[RU];
+      dof_f32x16 x = dof_zero16(), y = dof_zero16();
 #pragma unroll
-      for (int u = 0; u < RU; ++u) {
-        x[u] = y[u] = dof_zero16();
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          x[u] = dof_mma32<T>(sq[buf].rowfrag(32 * u + col, 2 * s + half), kf[s], x[u]);
-          y[u] = dof_mma32<T>(sg[buf].rowfrag(32 * u + col, 2 * s + half), vf[s], y[u]);
-        }
+      for (int s = 0; s < KS; ++s) {
+        x = dof_mma32<T>(sq[buf].rowfrag(col, 2 * s + half), kf[s], x);
+        if constexpr (DK) y = dof_mma32<T>(sg[buf].rowfrag(col, 2 * s + half), vf[s], y);
       }
+      float p[16], ds[16];
+      const float slope = !PLAIN && A.slopes ? A.slopes[h] * kLog2e : 0.0f;
+      const float base = (float)(i0 + off + 4 * half - key);
+      const bool partial = i0 < w_full;
+      const int left = mine - i0 - 4 * half;  // rows before this one do not see the lane's key
 #pragma unroll
-      for (int u = 0; u < RU; ++u) {
-        float p[16], ds[16];
-        const float base = (float)(i0 + 32 * u + off + 4 * half - key);
+      for (int v = 0; v < 16; ++v) {
+        const int r = 8 * (v / 4) + v % 4;
+        float c = Lift<T>::ds / Lift<T>::p;
+        const float lse2 = sl[buf][r + 4 * half];
+        if constexpr (PLAIN) {
+          p[v] = dof_exp2(fmaf(x[v], A.score.mul, -lse2));
+        } else {
+          float w = x[v] * A.score.mul;
+          if (A.score.cap_l2 != 0.0f) {
+            const float th = dof_cap_tanh<T>(w);
+            w = A.score.cap_l2 * th;
+            c *= 1.0f - th * th;
+          }
+          if (A.slopes) w -= slope * fabsf(base + (float)r);
+          p[v] = dof_exp2(w - lse2);
+        }
+        if constexpr (DK) ds[v] = p[v] * c * (y[v] - sd[buf][r + 4 * half]);
+      }
+      if (partial) {
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
-          const int r = 8 * (v / 4) + v % 4, at = 32 * u + r + 4 * half;
-          float c = Lift<T>::ds / Lift<T>::p, w;
-          if (sc.cap_l2 != 0.0f) {
-            const float th = dof_cap_tanh<T>(x[u][v] * sc.mul);
-            w = sc.cap_l2 * th;
-            c *= 1.0f - th * th;
-          } else {
-            w = x[u][v] * sc.mul;
-          }
-          if (A.slopes) w -= sc.slope_l2 * fabsf(base + (float)r);
-          p[v] = dof_exp2(w - sl[buf][at]);
-          ds[v] = p[v] * c * (y[u][v] - sd[buf][at]);
-          if (partial && key >= dof_attn_kend(t, A.causal, i0 + at)) p[v] = ds[v] = 0.0f;
+          const bool hidden = 8 * (v / 4) + v % 4 < left;
+          if constexpr (DV) p[v] = hidden ? 0.0f : p[v];
+          if constexpr (DK) ds[v] = hidden ? 0.0f : ds[v];
         }
+      }
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const DofFrag<T> pf = dof_frag_pack<T>(p + 8 * s), df = dof_frag_pack<T>(ds + 8 * s);
-          const int r = 32 * u + 16 * s + 4 * half;
+      for (int s = 0; s < 2; ++s) {
+        const int r = 16 * s + 4 * half;
+        if constexpr (DV) {
+          const DofFrag<T> f = dof_frag_pack<T>(p + 8 * s);
 #pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            dv[d] = dof_mma32<T>(sg[buf].colfrag(r, r + 8, 32 * d + col), pf, dv[d]);
-            dk[d] = dof_mma32<T>(sq[buf].colfrag(r, r + 8, 32 * d + col), df, dk[d]);
-          }
+          for (int d = 0; d < DT; ++d) dv[d] = dof_mma32<T>(sg[buf].colfrag(r, r + 8, 32 * d + col), f, dv[d]);
+        }
+        if constexpr (DK) {
+          const DofFrag<T> f = dof_frag_pack<T>(ds + 8 * s);
+#pragma unroll
+          for (int d = 0; d < DT; ++d) dk[d] = dof_mma32<T>(sq[buf].colfrag(r, r + 8, 32 * d + col), f, dk[d]);
         }
       }
     }
-    if (step + 1 < steps) store(buf ^ 1);
+    if (next_h < h_lo + heads) store(buf ^ 1);
+    h = next_h;
+    i0 = next_i;
   }
   if (!live) return;
-  T* dkp = static_cast<T*>(B.dk) + (t.k0 + key) * B.dks[0] + hk * B.dks[1];
-  T* dvp = static_cast<T*>(B.dv) + (t.k0 + key) * B.dvs[0] + hk * B.dvs[1];
   const float ok = B.scale / Lift<T>::ds, ov = 1.0f / Lift<T>::p;
+  auto write = [&](const dof_f32x16* acc, float f, void* out, const int64_t* st, float* part) {
 #pragma unroll
-  for (int d = 0; d < DT; ++d)
+    for (int d = 0; d < DT; ++d)
 #pragma unroll
-    for (int v = 0; v < 16; v += 4) {
-      const int e = 32 * d + 2 * v + 4 * half;
-      if (e < A.dim) {
-        const float a[4] = {dk[d][v] * ok, dk[d][v + 1] * ok, dk[d][v + 2] * ok, dk[d][v + 3] * ok};
-        const float b[4] = {dv[d][v] * ov, dv[d][v + 1] * ov, dv[d][v + 2] * ov, dv[d][v + 3] * ov};
-        dof_store_vec<T, 4>(dkp + e, a);
-        dof_store_vec<T, 4>(dvp + e, b);
+      for (int v = 0; v < 16; v += 4) {
+        const int e = 32 * d + 2 * v + 4 * half;
+        if (e >= A.dim) continue;
+        const float r[4] = {acc[d][v] * f, acc[d][v + 1] * f, acc[d][v + 2] * f, acc[d][v + 3] * f};
+        if (B.splits == 1) dof_store_vec<T, 4>(static_cast<T*>(out) + (t.k0 + key) * st[0] + hk * st[1] + e, r);
+        else dof_store_vec<float, 4>(part + ((split * B.k_rows + t.k0 + key) * A.k_heads + hk) * A.dim + e, r);
       }
-    }
+  };
+  if constexpr (DK) write(dk, ok, B.dk, B.dks, B.part);
+  if constexpr (DV) write(dv, ov, B.dv, B.dvs, B.part + B.splits * B.k_rows * A.k_heads * A.dim);
 }
 
+// dk and dv (blockIdx.y) from the parts of several workgroups per key tile, added in order.  Four elements a thread, rows of the tiles.
+template <class T>
+__global__ void __launch_bounds__(256) k_attn_join(DofAttnBwd B) {
+  const DofAttnFwd& A = B.f;
+  const int quads = A.dim / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t rh = i / quads, row = rh / A.k_heads;
+  if (row >= B.k_rows) return;
+  const int e = (int)(i - rh * quads) * 4, hk = (int)(rh - row * A.k_heads);
+  const float* part = B.part + (blockIdx.y ? B.splits * B.k_rows * A.k_heads * A.dim : 0);
+  float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int k = 0; k < B.splits; ++k) {
+    float v[4];
+    dof_load_vec<float, 4>(part + ((k * B.k_rows + row) * A.k_heads + hk) * A.dim + e, v);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[j] += v[j];
+  }
+  const int64_t* st = blockIdx.y ? B.dvs : B.dks;
+  dof_store_vec<T, 4>(static_cast<T*>(blockIdx.y ? B.dv : B.dk) + row * st[0] + hk * st[1] + e, s);
+}
+
+template <class T, int DP, bool PLAIN>
+void launch_dq_as(const DofAttnBwd& B, int flat, hipStream_t stream) {
+  const unsigned blocks = (unsigned)((int64_t)B.f.n_tiles * B.f.q_heads);
+  if (flat) DOF_LAUNCH((k_attn_dq<T, DP, 1, PLAIN>), (blocks, 1, 1), (64, 1, 1), stream, B);
+  else DOF_LAUNCH((k_attn_dq<T, DP, 4, PLAIN>), (blocks, 1, 1), (256, 1, 1), stream, B);
+}
+template <class T, int DP, bool PLAIN, int WANT>
+void launch_dkv_want(const DofAttnBwd& B, int flat, hipStream_t stream) {
+  const unsigned blocks = (unsigned)((int64_t)B.f.n_tiles * B.f.k_heads * B.splits);
+  if (flat) DOF_LAUNCH((k_attn_dkv<T, DP, 1, PLAIN, WANT>), (blocks, 1, 1), (64, 1, 1), stream, B);
+  else DOF_LAUNCH((k_attn_dkv<T, DP, 4, PLAIN, WANT>), (blocks, 1, 1), (256, 1, 1), stream, B);
+}
+template <class T, int DP, bool PLAIN>
+void launch_dkv_as(const DofAttnBwd& B, int flat, hipStream_t stream) {
+  if constexpr (DP <= 64) {
+    launch_dkv_want<T, DP, PLAIN, 3>(B, flat, stream);
+  } else {
+    launch_dkv_want<T, DP, PLAIN, 1>(B, flat, stream);
+    launch_dkv_want<T, DP, PLAIN, 2>(B, flat, stream);
+  }
+}
 template <class T, int DP>
 void launch_dq(const DofAttnBwd& B, int flat, hipStream_t stream) {
-  const unsigned blocks = (unsigned)((int64_t)B.f.n_tiles * B.f.q_heads);
-  if (flat) DOF_LAUNCH((k_attn_dq<T, DP, 1>), (blocks, 1, 1), (64, 1, 1), stream, B);
-  else DOF_LAUNCH((k_attn_dq<T, DP, 4>), (blocks, 1, 1), (256, 1, 1), stream, B);
+  if (dof_attn_plain(B.f)) launch_dq_as<T, DP, true>(B, flat, stream);
+  else launch_dq_as<T, DP, false>(B, flat, stream);
 }
 template <class T, int DP>
 void launch_dkv(const DofAttnBwd& B, int flat, hipStream_t stream) {
-  const unsigned blocks = (unsigned)((int64_t)B.f.n_tiles * B.f.k_heads);
-  if (flat) DOF_LAUNCH((k_attn_dkv<T, DP, 1>), (blocks, 1, 1), (64, 1, 1), stream, B);
-  else DOF_LAUNCH((k_attn_dkv<T, DP, 4>), (blocks, 1, 1), (256, 1, 1), stream, B);
+  if (dof_attn_plain(B.f)) launch_dkv_as<T, DP, true>(B, flat, stream);
+  else launch_dkv_as<T, DP, false>(B, flat, stream);
 }
 
 }  // namespace
@@ -336,6 +400,8 @@ int dof_launch_attn_dkv(const DofAttnBwd& B, int dtype, int flat, hipStream_t st
     else if (B.f.dim <= 64) launch_dkv<T, 64>(B, flat, stream);
     else if (B.f.dim <= 96) launch_dkv<T, 96>(B, flat, stream);
     else launch_dkv<T, 128>(B, flat, stream);
+    if (B.splits > 1)
+      DOF_LAUNCH((k_attn_join<T>), (dof_cdiv(B.k_rows * B.f.k_heads * (B.f.dim / 4), 256), 2, 1), (256, 1, 1), stream, B);
   });
   return dof_check_launch("k_attn_dkv");
 }

@@ -20,7 +20,8 @@
 namespace {
 
 // keys per step: 64; a single wavefront stages a tile alone and takes 32, which fit its registers
-template <class T, int DP, int NW>
+// PLAIN: neither cap nor bias, scale > 0 (its multiplication is part of the exponent's)
+template <class T, int DP, int NW, bool PLAIN>
 __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 64 ? 1 : 2) k_attn_fwd(DofAttnFwd A) {
   constexpr int KU = NW == 1 ? 1 : 2, kKeys = 32 * KU;
   using Tile = DofTile<T, kKeys, DP>;
@@ -93,27 +94,27 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 64 ? 1 : 2) k_
 #pragma unroll
         for (int s = 0; s < KS; ++s) x[u] = dof_mma32<T>(sk[buf].rowfrag(32 * u + col, 2 * s + half), q[s], x[u]);
       }
-      float unit = 1.0f;  // of x, in log 2: the scale of plain scores is folded into the exponent's argument
-      if (sc.cap_l2 != 0.0f) {
+      if constexpr (!PLAIN) {
+        if (sc.cap_l2 != 0.0f) {
 #pragma unroll
-        for (int u = 0; u < KU; ++u)
+          for (int u = 0; u < KU; ++u)
 #pragma unroll
-          for (int v = 0; v < 16; ++v) x[u][v] = sc.cap_l2 * dof_cap_tanh<T>(x[u][v] * sc.mul);
-      } else if (A.slopes || !(sc.mul > 0.0f)) {
+            for (int v = 0; v < 16; ++v) x[u][v] = sc.cap_l2 * dof_cap_tanh<T>(x[u][v] * sc.mul);
+        } else {
 #pragma unroll
-        for (int u = 0; u < KU; ++u)
+          for (int u = 0; u < KU; ++u)
 #pragma unroll
-          for (int v = 0; v < 16; ++v) x[u][v] *= sc.mul;
-      } else {
-        unit = sc.mul;
+            for (int v = 0; v < 16; ++v) x[u][v] *= sc.mul;
+        }
+        if (A.slopes) {
+          const float base = (float)(pos - j0 - 4 * half);
+#pragma unroll
+          for (int u = 0; u < KU; ++u)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) x[u][v] -= sc.slope_l2 * fabsf(base - (float)(32 * u + 8 * (v / 4) + v % 4));
+        }
       }
-      if (A.slopes) {
-        const float base = (float)(pos - j0 - 4 * half);
-#pragma unroll
-        for (int u = 0; u < KU; ++u)
-#pragma unroll
-          for (int v = 0; v < 16; ++v) x[u][v] -= sc.slope_l2 * fabsf(base - (float)(32 * u + 8 * (v / 4) + v % 4));
-      }
+      const float unit = PLAIN ? sc.mul : 1.0f;  // of x, in log 2
       if (j0 + kKeys > wmin) {
         const int left = kend - j0 - 4 * half;
 #pragma unroll
@@ -193,11 +194,16 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 64 ? 1 : 2) k_
   if (half == 0) A.lse[(t.q0 + row) * A.q_heads + h] = l == 0.0f ? -INFINITY : (m + dof_log2(l)) * kLn2;
 }
 
+template <class T, int DP, bool PLAIN>
+void launch_as(const DofAttnFwd& A, int flat, hipStream_t stream) {
+  const unsigned blocks = (unsigned)((int64_t)A.n_tiles * A.q_heads);
+  if (flat) DOF_LAUNCH((k_attn_fwd<T, DP, 1, PLAIN>), (blocks, 1, 1), (64, 1, 1), stream, A);
+  else DOF_LAUNCH((k_attn_fwd<T, DP, 4, PLAIN>), (blocks, 1, 1), (256, 1, 1), stream, A);
+}
 template <class T, int DP>
 void launch(const DofAttnFwd& A, int flat, hipStream_t stream) {
-  const unsigned blocks = (unsigned)((int64_t)A.n_tiles * A.q_heads);
-  if (flat) DOF_LAUNCH((k_attn_fwd<T, DP, 1>), (blocks, 1, 1), (64, 1, 1), stream, A);
-  else DOF_LAUNCH((k_attn_fwd<T, DP, 4>), (blocks, 1, 1), (256, 1, 1), stream, A);
+  if (dof_attn_plain(A)) launch_as<T, DP, true>(A, flat, stream);
+  else launch_as<T, DP, false>(A, flat, stream);
 }
 
 }  // namespace

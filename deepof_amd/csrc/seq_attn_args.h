@@ -20,7 +20,14 @@ struct DofAttnBwd {
   float scale;           // d(score) / d(q.k) without the cap
   void *dq, *dk, *dv;
   int64_t gs[2], dqs[2], dks[2], dvs[2];
+  // dk / dv: a group's query heads in `splits` workgroups of `heads_per` each; more than one leave fp32 parts
+  // [dk, dv][split][key row][key head][dim] in `part`
+  int32_t splits, heads_per;
+  int64_t k_rows;
+  float* part;
 };
+
+static inline bool dof_attn_plain(const DofAttnFwd& A) { return A.score.cap_l2 == 0.0f && !A.slopes && A.score.mul > 0.0f; }
 
 int dof_launch_attn_fwd(const DofAttnFwd& A, int dtype, int flat, hipStream_t stream);
 int dof_launch_attn_dq(const DofAttnBwd& A, int dtype, int flat, hipStream_t stream);

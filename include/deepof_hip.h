@@ -522,14 +522,15 @@ int dof_norm_rope_backward(const DofNormRope* dims, const void* gq, const void* 
  * aligned) and passes both to the calls.  A plan serves any head count, head size and dtype. */
 typedef struct {
   int32_t n_docs, causal;
+  int64_t q_rows, k_rows; /* the last offsets */
   int64_t n_tiles[4];
   int64_t table_bytes;
 } DofAttnPlan;
 int dof_attn_plan_size(int32_t n_docs, const int64_t* q_off, const int64_t* k_off, int32_t causal, DofAttnPlan* plan);
 int dof_attn_plan_table(const DofAttnPlan* plan, const int64_t* q_off, const int64_t* k_off, const int32_t* prefix, void* table);
 /* head_dim: multiples of 8 from 8 to 128; every tensor and stride a multiple of 16 bytes.  lse (fp32): (query rows, q_heads),
- * natural log.  Backward: g is the gradient at o; o and lse are the forward's; the workspace holds
- * dof_attention_workspace_bytes(highest query row + 1, q_heads).  Every gradient is summed in a fixed order (no atomics). */
+ * natural log.  Backward: g is the gradient at o; o and lse are the forward's; the workspace is 16-byte aligned.  Every gradient is
+ * summed in a fixed order (no atomics). */
 typedef struct {
   int32_t dtype, head_dim, q_heads, k_heads;
   float scale, cap;
@@ -538,7 +539,7 @@ typedef struct {
 } DofAttention;
 int dof_attention_forward(const DofAttnPlan* plan, const void* table, const DofAttention* dims, const void* q, const void* k,
                           const void* v, const float* slopes, void* o, float* lse, void* stream);
-int64_t dof_attention_workspace_bytes(int64_t query_rows, int32_t q_heads);
+int64_t dof_attention_workspace_bytes(const DofAttnPlan* plan, const DofAttention* dims); /* of the backward call; -1: bad dims */
 int dof_attention_backward(const DofAttnPlan* plan, const void* table, const DofAttention* dims, const void* g, const void* q,
                            const void* k, const void* v, const float* slopes, const void* o, const float* lse, void* dq, void* dk,
                            void* dv, void* workspace, void* stream);
