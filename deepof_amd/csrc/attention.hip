@@ -130,6 +130,9 @@ Shares shares_of(const DofAttnPlan* p, const DofAttention* d) {
   return s;
 }
 
+// Small documents and heads up to 64: one kernel for all three gradients (4096 windows of 25 frames, 4 heads of 16, fp32)
+bool one_pass(const DofAttnPlan* p, const DofAttention* d) { return p->small && d->head_dim <= 64; }
+
 int64_t delta_bytes(const DofAttnPlan* p, const DofAttention* d) { return (p->q_rows * d->q_heads * 4 + 15) / 16 * 16; }
 
 DofAttnFwd forward_args(const DofAttention* d, const void* q, const void* k, const void* v, const float* slopes, void* o, float* lse) {
@@ -173,6 +176,12 @@ extern "C" int dof_attn_plan_size(int32_t n_docs, const int64_t* q_off, const in
   if (rc != DOF_OK) return rc;
   plan->n_docs = n_docs;
   plan->causal = causal != 0;
+  plan->small = 1;
+  plan->reserved = 0;
+  for (int32_t i = 0; i < n_docs; ++i) {
+    const int64_t lq = q_off[i + 1] - q_off[i], lk = k_off[i + 1] - k_off[i];
+    if (lq > kAttnFlat || lk > kAttnFlat || (lq > 0 && lk == 0)) plan->small = 0;
+  }
   plan->q_rows = n_docs ? q_off[n_docs] : 0;
   plan->k_rows = n_docs ? k_off[n_docs] : 0;
   plan->n_tiles[0] = count_tiles(n_docs, q_off, kAttnTall);
@@ -241,6 +250,7 @@ extern "C" int dof_attention_forward(const DofAttnPlan* plan, const void* table,
 extern "C" int64_t dof_attention_workspace_bytes(const DofAttnPlan* plan, const DofAttention* d) {
   static const char none = 0;
   if (check(plan, &none, d, "dof_attention_workspace_bytes") != DOF_OK) return -1;
+  if (one_pass(plan, d)) return 0;
   const Shares s = shares_of(plan, d);
   return delta_bytes(plan, d) + (s.splits > 1 ? 2 * s.splits * plan->k_rows * d->k_heads * d->head_dim * 4 : 0);
 }
@@ -252,7 +262,8 @@ extern "C" int dof_attention_backward(const DofAttnPlan* plan, const void* table
   if (rc != DOF_OK) return rc;
   const bool rows = plan->n_tiles[0] > 0, keys = plan->n_tiles[2] > 0;
   if (!rows && !keys) return DOF_OK;
-  if (!workspace || (rows && (!g || !q || !o || !lse || !dq)) || (keys && (!k || !v || !dk || !dv))) {
+  const bool one = one_pass(plan, d);
+  if ((!one && !workspace) || (rows && (!g || !q || !o || !lse || !dq)) || (keys && (!k || !v || !dk || !dv))) {
     dof_set_error("dof_attention_backward: null tensor");
     return DOF_ERR_ARG;
   }
@@ -277,6 +288,10 @@ extern "C" int dof_attention_backward(const DofAttnPlan* plan, const void* table
     B.dqs[i] = d->dq_stride[i];
     B.dks[i] = d->dk_stride[i];
     B.dvs[i] = d->dv_stride[i];
+  }
+  if (one) {
+    set_tiles(&B.f, plan, table, 2, 1);
+    return dof_launch_attn_bwd_one(B, d->dtype, (hipStream_t)stream);
   }
   if (rows) {
     const int flat = flat_tiles(plan, 0, d->q_heads);

@@ -32,7 +32,8 @@ template <> struct Lift<DofF16> {
 template <class T, int DP, int NW, bool PLAIN>
 __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_attn_dq(DofAttnBwd B) {
   const DofAttnFwd& A = B.f;
-  constexpr int KU = NW == 1 ? 1 : 2, kKeys = 32 * KU;  // keys per step, as in the forward
+  // keys per step: 64 where two wavefronts per SIMD still fit (heads of 96: 162 us with 64, 174 with 32; of 128: 2.4 ms and 1.77)
+  constexpr int KU = NW == 4 && DP == 96 ? 2 : 1, kKeys = 32 * KU;
   using Tile = DofTile<T, kKeys, DP>;
   using Stage = DofStage<T, kKeys, DP, 64 * NW>;
   __shared__ Tile sk[2], sv[2];
@@ -158,6 +159,163 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_
         const float r[4] = {dq[d][v] * out, dq[d][v + 1] * out, dq[d][v + 2] * out, dq[d][v + 3] * out};
         dof_store_vec<T, 4>(dqp + e, r);
       }
+    }
+}
+
+// Documents of at most 32 query rows and 32 keys: all three gradients from one pass of one wavefront per document and key head.  S and dP
+// are computed once (five products), q, k, v, o and g are read once and delta never leaves the workgroup.  dS turns from "lane = key"
+// to "lane = query" through LDS for dq; dk and dv add up over the group's query heads in registers.
+template <class T, int DP, bool PLAIN>
+__global__ void __launch_bounds__(64, DP <= 32 ? 2 : 1) k_attn_bwd_one(DofAttnBwd B) {
+  const DofAttnFwd& A = B.f;
+  constexpr int KS = DP / 16, DT = (DP + 31) / 32;
+  using Tile = DofTile<T, 32, 32 * DT>;
+  using Stage = DofStage<T, 32, 32 * DT, 64>;
+  __shared__ Tile sq, sg, sk;
+  __shared__ DofTile<T, 32, 32> sds;  // dS, [query][key]
+  alignas(16) __shared__ float sl[32];
+  alignas(16) __shared__ float sd[32];
+  const int lane = threadIdx.x, col = lane & 31, half = lane >> 5;
+  const int group = A.q_heads / A.k_heads;
+  int tile, hk;
+  dof_attn_item(blockIdx.x, A.n_tiles, A.k_heads, &tile, &hk);
+  const DofAttnTile t = A.tiles[tile];
+  const int off = t.lk - t.lq;
+  const bool live = col < t.lk, row = col < t.lq;
+
+  const T* kp = static_cast<const T*>(A.k) + t.k0 * A.ks[0] + hk * A.ks[1];
+  const T* vp = static_cast<const T*>(A.v) + (t.k0 + col) * A.vs[0] + hk * A.vs[1];
+  Stage rq, rg, rk;
+  rk.load(kp, A.ks[0], t.lk, A.dim, lane);
+  DofFrag<T> vf[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int e = 16 * s + 8 * half;
+    vf[s] = dof_frag_zero<T>();
+    if (live && e < A.dim) vf[s] = dof_frag_load<T>(vp + e);
+  }
+  rk.store(sk, lane);
+  dof_f32x16 dk[DT], dv[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d) dk[d] = dv[d] = dof_zero16();
+  // the first row that sees the lane's key
+  const int mine = !A.causal || col < t.prefix || col - off < 0 ? 0 : col - off;
+
+  for (int h = hk * group; h < (hk + 1) * group; ++h) {
+    rq.load(static_cast<const T*>(A.q) + t.q0 * A.qs[0] + h * A.qs[1], A.qs[0], t.lq, A.dim, lane);
+    rg.load(static_cast<const T*>(B.g) + t.q0 * B.gs[0] + h * B.gs[1], B.gs[0], t.lq, A.dim, lane);
+    const T* op = static_cast<const T*>(A.o) + (t.q0 + col) * A.os[0] + h * A.os[1];
+    DofFrag<T> of[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int e = 16 * s + 8 * half;
+      of[s] = dof_frag_zero<T>();
+      if (row && e < A.dim) of[s] = dof_frag_load<T>(op + e);
+    }
+    float lse2 = INFINITY;
+    if (row) lse2 = A.lse[(t.q0 + col) * A.q_heads + h] * kLog2e;
+    if (lse2 == -INFINITY) lse2 = INFINITY;  // a row without keys takes no part
+    __syncthreads();  // the previous head's reads are done
+    rq.store(sq, lane);
+    rg.store(sg, lane);
+    __syncthreads();
+    float delta = 0.0f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      float a[8], b[8];
+      dof_frag_unpack<T>(sg.rowfrag(col, 2 * s + half), a);
+      dof_frag_unpack<T>(of[s], b);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) delta = fmaf(a[i], b[i], delta);
+    }
+    delta += dof_swap32(delta);
+    if (half == 0) {
+      sl[col] = lse2 - Lift<T>::p2;
+      sd[col] = delta;
+    }
+    __syncthreads();
+    dof_f32x16 x = dof_zero16(), y = dof_zero16();
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      x = dof_mma32<T>(sq.rowfrag(col, 2 * s + half), sk.rowfrag(col, 2 * s + half), x);
+      y = dof_mma32<T>(sg.rowfrag(col, 2 * s + half), vf[s], y);
+    }
+    float p[16], ds[16];
+    const float slope = !PLAIN && A.slopes ? A.slopes[h] * kLog2e : 0.0f;
+    const float base = (float)(off + 4 * half - col);
+    const int left = live ? mine - 4 * half : 32;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      const int r = 8 * (v / 4) + v % 4;
+      float c = Lift<T>::ds / Lift<T>::p;
+      const float ls = sl[r + 4 * half];
+      if constexpr (PLAIN) {
+        p[v] = dof_exp2(fmaf(x[v], A.score.mul, -ls));
+      } else {
+        float w = x[v] * A.score.mul;
+        if (A.score.cap_l2 != 0.0f) {
+          const float th = dof_cap_tanh<T>(w);
+          w = A.score.cap_l2 * th;
+          c *= 1.0f - th * th;
+        }
+        if (A.slopes) w -= slope * fabsf(base + (float)r);
+        p[v] = dof_exp2(w - ls);
+      }
+      ds[v] = p[v] * c * (y[v] - sd[r + 4 * half]);
+      if (r < left) p[v] = ds[v] = 0.0f;
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const DofFrag<T> pf = dof_frag_pack<T>(p + 8 * s), df = dof_frag_pack<T>(ds + 8 * s);
+      const int r = 16 * s + 4 * half;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        dv[d] = dof_mma32<T>(sg.colfrag(r, r + 8, 32 * d + col), pf, dv[d]);
+        dk[d] = dof_mma32<T>(sq.colfrag(r, r + 8, 32 * d + col), df, dk[d]);
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      const int r = 8 * (v / 4) + v % 4 + 4 * half;
+      DofElem<T>::put(reinterpret_cast<T*>(sds.mem + sds.offset(r, col / Tile::EPC)) + col % Tile::EPC, ds[v]);
+    }
+    __syncthreads();
+    // dq (queries in registers, d over the lanes) = dS K
+    dof_f32x16 dq[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) dq[d] = dof_zero16();
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      // the eight keys of an operand are rows 16 s + 8 half .. of K, four and four
+      const DofFrag<T> f = sds.rowfrag(col, 2 * s + half);
+      const int r = 16 * s + 8 * half;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) dq[d] = dof_mma32<T>(f, sk.colfrag(r, r + 4, 32 * d + col), dq[d]);
+    }
+    const float out = B.scale / Lift<T>::ds;
+    T* dqp = static_cast<T*>(B.dq) + t.q0 * B.dqs[0] + h * B.dqs[1];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        const int r = 8 * (v / 4) + v % 4 + 4 * half, e = 32 * d + col;
+        if (r < t.lq && e < A.dim) DofElem<T>::put(dqp + r * B.dqs[0] + e, dq[d][v] * out);
+      }
+  }
+  if (!live) return;
+  T* dkp = static_cast<T*>(B.dk) + (t.k0 + col) * B.dks[0] + hk * B.dks[1];
+  T* dvp = static_cast<T*>(B.dv) + (t.k0 + col) * B.dvs[0] + hk * B.dvs[1];
+  const float ok = B.scale / Lift<T>::ds, ov = 1.0f / Lift<T>::p;
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int v = 0; v < 16; v += 4) {
+      const int e = 32 * d + 2 * v + 4 * half;
+      if (e >= A.dim) continue;
+      const float a[4] = {dk[d][v] * ok, dk[d][v + 1] * ok, dk[d][v + 2] * ok, dk[d][v + 3] * ok};
+      const float b[4] = {dv[d][v] * ov, dv[d][v + 1] * ov, dv[d][v + 2] * ov, dv[d][v + 3] * ov};
+      dof_store_vec<T, 4>(dkp + e, a);
+      dof_store_vec<T, 4>(dvp + e, b);
     }
 }
 
@@ -382,6 +540,13 @@ void launch_dkv(const DofAttnBwd& B, int flat, hipStream_t stream) {
   else launch_dkv_as<T, DP, false>(B, flat, stream);
 }
 
+template <class T, int DP>
+void launch_one(const DofAttnBwd& B, hipStream_t stream) {
+  const unsigned blocks = (unsigned)((int64_t)B.f.n_tiles * B.f.k_heads);
+  if (dof_attn_plain(B.f)) DOF_LAUNCH((k_attn_bwd_one<T, DP, true>), (blocks, 1, 1), (64, 1, 1), stream, B);
+  else DOF_LAUNCH((k_attn_bwd_one<T, DP, false>), (blocks, 1, 1), (64, 1, 1), stream, B);
+}
+
 }  // namespace
 
 int dof_launch_attn_dq(const DofAttnBwd& B, int dtype, int flat, hipStream_t stream) {
@@ -404,4 +569,13 @@ int dof_launch_attn_dkv(const DofAttnBwd& B, int dtype, int flat, hipStream_t st
       DOF_LAUNCH((k_attn_join<T>), (dof_cdiv(B.k_rows * B.f.k_heads * (B.f.dim / 4), 256), 2, 1), (256, 1, 1), stream, B);
   });
   return dof_check_launch("k_attn_dkv");
+}
+
+int dof_launch_attn_bwd_one(const DofAttnBwd& B, int dtype, hipStream_t stream) {
+  DOF_SEQ_DISPATCH(dtype, T, {
+    if (B.f.dim <= 16) launch_one<T, 16>(B, stream);
+    else if (B.f.dim <= 32) launch_one<T, 32>(B, stream);
+    else launch_one<T, 64>(B, stream);
+  });
+  return dof_check_launch("k_attn_bwd_one");
 }

@@ -19,15 +19,17 @@
 
 namespace {
 
-// keys per step: 64; a single wavefront stages a tile alone and takes 32, which fit its registers
+// Keys per step: 32, or 64 for heads over 64 (24 ragged recordings, heads of 64: 236 us with 64, 199 with 32, which leave room for four
+// wavefronts per SIMD; 16384 frames, heads of 128: 1.40 ms with 64, 1.48 with 32: two wavefronts either way).  A single wavefront takes
+// 32 and one LDS image: nobody else waits for it, and the smaller image lets more of them onto a CU.
 // PLAIN: neither cap nor bias, scale > 0 (its multiplication is part of the exponent's)
 template <class T, int DP, int NW, bool PLAIN>
-__global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 64 ? 1 : 2) k_attn_fwd(DofAttnFwd A) {
-  constexpr int KU = NW == 1 ? 1 : 2, kKeys = 32 * KU;
-  using Tile = DofTile<T, kKeys, DP>;
-  using Stage = DofStage<T, kKeys, DP, 64 * NW>;
-  __shared__ Tile sk[2], sv[2];
-  constexpr int KS = DP / 16, DT = DP / 32;
+__global__ void __launch_bounds__(64 * NW, DP <= 32 ? (NW == 1 && sizeof(T) == 4 ? 3 : 4) : sizeof(T) == 4 && DP > 64 ? 1 : 2) k_attn_fwd(DofAttnFwd A) {
+  constexpr int KU = NW == 1 || DP <= 64 ? 1 : 2, kKeys = 32 * KU, BUF = NW == 1 ? 1 : 2;
+  constexpr int KS = DP / 16, DT = (DP + 31) / 32;  // DP = 16: half of the only 32-wide tile of d is padding
+  using Tile = DofTile<T, kKeys, 32 * DT>;
+  using Stage = DofStage<T, kKeys, 32 * DT, 64 * NW>;
+  __shared__ Tile sk[BUF], sv[BUF];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
   int tile, h;
   dof_attn_item(blockIdx.x, A.n_tiles, A.q_heads, &tile, &h);
@@ -79,7 +81,7 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 64 ? 1 : 2) k_
     rk.store(sk[0], tid);
     store_v(0, 0);
   }
-  for (int j0 = 0, buf = 0; j0 < kmax; j0 += kKeys, buf ^= 1) {
+  for (int j0 = 0, buf = 0; j0 < kmax; j0 += kKeys, buf ^= BUF - 1) {
     __syncthreads();
     const int next = j0 + kKeys;
     if (next < kmax) {
@@ -160,8 +162,9 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 64 ? 1 : 2) k_
       }
     }
     if (next < kmax) {
-      rk.store(sk[buf ^ 1], tid);
-      store_v(buf ^ 1, next);
+      if (BUF == 1) __syncthreads();
+      rk.store(sk[buf ^ (BUF - 1)], tid);
+      store_v(buf ^ (BUF - 1), next);
     }
   }
 
@@ -210,7 +213,8 @@ void launch(const DofAttnFwd& A, int flat, hipStream_t stream) {
 
 int dof_launch_attn_fwd(const DofAttnFwd& A, int dtype, int flat, hipStream_t stream) {
   DOF_SEQ_DISPATCH(dtype, T, {
-    if (A.dim <= 32) launch<T, 32>(A, flat, stream);
+    if (A.dim <= 16) launch<T, 16>(A, flat, stream);
+    else if (A.dim <= 32) launch<T, 32>(A, flat, stream);
     else if (A.dim <= 64) launch<T, 64>(A, flat, stream);
     else if (A.dim <= 96) launch<T, 96>(A, flat, stream);
     else launch<T, 128>(A, flat, stream);

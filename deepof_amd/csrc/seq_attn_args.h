@@ -32,3 +32,4 @@ static inline bool dof_attn_plain(const DofAttnFwd& A) { return A.score.cap_l2 =
 int dof_launch_attn_fwd(const DofAttnFwd& A, int dtype, int flat, hipStream_t stream);
 int dof_launch_attn_dq(const DofAttnBwd& A, int dtype, int flat, hipStream_t stream);
 int dof_launch_attn_dkv(const DofAttnBwd& A, int dtype, int flat, hipStream_t stream);
+int dof_launch_attn_bwd_one(const DofAttnBwd& B, int dtype, hipStream_t stream);  // heads of at most 64

@@ -522,7 +522,8 @@ int dof_norm_rope_backward(const DofNormRope* dims, const void* gq, const void* 
  * aligned) and passes both to the calls.  A plan serves any head count, head size and dtype. */
 typedef struct {
   int32_t n_docs, causal;
-  int64_t q_rows, k_rows; /* the last offsets */
+  int32_t small, reserved; /* 1: no document has more than 32 rows or keys, or rows without any key */
+  int64_t q_rows, k_rows;  /* the last offsets */
   int64_t n_tiles[4];
   int64_t table_bytes;
 } DofAttnPlan;

@@ -102,6 +102,8 @@ CASES = [
     ([70], [5], 2, 2, 16, True, [3], 0.0, False, "plain"),             # ... whose prefix gives them some
     ([0, 6, 0], [3, 6, 0], 1, 1, 16, False, None, 0.0, False, "plain"),  # keys without rows
     ([130, 35], None, 2, 1, 96, True, None, 0.0, False, "odd"),
+    ([32, 7, 25], [32, 30, 25], 4, 2, 64, True, [0, 3, 9], 6.0, True, "packed"),  # small documents: one backward kernel
+    ([3, 0, 31], [32, 4, 1], 6, 1, 40, False, None, 0.0, False, "plain"),
 ]
 
 
