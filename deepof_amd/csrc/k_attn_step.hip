@@ -9,7 +9,9 @@
 //
 // Inside a wavefront the products are transposed as in the forward pass (S^T = K Q^T, O^T = V^T P^T): keys go from memory straight
 // into the operand registers (a lane's 16 bytes are eight elements of one key), values through a wavefront-private LDS tile for the
-// transposing read, and the next tile's loads and page lookups are in flight under the present one's products.
+// transposing read, and the next tile's loads and page lookups are in flight under the present one's products.  A lane looks up one
+// frame of a round and loads half of that frame's value itself, so that a round's loads are one address and fixed offsets per lane
+// (with an address per load the address arithmetic took longer than the loads: 64 streams of up to 5000 frames 201 us).
 // New frames are read from k and v, not from the cache, so storing them (by the first workgroup of a stream's head) races with nobody.
 #include <cmath>
 #include <cstring>
@@ -22,7 +24,7 @@
 namespace {
 
 constexpr int kStepKeys = 32;   // frames per wavefront and round
-constexpr int kMinTiles = 8;    // rounds worth a workgroup of their own: two per wavefront
+constexpr int kMinTiles = 16;   // rounds worth a workgroup of their own: four per wavefront
 constexpr int kMaxSplits = 512;
 
 struct Step {
@@ -35,45 +37,54 @@ struct Step {
   void* o;
   float* part;    // [stream][key head][split][row][dim] unnormalised sums, then [..][row][2] maximum and sum
   float* stat;
-  int32_t splits, rows, row_blocks;
+  int32_t splits, rows, row_blocks, page_shift;  // page_shift: log2 of the page size, -1 if it is no power of two
 };
 
-// Where a frame lives: page >= 0 and its slot there, a new frame (kFresh, its number), or nowhere.
-constexpr int kNowhere = -1, kFresh = -2;
-struct Slot { int page, at; };
-__device__ __forceinline__ Slot find_slot(const Step& A, const int32_t* table, int len, int total, int key) {
-  Slot s = {kNowhere, 0};
-  if (key >= total) return s;
-  const int p = key / A.d.page_size, page = table[p];
-  if (page < 0 || page >= A.d.n_pages) return s;
-  s.page = key < len ? page : kFresh;
-  s.at = key < len ? key - p * A.d.page_size : key - len;
-  return s;
+// the page of frame `key` and its slot there; page -1: nowhere
+__device__ __forceinline__ int find_page(const Step& A, const int32_t* table, int total, int key, int* slot) {
+  if (key >= total) return -1;
+  const int p = A.page_shift >= 0 ? key >> A.page_shift : key / A.d.page_size, page = table[p];
+  *slot = key - p * A.d.page_size;
+  return page >= 0 && page < A.d.n_pages ? page : -1;
 }
 
-struct Rows {  // one of the two cached tensors and its new frames, of one stream and head
-  const char *cache, *fresh;
-  int64_t page, slot, step;  // strides in bytes
-};
-template <class T> __device__ __forceinline__ const T* row_at(const Rows& r, int page, int at) {
-  return reinterpret_cast<const T*>(page >= 0 ? r.cache + page * r.page + at * r.slot : r.fresh + at * r.step);
+// Four elements of a row's output: the sums divided by the weights' sum, and with several new frames the infinities and NaN among the
+// values that the row sees of them (left out of the products).
+template <class T>
+__device__ __forceinline__ void finish(const Step& A, const int32_t* table, int b, int hk, int r, int e, int len, int total, float l, float* v) {
+  const int group = A.d.q_heads / A.d.k_heads, t = r / group, g = r - t * group;
+  const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // nothing seen: zeros; NaN stays NaN
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v[k] *= inv;
+  if (A.d.new_frames > 1)
+    for (int i = 0; i <= t; ++i) {
+      int slot;
+      if (find_page(A, table, total, len + i, &slot) < 0) continue;
+      const T* vn = static_cast<const T*>(A.v) + b * A.d.v_stride[0] + i * A.d.v_stride[1] + hk * A.d.v_stride[2] + e;
+      float x[4];
+      dof_load_vec<T, 4>(vn, x);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (!(fabsf(x[k]) < INFINITY)) v[k] += x[k];
+    }
+  dof_store_vec<T, 4>(static_cast<T*>(A.o) + b * A.d.o_stride[0] + t * A.d.o_stride[1] + (hk * group + g) * A.d.o_stride[2] + e, v);
 }
 
 // RT: tiles of 16 rows.  MULTI: more than one new frame.
 template <class T, int DP, int RT, bool MULTI>
-__global__ void __launch_bounds__(256) k_attn_step(Step A) {
+__global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) k_attn_step(Step A) {
   using Tile = DofTile<T, kStepKeys, DP>;
   __shared__ Tile sv[4];
   __shared__ float sm[4][16 * RT], sl[4][16 * RT];
-  constexpr int KS = DP / 32, DT = DP / 16, NV = (kStepKeys * Tile::CH + 63) / 64, EPC = Tile::EPC;
+  constexpr int KS = DP / 32, DT = DP / 16, NV = Tile::CH / 2, EPC = Tile::EPC;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, quad = lane >> 4;
   const int dim = A.d.head_dim, nnew = A.d.new_frames, group = A.d.q_heads / A.d.k_heads;
-  int64_t item = blockIdx.x;
-  const int rb = (int)(item % A.row_blocks);
+  int item = blockIdx.x;  // row block, then split, then key head, then stream
+  const int rb = item % A.row_blocks;
   item /= A.row_blocks;
-  const int split = (int)(item % A.splits);
+  const int split = item % A.splits;
   item /= A.splits;
-  const int hk = (int)(item % A.d.k_heads), b = (int)(item / A.d.k_heads);
+  const int b = item / A.d.k_heads, hk = item - b * A.d.k_heads;
 
   int len = A.lengths[b];
   if (len < 0) return;  // uniform: an idle stream
@@ -125,16 +136,11 @@ __global__ void __launch_bounds__(256) k_attn_step(Step A) {
       if (live && e < dim) q[i][s] = dof_frag_load<T>(qp + e);
     }
   }
-  Rows kr, vr;
-  {
-    const T* kc = static_cast<const T*>(A.kc) + hk * A.d.kc_stride[2];
-    const T* vc = static_cast<const T*>(A.vc) + hk * A.d.vc_stride[2];
-    const T* kn = static_cast<const T*>(A.k) + b * A.d.k_stride[0] + hk * A.d.k_stride[2];
-    const T* vn = static_cast<const T*>(A.v) + b * A.d.v_stride[0] + hk * A.d.v_stride[2];
-    const int64_t es = sizeof(T);
-    kr = {(const char*)kc, (const char*)kn, A.d.kc_stride[0] * es, A.d.kc_stride[1] * es, A.d.k_stride[1] * es};
-    vr = {(const char*)vc, (const char*)vn, A.d.vc_stride[0] * es, A.d.vc_stride[1] * es, A.d.v_stride[1] * es};
-  }
+  // byte offsets of a frame from the first element of this head in the caches; a new frame's lead to k and v themselves
+  const char* const kbase = reinterpret_cast<const char*>(static_cast<const T*>(A.kc) + hk * A.d.kc_stride[2]);
+  const char* const vbase = reinterpret_cast<const char*>(static_cast<const T*>(A.vc) + hk * A.d.vc_stride[2]);
+  const int64_t kfresh = reinterpret_cast<const char*>(static_cast<const T*>(A.k) + b * A.d.k_stride[0] + hk * A.d.k_stride[2]) - kbase;
+  const int64_t vfresh = reinterpret_cast<const char*>(static_cast<const T*>(A.v) + b * A.d.v_stride[0] + hk * A.d.v_stride[2]) - vbase;
 
   dof_f32x4 o[RT][DT];
   float m[RT], l[RT];
@@ -148,40 +154,63 @@ __global__ void __launch_bounds__(256) k_attn_step(Step A) {
 
   DofFrag<T> kf[2][KS];
   DofWords<4> vreg[NV];
-  auto slot_of = [&](int tile) { return find_slot(A, table, len, tile < tile1 ? total : 0, tile * kStepKeys + (lane & 31)); };
-  auto load = [&](Slot slot) {
+  struct Where { int page, slot; };
+  // the lane's frame of a tile (lanes l and l + 32: the same one)
+  auto look_up = [&](int tile) {
+    Where w = {-1, 0};
+    w.page = find_page(A, table, tile < tile1 ? total : 0, tile * kStepKeys + (lane & 31), &w.slot);
+    return w;
+  };
+  // Loads of a tile.  A frame that is nowhere reads the head's first one instead: its score is masked, its value made zero.  Elements
+  // behind the head size read its start: they meet zeros of q, or columns of the result that are not written.
+  auto load = [&](int tile, Where w) {
+    const int key = tile * kStepKeys + (lane & 31);
+    int64_t ko = w.page * A.d.kc_stride[0] + w.slot * A.d.kc_stride[1], vo = w.page * A.d.vc_stride[0] + w.slot * A.d.vc_stride[1];
+    ko = w.page < 0 ? 0 : ko * (int64_t)sizeof(T);
+    vo = w.page < 0 ? 0 : vo * (int64_t)sizeof(T);
+    if (w.page >= 0 && key >= len) {
+      ko = kfresh + (key - len) * A.d.k_stride[1] * (int64_t)sizeof(T);
+      vo = vfresh + (key - len) * A.d.v_stride[1] * (int64_t)sizeof(T);
+    }
+    const int lo = (int)(uint32_t)ko, hi = (int)(ko >> 32);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int page = dof_shfl_int(slot.page, 16 * u + col), at = dof_shfl_int(slot.at, 16 * u + col);
-      const T* p = row_at<T>(kr, page, at);
+      const uint32_t l32 = (uint32_t)dof_shfl_int(lo, 16 * u + col);
+      const int64_t off = ((int64_t)dof_shfl_int(hi, 16 * u + col) << 32) | l32;
+      const T* p = reinterpret_cast<const T*>(kbase + off);
 #pragma unroll
       for (int c = 0; c < KS; ++c) {
         const int e = 32 * c + 8 * quad;
-        kf[u][c] = dof_frag_zero<T>();
-        if (page != kNowhere && e < dim) kf[u][c] = dof_frag_load<T>(p + e);
+        kf[u][c] = dof_frag_load<T>(p + (e < dim ? e : 0));
       }
     }
+    const T* p = reinterpret_cast<const T*>(vbase + vo);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int e = lane + 64 * i, r = e / Tile::CH, c = e - r * Tile::CH;
-      const int page = dof_shfl_int(slot.page, r & 31), at = dof_shfl_int(slot.at, r & 31);
-#pragma unroll
-      for (int w = 0; w < 4; ++w) vreg[i].w[w] = 0u;
-      if (r < kStepKeys && page != kNowhere && c * EPC < dim) vreg[i] = *reinterpret_cast<const DofWords<4>*>(row_at<T>(vr, page, at) + c * EPC);
+      const int e = ((lane >> 5) + 2 * i) * EPC;
+      vreg[i] = *reinterpret_cast<const DofWords<4>*>(p + (e < dim ? e : 0));
     }
   };
 
   int tile = tile0 + wave;
-  Slot slot = slot_of(tile), ahead = slot_of(tile + 4);
-  load(slot);
+  Where here = look_up(tile), ahead = look_up(tile + 4);
+  load(tile, here);
   for (; tile < tile1; tile += 4) {
     const int j0 = tile * kStepKeys;
-    const uint32_t there = (uint32_t)dof_ballot(slot.page != kNowhere && lane < 32);
+    const uint32_t there = (uint32_t)dof_ballot(here.page >= 0);
+    const bool inner = there == 0xFFFFFFFFu && j0 + kStepKeys <= len + 1;  // uniform: every row sees every frame of the tile
+    if (!inner) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int e = lane + 64 * i, r = e / Tile::CH, c = e - r * Tile::CH;
-      if ((kStepKeys * Tile::CH) % 64 == 0 || r < kStepKeys) sv[wave].put(r, c, vreg[i]);
+      for (int i = 0; i < NV; ++i) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) vreg[i].w[k] = here.page >= 0 ? vreg[i].w[k] : 0u;
+        // several new frames: a later one's value is hidden from the earlier rows, whose zero weight must not meet an infinity or
+        // NaN; finish() puts such values where they are seen
+        if (MULTI && j0 + kStepKeys > len + 1) dof_make_finite<T>(vreg[i]);
+      }
     }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) sv[wave].put(lane & 31, (lane >> 5) + 2 * i, vreg[i]);
     dof_f32x4 x[RT][2];
 #pragma unroll
     for (int i = 0; i < RT; ++i)
@@ -191,28 +220,48 @@ __global__ void __launch_bounds__(256) k_attn_step(Step A) {
 #pragma unroll
         for (int c = 0; c < KS; ++c) x[i][u] = dof_mma16<T>(kf[u][c], q[i][c], x[i][u]);
       }
-    slot = ahead;
     if (tile + 4 < tile1) {  // uniform over the wavefront
-      load(slot);
-      ahead = slot_of(tile + 8);
+      here = ahead;
+      load(tile + 4, here);
+      ahead = look_up(tile + 8);
     }
     DOF_WAVE_LDS_ORDER();
     // keys 16 u + 4 quad + e of the tile, e = 0 .. 3, sit in this lane's registers
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[i][u][e] *= A.score.mul;
+      if (A.score.cap_l2 != 0.0f) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[i][u][e] = A.score.cap_l2 * dof_cap_tanh<T>(x[i][u][e]);
+      }
+      if (A.slopes) {
+        const float base = (float)(pos[i] - j0 - 4 * quad);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[i][u][e] -= slope[i] * fabsf(base - (float)(16 * u + e));
+      }
+      if (!inner) {
+        const uint32_t mine = there >> (4 * quad);
+        const int left = kend[i] - j0 - 4 * quad;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const bool seen = (16 * u + e < left) & (((mine >> (16 * u + e)) & 1u) != 0u);
+            x[i][u][e] = seen ? x[i][u][e] : -INFINITY;
+          }
+      }
       float mt = -INFINITY;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int kk = 16 * u + 4 * quad + e;
-          float w = x[i][u][e] * A.score.mul;
-          if (A.score.cap_l2 != 0.0f) w = A.score.cap_l2 * dof_cap_tanh<T>(w);
-          w -= slope[i] * fabsf((float)(pos[i] - j0 - kk));
-          if (j0 + kk >= kend[i] || !((there >> kk) & 1u)) w = -INFINITY;
-          x[i][u][e] = w;
-          mt = fmaxf(mt, w);
-        }
+        for (int e = 0; e < 4; ++e) mt = fmaxf(mt, x[i][u][e]);
       mt = fmaxf(mt, __shfl_xor(mt, 16));
       mt = fmaxf(mt, dof_swap32(mt));
       if (dof_wave_any(mt > m[i] + 8.0f)) {  // as in the forward pass: the maximum follows in steps of 2^8
@@ -235,43 +284,14 @@ __global__ void __launch_bounds__(256) k_attn_step(Step A) {
           l[i] += p[4 * u + e];
         }
       const DofFrag<T> pf = dof_frag_pack<T>(p);
-      // several new frames: a later one's value is hidden from the earlier rows, whose zero weight must not meet an infinity or NaN
-      bool careful = false;
-      if (MULTI && j0 + kStepKeys > len + 1) {
-        bool bad = false;
 #pragma unroll
-        for (int d = 0; d < DT; ++d) bad |= dof_frag_nonfinite<T>(sv[wave].colfrag(4 * quad, 16 + 4 * quad, 16 * d + col));
-        careful = dof_wave_any(bad);
-      }
-      if (!careful) {
-#pragma unroll
-        for (int d = 0; d < DT; ++d) o[i][d] = dof_mma16<T>(sv[wave].colfrag(4 * quad, 16 + 4 * quad, 16 * d + col), pf, o[i][d]);
-      } else {
-        float seen[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int kk = 16 * (e / 4) + 4 * quad + e % 4;
-          seen[e] = j0 + kk < kend[i] && ((there >> kk) & 1u) ? 1.0f : 0.0f;
-        }
-        const DofFrag<T> sf = dof_frag_pack<T>(seen);
-#pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          DofFrag<T> f = sv[wave].colfrag(4 * quad, 16 + 4 * quad, 16 * d + col), pos_f, neg_f;
-          dof_frag_split<T>(f, pos_f, neg_f);
-          o[i][d] = dof_mma16<T>(f, pf, o[i][d]);
-          const dof_f32x4 up = dof_mma16<T>(pos_f, sf, dof_zero4()), down = dof_mma16<T>(neg_f, sf, dof_zero4());
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (up[e] > 0.0f) o[i][d][e] += INFINITY;
-            if (down[e] > 0.0f) o[i][d][e] -= INFINITY;
-          }
-        }
-      }
+      for (int d = 0; d < DT; ++d) o[i][d] = dof_mma16<T>(sv[wave].colfrag(4 * quad, 16 + 4 * quad, 16 * d + col), pf, o[i][d]);
     }
     DOF_WAVE_LDS_ORDER();
   }
 
-  // the four wavefronts meet: a common maximum, then their sums one after the other
+  // The four wavefronts meet in LDS: each leaves its sums in its own value tile, then every thread adds up the four of its elements,
+  // weighted to the rows' common maximum.
 #pragma unroll
   for (int i = 0; i < RT; ++i) {
     l[i] += __shfl_xor(l[i], 16);
@@ -281,78 +301,42 @@ __global__ void __launch_bounds__(256) k_attn_step(Step A) {
       sl[wave][16 * i + col] = l[i];
     }
   }
-  __syncthreads();  // also: every wavefront is done with its value tile
-  float lt[RT];
+  static_assert(sizeof(Tile) >= 16 * DP * sizeof(float), "a value tile holds sixteen rows of sums");
+  auto meet = [&](int w, int row, int c) { return reinterpret_cast<DofWords<4>*>(sv[w].mem) + row * (DP / 4) + (c ^ (row & 7)); };
 #pragma unroll
   for (int i = 0; i < RT; ++i) {
-    float mn = -INFINITY;
+    if (i > 0) __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 4; ++w) mn = fmaxf(mn, sm[w][16 * i + col]);
-    lt[i] = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float mw = sm[w][16 * i + col];
-      lt[i] += mw == -INFINITY ? sl[w][16 * i + col] : sl[w][16 * i + col] * dof_exp2(mw - mn);
-    }
-    const float a = m[i] == -INFINITY ? 1.0f : dof_exp2(m[i] - mn);  // -inf: nothing seen, the sums are zeros (or NaN)
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[i][d][e] *= a;
-    m[i] = mn;
-  }
-  float* meet = reinterpret_cast<float*>(sv);  // [16 RT rows][DP]
-  static_assert(sizeof(sv) >= 16 * RT * DP * sizeof(float), "the value tiles hold the meeting place");
-  for (int w = 1; w < 4; ++w) {
-    if (wave == w) {
-#pragma unroll
-      for (int i = 0; i < RT; ++i)
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) meet[(16 * i + col) * DP + 16 * d + 4 * quad + e] = o[i][d][e];
+    for (int d = 0; d < DT; ++d) {
+      const float v[4] = {o[i][d][0], o[i][d][1], o[i][d][2], o[i][d][3]};
+      DofElem<float>::pack(v, *meet(wave, col, 4 * d + quad));
     }
     __syncthreads();
-    if (wave == 0) {
+    for (int e4 = tid; e4 < 4 * DP; e4 += 256) {
+      const int row = e4 / (DP / 4), c = e4 - row * (DP / 4), r = rb * 16 * RT + 16 * i + row, at = 16 * i + row;
+      if (r >= A.rows || 4 * c >= dim) continue;
+      float mn = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < RT; ++i)
+      for (int w = 0; w < 4; ++w) mn = fmaxf(mn, sm[w][at]);
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f}, lt = 0.0f;
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
+      for (int w = 0; w < 4; ++w) {
+        const float f = sm[w][at] == -INFINITY ? 1.0f : dof_exp2(sm[w][at] - mn);  // -inf: nothing seen, zeros (or NaN)
+        float v[4];
+        DofElem<float>::unpack(*meet(w, row, c), v);
+        lt = fmaf(f, sl[w][at], lt);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[i][d][e] += meet[(16 * i + col) * DP + 16 * d + 4 * quad + e];
-    }
-    __syncthreads();
-  }
-  if (wave != 0) return;
-#pragma unroll
-  for (int i = 0; i < RT; ++i) {
-    const int r = rb * 16 * RT + 16 * i + col;
-    if (r >= A.rows) continue;
-    if (A.splits == 1) {
-      const int t = r / group, g = r - t * group;
-      const float inv = lt[i] > 0.0f ? 1.0f / lt[i] : (lt[i] == 0.0f ? 0.0f : lt[i]);
-      T* op = static_cast<T*>(A.o) + b * A.d.o_stride[0] + t * A.d.o_stride[1] + (hk * group + g) * A.d.o_stride[2];
-#pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const int e = 16 * d + 4 * quad;
-        if (e < dim) {
-          const float v[4] = {o[i][d][0] * inv, o[i][d][1] * inv, o[i][d][2] * inv, o[i][d][3] * inv};
-          dof_store_vec<T, 4>(op + e, v);
-        }
+        for (int k = 0; k < 4; ++k) sum[k] = fmaf(f, v[k], sum[k]);
       }
-    } else {
-      const int64_t at = (((int64_t)b * A.d.k_heads + hk) * A.splits + split) * A.rows + r;
-#pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const int e = 16 * d + 4 * quad;
-        if (e < dim) {
-          const float v[4] = {o[i][d][0], o[i][d][1], o[i][d][2], o[i][d][3]};
-          dof_store_vec<float, 4>(A.part + at * dim + e, v);
+      if (A.splits == 1) {
+        finish<T>(A, table, b, hk, r, 4 * c, len, total, lt, sum);
+      } else {
+        const int64_t part = (((int64_t)b * A.d.k_heads + hk) * A.splits + split) * A.rows + r;
+        dof_store_vec<float, 4>(A.part + part * dim + 4 * c, sum);
+        if (c == 0) {
+          A.stat[part * 2] = mn;
+          A.stat[part * 2 + 1] = lt;
         }
-      }
-      if (quad == 0) {
-        A.stat[at * 2] = m[i];
-        A.stat[at * 2 + 1] = lt[i];
       }
     }
   }
@@ -364,7 +348,7 @@ __global__ void __launch_bounds__(256) k_attn_step_join(Step A) {
   __shared__ float so[8][128];
   __shared__ float sw[kMaxSplits];
   __shared__ float red[4][2];
-  const int tid = threadIdx.x, dim = A.d.head_dim, group = A.d.q_heads / A.d.k_heads;
+  const int tid = threadIdx.x, dim = A.d.head_dim;
   int64_t item = blockIdx.x;
   const int r = (int)(item % A.rows);
   item /= A.rows;
@@ -411,15 +395,11 @@ __global__ void __launch_bounds__(256) k_attn_step_join(Step A) {
   for (int i = 0; i < 4; ++i) so[grp][e + i] = acc[i];
   __syncthreads();
   if (tid < 32 && e < dim) {
-    const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
     float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int g = 0; g < 8; ++g)
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] += so[g][e + i];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] *= inv;
-    const int t = r / group, g = r - t * group;
-    dof_store_vec<T, 4>(static_cast<T*>(A.o) + b * A.d.o_stride[0] + t * A.d.o_stride[1] + (hk * group + g) * A.d.o_stride[2] + e, v);
+    finish<T>(A, A.table + (int64_t)b * A.d.max_pages, b, hk, r, e, len, total, sum, v);
   }
 }
 
@@ -461,7 +441,7 @@ Shape shape_of(const DofAttnStep* d) {
   s.row_blocks = (s.rows + 16 * s.rt - 1) / (16 * s.rt);
   const int64_t base = (int64_t)d->streams * d->k_heads * s.row_blocks;
   const int64_t tiles = ((int64_t)d->max_pages * d->page_size + kStepKeys - 1) / kStepKeys;
-  int64_t want = base > 0 ? (4096 + base - 1) / base : 1;
+  int64_t want = base > 0 ? (2048 + base - 1) / base : 1;
   const int64_t most = (tiles + kMinTiles - 1) / kMinTiles;
   if (want > most) want = most;
   if (want > kMaxSplits) want = kMaxSplits;
@@ -537,6 +517,9 @@ extern "C" int dof_attention_step(const DofAttnStep* d, const void* q, const voi
   A.splits = s.splits;
   A.rows = s.rows;
   A.row_blocks = s.row_blocks;
+  A.page_shift = -1;
+  if ((d->page_size & (d->page_size - 1)) == 0)
+    while ((int64_t)1 << (A.page_shift + 1) <= d->page_size) ++A.page_shift;
   DOF_SEQ_DISPATCH(d->dtype, T, {
     if (d->head_dim <= 32) launch_rt<T, 32>(A, s.rt, (unsigned)blocks, (hipStream_t)stream);
     else if (d->head_dim <= 64) launch_rt<T, 64>(A, s.rt, (unsigned)blocks, (hipStream_t)stream);

@@ -58,33 +58,23 @@ template <class T> __device__ __forceinline__ void dof_frag_unpack(const DofFrag
   }
 }
 
-// Infinities and NaN inside a fragment.  any: is there one; split: the fragment with zeros in their places, and two fragments of ones
-// where +inf or NaN (pos) and where -inf or NaN (neg) stood.
-template <class T> __device__ __forceinline__ bool dof_frag_nonfinite(const DofFrag<T>& f) {
-  bool bad = false;
-  if constexpr (sizeof(T) == 4) {
+// Sixteen bytes of elements with zeros in the place of infinities and NaN; were there any?
+template <class T> __device__ __forceinline__ bool dof_make_finite(DofWords<4>& v) {
+  bool any = false;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) bad |= (__builtin_bit_cast(uint32_t, f.v[i]) & 0x7F800000u) == 0x7F800000u;
-  } else {
-    constexpr uint32_t e = std::is_same<T, DofBf16>::value ? 0x7F80u : 0x7C00u;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) bad |= (f.w[i] & e) == e || (f.w[i] & (e << 16)) == (e << 16);
+  for (int k = 0; k < 4; ++k) {
+    if constexpr (sizeof(T) == 4) {
+      const bool bad = (v.w[k] & 0x7F800000u) == 0x7F800000u;
+      any |= bad;
+      if (bad) v.w[k] = 0u;
+    } else {
+      constexpr uint32_t m = std::is_same<T, DofBf16>::value ? 0x7F80u : 0x7C00u;
+      const bool lo = (v.w[k] & m) == m, hi = (v.w[k] & (m << 16)) == (m << 16);
+      any |= lo || hi;
+      v.w[k] &= (lo ? 0xFFFF0000u : 0xFFFFFFFFu) & (hi ? 0x0000FFFFu : 0xFFFFFFFFu);
+    }
   }
-  return bad;
-}
-template <class T> __device__ __forceinline__ void dof_frag_split(DofFrag<T>& f, DofFrag<T>& pos, DofFrag<T>& neg) {
-  float v[8], a[8], b[8];
-  dof_frag_unpack<T>(f, v);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const bool bad = !(fabsf(v[i]) < INFINITY);
-    a[i] = bad && !(v[i] < 0.0f) ? 1.0f : 0.0f;
-    b[i] = bad && !(v[i] > 0.0f) ? 1.0f : 0.0f;
-    v[i] = bad ? 0.0f : v[i];
-  }
-  f = dof_frag_pack<T>(v);
-  pos = dof_frag_pack<T>(a);
-  neg = dof_frag_pack<T>(b);
+  return any;
 }
 
 // c (32 x 32) += a (32 x 16) b (16 x 32); register v of lane l: row 8 (v / 4) + 4 (l >> 5) + v % 4, column l & 31
@@ -208,19 +198,7 @@ template <class T, int ROWS, int DP, int NT> struct DofStage {
     for (int i = 0; i < N; ++i) {
       const int e = tid + i * NT, r = e / Tile::CH, c = e - r * Tile::CH;
       DofWords<4> v = reg[i];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if constexpr (sizeof(T) == 4) {
-          const bool bad = (v.w[k] & 0x7F800000u) == 0x7F800000u;
-          any |= bad;
-          if (bad) v.w[k] = 0u;
-        } else {
-          constexpr uint32_t m = std::is_same<T, DofBf16>::value ? 0x7F80u : 0x7C00u;
-          const bool lo = (v.w[k] & m) == m, hi = (v.w[k] & (m << 16)) == (m << 16);
-          any |= lo || hi;
-          v.w[k] &= (lo ? 0xFFFF0000u : 0xFFFFFFFFu) & (hi ? 0x0000FFFFu : 0xFFFFFFFFu);
-        }
-      }
+      any |= dof_make_finite<T>(v);
       if ((ROWS * Tile::CH) % NT == 0 || r < ROWS) t.put(r, c, v);
     }
     if (any) *found = 1;
