@@ -7,6 +7,11 @@
 // over its four wavefronts, 32 frames at a time; each keeps its own running maximum and sum.  The wavefronts meet in LDS, the
 // workgroups' partial results in the workspace, joined by k_attn_step_join.
 //
+// The lengths are device data, so the split is made on the device: every workgroup adds up the streams' lengths, takes the part size
+// that yields about kTarget parts in all and finds the stream its own part lies in.  All parts are then about equally long, whatever the
+// mix of streams, and few workgroups are left without one (a split made on the host for the longest possible stream left most of
+// them empty or the longest stream's for the end: 64 streams of up to 5000 frames 81 us).
+//
 // Inside a wavefront the products are transposed as in the forward pass (S^T = K Q^T, O^T = V^T P^T): keys go from memory straight
 // into the operand registers (a lane's 16 bytes are eight elements of one key), values through a wavefront-private LDS tile for the
 // transposing read, and the next tile's loads and page lookups are in flight under the present one's products.  A lane looks up one
@@ -24,8 +29,9 @@
 namespace {
 
 constexpr int kStepKeys = 32;   // frames per wavefront and round
-constexpr int kMinTiles = 16;   // rounds worth a workgroup of their own: four per wavefront
-constexpr int kMaxSplits = 512;
+constexpr int kMinTiles = 16;   // rounds of a part at least: four per wavefront
+constexpr int kWhole = 32;      // streams whose table holds no more rounds stay whole: a second kernel for the join costs more
+constexpr int kTarget = 1024;   // parts of a call in all: two rounds of two workgroups per CU
 
 struct Step {
   DofAttnStep d;
@@ -35,9 +41,10 @@ struct Step {
   const int32_t *table, *lengths;
   const float* slopes;
   void* o;
-  float* part;    // [stream][key head][split][row][dim] unnormalised sums, then [..][row][2] maximum and sum
-  float* stat;
-  int32_t splits, rows, row_blocks, page_shift;  // page_shift: log2 of the page size, -1 if it is no power of two
+  float* part;    // [part][key head][row][dim] unnormalised sums
+  float* stat;    // [part][key head][row][2] maximum and sum
+  int32_t* sched; // [stream][2] first part and their number
+  int32_t rows, row_blocks, min_tiles, join_lanes, page_shift;  // page_shift: log2 of the page size, -1 if it is no power of two
 };
 
 // the page of frame `key` and its slot there; page -1: nowhere
@@ -46,6 +53,72 @@ __device__ __forceinline__ int find_page(const Step& A, const int32_t* table, in
   const int p = A.page_shift >= 0 ? key >> A.page_shift : key / A.d.page_size, page = table[p];
   *slot = key - p * A.d.page_size;
   return page >= 0 && page < A.d.n_pages ? page : -1;
+}
+
+// frames of stream b after the call (0: idle)
+__device__ __forceinline__ int frames_of(const Step& A, int b, int* len) {
+  *len = A.lengths[b];
+  if (*len < 0) return 0;
+  const int64_t capacity = (int64_t)A.d.max_pages * A.d.page_size;
+  if (*len > capacity) *len = (int)capacity;
+  return (int)(*len + A.d.new_frames < capacity ? *len + A.d.new_frames : capacity);
+}
+__device__ __forceinline__ int tiles_of(const Step& A, int b) {
+  int len;
+  return (frames_of(A, b, &len) + kStepKeys - 1) / kStepKeys;
+}
+
+// The stream and the part of it that is number `unit` of all parts, and the part size in tiles; by all 256 threads.
+struct Part { int stream, index, count, per; };
+__device__ __forceinline__ Part find_part(const Step& A, int unit) {
+  __shared__ int low[4], high[4], upto_wave[4], found[3];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int mine = tid < A.d.streams ? tiles_of(A, tid) : 0;
+  auto tiles_at = [&](int b0) { return b0 == 0 ? mine : b0 + tid < A.d.streams ? tiles_of(A, b0 + tid) : 0; };
+  auto wave_sum = [&](int v) {
+    for (int k = 32; k > 0; k >>= 1) v += dof_shfl_int(v, lane ^ k);
+    return v;
+  };
+  if (tid == 0) found[0] = -1;
+  int64_t all = 0;
+  for (int b0 = 0; b0 < A.d.streams; b0 += 256) {  // in two halves of 16 bits: the sum itself may pass 32
+    if (b0 > 0) __syncthreads();
+    const int v = tiles_at(b0), lo = wave_sum(v & 0xFFFF), hi = wave_sum(v >> 16);
+    if (lane == 0) {
+      low[wave] = lo;
+      high[wave] = hi;
+    }
+    __syncthreads();
+    all += (int64_t)(low[0] + low[1] + low[2] + low[3]) + ((int64_t)(high[0] + high[1] + high[2] + high[3]) << 16);
+  }
+  const int64_t share = (all * A.d.k_heads * A.row_blocks + kTarget - 1) / kTarget;
+  Part p;
+  p.per = share > A.min_tiles ? (int)share : A.min_tiles;
+  int before = 0;
+  for (int b0 = 0; b0 < A.d.streams; b0 += 256) {
+    if (b0 > 0) __syncthreads();
+    const int n = (tiles_at(b0) + p.per - 1) / p.per;
+    int upto = n;  // inclusive sum over the wavefront
+    for (int k = 1; k < 64; k <<= 1) {
+      const int below = dof_shfl_int(upto, lane >= k ? lane - k : lane);
+      if (lane >= k) upto += below;
+    }
+    if (lane == 63) upto_wave[wave] = upto;
+    __syncthreads();
+    int first = before + upto - n;
+    for (int w = 0; w < wave; ++w) first += upto_wave[w];
+    if (n > 0 && unit >= first && unit < first + n) {
+      found[0] = b0 + tid;
+      found[1] = unit - first;
+      found[2] = n;
+    }
+    before += upto_wave[0] + upto_wave[1] + upto_wave[2] + upto_wave[3];
+  }
+  __syncthreads();
+  p.stream = found[0];
+  p.index = found[1];
+  p.count = found[2];
+  return p;
 }
 
 // Four elements of a row's output: the sums divided by the weights' sum, and with several new frames the infinities and NaN among the
@@ -79,24 +152,23 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) k_attn
   constexpr int KS = DP / 32, DT = DP / 16, NV = Tile::CH / 2, EPC = Tile::EPC;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, quad = lane >> 4;
   const int dim = A.d.head_dim, nnew = A.d.new_frames, group = A.d.q_heads / A.d.k_heads;
-  int item = blockIdx.x;  // row block, then split, then key head, then stream
+  int item = blockIdx.x;  // row block, then key head, then part
   const int rb = item % A.row_blocks;
   item /= A.row_blocks;
-  const int split = item % A.splits;
-  item /= A.splits;
-  const int b = item / A.d.k_heads, hk = item - b * A.d.k_heads;
-
-  int len = A.lengths[b];
-  if (len < 0) return;  // uniform: an idle stream
-  const int64_t capacity = (int64_t)A.d.max_pages * A.d.page_size;
-  if (len > capacity) len = (int)capacity;
-  const int total = (int)(len + nnew < capacity ? len + nnew : capacity);
+  const int unit = item / A.d.k_heads, hk = item - unit * A.d.k_heads;
+  const Part part = find_part(A, unit);
+  if (part.stream < 0) return;  // uniform: fewer parts than workgroups
+  const int b = part.stream;
+  int len;
+  const int total = frames_of(A, b, &len);
   const int tiles = (total + kStepKeys - 1) / kStepKeys;
-  int per = (tiles + A.splits - 1) / A.splits;
-  if (per < kMinTiles) per = kMinTiles;
   const int32_t* table = A.table + (int64_t)b * A.d.max_pages;
+  if (A.sched && part.index == 0 && hk == 0 && rb == 0 && tid == 0) {
+    A.sched[2 * b] = unit;
+    A.sched[2 * b + 1] = part.count;
+  }
 
-  if (split == 0 && rb == 0) {  // the new frames into the cache
+  if (part.index == 0 && rb == 0) {  // the new frames into the cache
     const int chunks = dim / EPC;
     for (int e = tid; e < nnew * chunks; e += 256) {
       const int t = e / chunks, c = e - t * chunks, at = len + t;
@@ -112,8 +184,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) k_attn
       reinterpret_cast<DofWords<4>*>(vd)[c] = reinterpret_cast<const DofWords<4>*>(vn)[c];
     }
   }
-  const int tile0 = split * per, tile1 = tile0 + per < tiles ? tile0 + per : tiles;
-  if (A.splits > 1 && tile0 >= tile1 && split > 0) return;  // uniform; the join knows which parts exist
+  const int tile0 = part.index * part.per, tile1 = tile0 + part.per < tiles ? tile0 + part.per : tiles;
 
   // rows of this block: row r = new frame r / group, head r % group of the key head's group
   int kend[RT];
@@ -328,77 +399,79 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) k_attn
 #pragma unroll
         for (int k = 0; k < 4; ++k) sum[k] = fmaf(f, v[k], sum[k]);
       }
-      if (A.splits == 1) {
+      if (part.count == 1) {
         finish<T>(A, table, b, hk, r, 4 * c, len, total, lt, sum);
       } else {
-        const int64_t part = (((int64_t)b * A.d.k_heads + hk) * A.splits + split) * A.rows + r;
-        dof_store_vec<float, 4>(A.part + part * dim + 4 * c, sum);
+        const int64_t to = ((int64_t)unit * A.d.k_heads + hk) * A.rows + r;
+        dof_store_vec<float, 4>(A.part + to * dim + 4 * c, sum);
         if (c == 0) {
-          A.stat[part * 2] = mn;
-          A.stat[part * 2 + 1] = lt;
+          A.stat[to * 2] = mn;
+          A.stat[to * 2 + 1] = lt;
         }
       }
     }
   }
 }
 
-// o of one row from its parts: a workgroup per row, eight groups of 32 lanes (four elements each) share the parts.
+// o of the streams in several parts: a workgroup per row, groups of 32 lanes (four elements each) share the parts, four loads in flight
+// each.  Few rows (of long streams, in many parts): a workgroup per row and 32 elements, groups of 8 lanes.
 template <class T>
 __global__ void __launch_bounds__(256) k_attn_step_join(Step A) {
-  __shared__ float so[8][128];
-  __shared__ float sw[kMaxSplits];
+  __shared__ float so[1152];  // [groups][4 lanes + 4]: 32 x 36 or 8 x 132
   __shared__ float red[4][2];
-  const int tid = threadIdx.x, dim = A.d.head_dim;
-  int64_t item = blockIdx.x;
-  const int r = (int)(item % A.rows);
+  const int tid = threadIdx.x, dim = A.d.head_dim, lanes = A.join_lanes, groups = 256 / lanes, pitch = 4 * lanes + 4;
+  int item = blockIdx.x;
+  const int r = item % A.rows;
   item /= A.rows;
-  const int hk = (int)(item % A.d.k_heads), b = (int)(item / A.d.k_heads);
-  int len = A.lengths[b];
-  if (len < 0) return;
-  const int64_t capacity = (int64_t)A.d.max_pages * A.d.page_size;
-  if (len > capacity) len = (int)capacity;
-  const int total = (int)(len + A.d.new_frames < capacity ? len + A.d.new_frames : capacity);
-  const int tiles = (total + kStepKeys - 1) / kStepKeys;
-  int per = (tiles + A.splits - 1) / A.splits;
-  if (per < kMinTiles) per = kMinTiles;
-  int parts = (tiles + per - 1) / per;
-  if (parts < 1) parts = 1;
-  const int64_t base = ((int64_t)b * A.d.k_heads + hk) * A.splits;
+  const int b = item / A.d.k_heads, hk = item - b * A.d.k_heads;
+  int len;
+  const int total = frames_of(A, b, &len);
+  if (total == 0) return;
+  const int first = A.sched[2 * b], parts = A.sched[2 * b + 1];
+  if (parts == 1) return;  // written by its only workgroup
+  auto at = [&](int s) { return ((int64_t)(first + s) * A.d.k_heads + hk) * A.rows + r; };
 
   float mx = -INFINITY;
-  for (int s = tid; s < parts; s += 256) mx = fmaxf(mx, A.stat[((base + s) * A.rows + r) * 2]);
+  for (int s = tid; s < parts; s += 256) mx = fmaxf(mx, A.stat[at(s) * 2]);
   for (int k = 32; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor(mx, k));
   if ((tid & 63) == 0) red[tid >> 6][0] = mx;
   __syncthreads();
   mx = fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0]));
+  auto weight = [&](float m) { return m == -INFINITY ? 1.0f : dof_exp2(m - mx); };  // -inf: nothing seen, zeros (or NaN)
   float sum = 0.0f;
-  for (int s = tid; s < parts; s += 256) {
-    const float* st = A.stat + ((base + s) * A.rows + r) * 2;
-    const float w = st[0] == -INFINITY ? 1.0f : dof_exp2(st[0] - mx);
-    sw[s] = w;
-    sum += w * st[1];
-  }
+  for (int s = tid; s < parts; s += 256) sum = fmaf(weight(A.stat[at(s) * 2]), A.stat[at(s) * 2 + 1], sum);
   for (int k = 32; k > 0; k >>= 1) sum += __shfl_xor(sum, k);
   if ((tid & 63) == 0) red[tid >> 6][1] = sum;
+  const int l = tid & (lanes - 1), e = 4 * (lanes * (int)blockIdx.y + l), grp = tid / lanes;
+  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (e < dim) {
+    for (int s0 = grp; s0 < parts; s0 += 4 * groups) {
+      float v[4][4], w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const bool in = s0 + groups * k < parts;
+        const int64_t from = at(in ? s0 + groups * k : s0);
+        dof_load_vec<float, 4>(A.part + from * dim + e, v[k]);
+        w[k] = A.stat[from * 2];
+        if (!in) v[k][0] = v[k][1] = v[k][2] = v[k][3] = 0.0f;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float f = weight(w[k]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] = fmaf(f, v[k][i], acc[i]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) so[grp * pitch + 4 * l + i] = acc[i];
   __syncthreads();
   sum = (red[0][1] + red[1][1]) + (red[2][1] + red[3][1]);
-  const int e = 4 * (tid & 31), grp = tid >> 5;
-  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (e < dim)
-    for (int s = grp; s < parts; s += 8) {
-      float v[4];
-      dof_load_vec<float, 4>(A.part + ((base + s) * A.rows + r) * dim + e, v);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i] = fmaf(sw[s], v[i], acc[i]);
-    }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) so[grp][e + i] = acc[i];
-  __syncthreads();
-  if (tid < 32 && e < dim) {
+  if (tid < lanes && e < dim) {
     float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int g = 0; g < 8; ++g)
+    for (int g = 0; g < groups; ++g)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] += so[g][e + i];
+      for (int i = 0; i < 4; ++i) v[i] += so[g * pitch + 4 * l + i];
     finish<T>(A, A.table + (int64_t)b * A.d.max_pages, b, hk, r, e, len, total, sum, v);
   }
 }
@@ -430,24 +503,23 @@ int check(const DofAttnStep* d, const char* who) {
   return DOF_OK;
 }
 
-// Row tiles of 16 per workgroup (1 or 2), blocks of them, and parts of a stream's length: enough workgroups to fill the chip and to
-// even out streams of different length, none smaller than two rounds per wavefront.  From the table's width: the lengths themselves
-// are device data (a workgroup whose part is empty ends at once).
-struct Shape { int rows, rt, row_blocks, splits; };
+// Row tiles of 16 per workgroup (1 or 2), blocks of them, and the most parts that find_part can make of the streams: each at most
+// one more than its share, and no more than its table holds.
+struct Shape { int rows, rt, row_blocks, min_tiles; int64_t parts; };
 Shape shape_of(const DofAttnStep* d) {
   Shape s;
   s.rows = d->q_heads / d->k_heads * d->new_frames;
   s.rt = s.rows > 16 ? 2 : 1;
   s.row_blocks = (s.rows + 16 * s.rt - 1) / (16 * s.rt);
-  const int64_t base = (int64_t)d->streams * d->k_heads * s.row_blocks;
   const int64_t tiles = ((int64_t)d->max_pages * d->page_size + kStepKeys - 1) / kStepKeys;
-  int64_t want = base > 0 ? (2048 + base - 1) / base : 1;
-  const int64_t most = (tiles + kMinTiles - 1) / kMinTiles;
-  if (want > most) want = most;
-  if (want > kMaxSplits) want = kMaxSplits;
-  s.splits = (int)(want < 1 ? 1 : want);
+  s.min_tiles = tiles <= kWhole ? kWhole : kMinTiles;
+  s.parts = d->streams + kTarget / ((int64_t)d->k_heads * s.row_blocks);
+  const int64_t most = (tiles + s.min_tiles - 1) / s.min_tiles * d->streams;
+  if (s.parts > most) s.parts = most;
   return s;
 }
+bool joins(const DofAttnStep* d, const Shape& s) { return s.parts > d->streams; }
+int64_t part_floats(const DofAttnStep* d, const Shape& s) { return s.parts * d->k_heads * s.rows * d->head_dim; }
 
 bool aligned(const void* p, const int64_t* s, int size) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && s[0] * size % 16 == 0 && s[1] * size % 16 == 0 && s[2] * size % 16 == 0;
@@ -467,8 +539,8 @@ void launch_rt(const Step& A, int rt, unsigned blocks, hipStream_t stream) {
 extern "C" int64_t dof_attention_step_workspace_bytes(const DofAttnStep* d) {
   if (check(d, "dof_attention_step_workspace_bytes") != DOF_OK) return -1;
   const Shape s = shape_of(d);
-  if (s.splits == 1) return 0;
-  return (int64_t)d->streams * d->k_heads * s.splits * s.rows * (d->head_dim + 2) * 4;
+  if (!joins(d, s)) return 0;
+  return (part_floats(d, s) + s.parts * d->k_heads * s.rows * 2 + 2 * (int64_t)d->streams) * 4;
 }
 
 extern "C" int dof_attention_step(const DofAttnStep* d, const void* q, const void* k, const void* v, void* k_cache, void* v_cache,
@@ -478,7 +550,7 @@ extern "C" int dof_attention_step(const DofAttnStep* d, const void* q, const voi
   if (rc != DOF_OK) return rc;
   if (d->streams == 0) return DOF_OK;
   const Shape s = shape_of(d);
-  if (!q || !k || !v || !k_cache || !v_cache || !page_table || !lengths || !o || (s.splits > 1 && !workspace)) {
+  if (!q || !k || !v || !k_cache || !v_cache || !page_table || !lengths || !o || (joins(d, s) && !workspace)) {
     dof_set_error("dof_attention_step: null tensor");
     return DOF_ERR_ARG;
   }
@@ -488,9 +560,9 @@ extern "C" int dof_attention_step(const DofAttnStep* d, const void* q, const voi
     dof_set_error("dof_attention_step: tensors and strides must be multiples of 16 bytes");
     return DOF_ERR_UNSUPPORTED;
   }
-  const int64_t blocks = (int64_t)d->streams * d->k_heads * s.splits * s.row_blocks;
-  const int64_t joins = (int64_t)d->streams * d->k_heads * s.rows;
-  if (blocks > 0x7FFFFFFF || joins > 0x7FFFFFFF) {
+  const int64_t blocks = s.parts * d->k_heads * s.row_blocks;
+  const int64_t rows = (int64_t)d->streams * d->k_heads * s.rows;
+  if (blocks > 0x7FFFFFFF || rows > 0x7FFFFFFF) {
     dof_set_error("dof_attention_step: too many streams and heads for one launch");
     return DOF_ERR_UNSUPPORTED;
   }
@@ -512,11 +584,15 @@ extern "C" int dof_attention_step(const DofAttnStep* d, const void* q, const voi
   A.lengths = lengths;
   A.slopes = slopes;
   A.o = o;
-  A.part = static_cast<float*>(workspace);
-  A.stat = A.part ? A.part + (int64_t)d->streams * d->k_heads * s.splits * s.rows * d->head_dim : nullptr;
-  A.splits = s.splits;
+  if (joins(d, s)) {
+    A.part = static_cast<float*>(workspace);
+    A.stat = A.part + part_floats(d, s);
+    A.sched = reinterpret_cast<int32_t*>(A.stat + s.parts * d->k_heads * s.rows * 2);
+  }
   A.rows = s.rows;
   A.row_blocks = s.row_blocks;
+  A.min_tiles = s.min_tiles;
+  A.join_lanes = rows < 512 ? 8 : 32;
   A.page_shift = -1;
   if ((d->page_size & (d->page_size - 1)) == 0)
     while ((int64_t)1 << (A.page_shift + 1) <= d->page_size) ++A.page_shift;
@@ -525,7 +601,7 @@ extern "C" int dof_attention_step(const DofAttnStep* d, const void* q, const voi
     else if (d->head_dim <= 64) launch_rt<T, 64>(A, s.rt, (unsigned)blocks, (hipStream_t)stream);
     else if (d->head_dim <= 96) launch_rt<T, 96>(A, s.rt, (unsigned)blocks, (hipStream_t)stream);
     else launch_rt<T, 128>(A, s.rt, (unsigned)blocks, (hipStream_t)stream);
-    if (s.splits > 1) DOF_LAUNCH((k_attn_step_join<T>), ((unsigned)joins, 1, 1), (256, 1, 1), (hipStream_t)stream, A);
+    if (joins(d, s)) DOF_LAUNCH((k_attn_step_join<T>), ((unsigned)rows, dof_cdiv(d->head_dim, 4 * A.join_lanes), 1), (256, 1, 1), (hipStream_t)stream, A);
   });
   return dof_check_launch("k_attn_step");
 }
