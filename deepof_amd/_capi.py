@@ -7,6 +7,7 @@ loudly if it is missing); this module itself has no knowledge of where a library
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 ABI_VERSION = 17
 
@@ -104,6 +105,14 @@ class AttnStep(C.Structure):
                 ("vc_stride", _ST3)]
 
 
+# The records of the sequence operators as one packing call each (filling a ctypes structure field by field takes several times as
+# long as the rest of a short call): fields in the structures' order, strides flat.
+PACK_NORM_ROPE = struct.Struct("@6iqfi12q")
+PACK_ATTENTION = struct.Struct("@4i2f16q")
+PACK_ATTN_STEP = struct.Struct("@10i2f18q")
+for _pack, _cls in ((PACK_NORM_ROPE, NormRope), (PACK_ATTENTION, Attention), (PACK_ATTN_STEP, AttnStep)):
+    assert _pack.size == C.sizeof(_cls), _cls
+
 PP_KINDS = {"other": 0, "coord": 1, "speed": 2, "dist_inner": 3, "dist_intra": 4, "angle": 5}
 PP_MODES = {None: 0, "per_column": 1, "groupwise": 2}
 PP_INTER_SCALE = {"mean": 0, "geom": 1, "global": 2}
@@ -182,16 +191,16 @@ SIGNATURES = {
     "dof_preprocess_fit_global": (C.c_int, [C.POINTER(PreprocDims), _I32, _P, _P, _P, _P]),
     "dof_preprocess_raw_moments": (C.c_int, [C.POINTER(PreprocDims)] + [_P] * 6),
     "dof_preprocess_order_stats": (C.c_int, [C.POINTER(PreprocDims)] + [_P] * 11),
-    "dof_norm_rope_forward": (C.c_int, [C.POINTER(NormRope)] + [_P] * 9),
-    "dof_norm_rope_workspace_bytes": (_I64, [C.POINTER(NormRope)]),
-    "dof_norm_rope_backward": (C.c_int, [C.POINTER(NormRope)] + [_P] * 14),
+    "dof_norm_rope_forward": (C.c_int, [_P] + [_P] * 9),
+    "dof_norm_rope_workspace_bytes": (_I64, [_P]),
+    "dof_norm_rope_backward": (C.c_int, [_P] + [_P] * 14),
     "dof_attn_plan_size": (C.c_int, [_I32, _P, _P, _I32, C.POINTER(AttnPlan)]),
     "dof_attn_plan_table": (C.c_int, [C.POINTER(AttnPlan), _P, _P, _P, _P]),
-    "dof_attention_forward": (C.c_int, [C.POINTER(AttnPlan), _P, C.POINTER(Attention)] + [_P] * 7),
-    "dof_attention_workspace_bytes": (_I64, [C.POINTER(AttnPlan), C.POINTER(Attention)]),
-    "dof_attention_backward": (C.c_int, [C.POINTER(AttnPlan), _P, C.POINTER(Attention)] + [_P] * 12),
-    "dof_attention_step_workspace_bytes": (_I64, [C.POINTER(AttnStep)]),
-    "dof_attention_step": (C.c_int, [C.POINTER(AttnStep)] + [_P] * 11),
+    "dof_attention_forward": (C.c_int, [C.POINTER(AttnPlan), _P, _P] + [_P] * 7),
+    "dof_attention_workspace_bytes": (_I64, [C.POINTER(AttnPlan), _P]),
+    "dof_attention_backward": (C.c_int, [C.POINTER(AttnPlan), _P, _P] + [_P] * 12),
+    "dof_attention_step_workspace_bytes": (_I64, [_P]),
+    "dof_attention_step": (C.c_int, [_P] + [_P] * 11),
 }
 
 

@@ -13,7 +13,6 @@ outputs come from torch's allocator, one per call, so calls on different streams
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 from typing import Optional, Sequence
 
@@ -80,14 +79,22 @@ def _vector(name: str, t: Optional[torch.Tensor], n: int, dtype, device):
 
 
 def _st(t: torch.Tensor):
-    """Row and head strides of a (rows, heads, head_dim) tensor."""
-    s = t.stride()
-    return (s[0], s[1])
+    """The strides but the last (which is 1): row and head, or stream, frame and head."""
+    return t.stride()[:-1]
+
+
+def _ptr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _is_wide(t: torch.Tensor) -> bool:
     """Address and strides are multiples of 16 bytes (what the attention kernels load at once)."""
     e = t.element_size()
+    bits = t.data_ptr()
+    for s in t.stride()[:-1]:
+        bits |= s * e
+    if not bits & 15:
+        return True
     return t.data_ptr() % 16 == 0 and all(s * e % 16 == 0 for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n > 1)
 
 
@@ -147,96 +154,88 @@ class AttentionOps:
         if self.device.type == "cuda" and self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
 
-    def _on_device(self):
-        """Launches go to the current device: make it this object's for the call if it is another one."""
-        if self.device.type == "cuda" and torch.cuda.current_device() != self.device.index:
-            return torch.cuda.device(self.device)
-        return contextlib.nullcontext()
-
-    def _stream(self):
-        if self.device.type == "cuda":
-            return torch.cuda.current_stream(self.device).cuda_stream
-        return 0
+    def _launch(self, name: str, *args):
+        """The entry point on the current stream of this object's device; launches go to the current device, so another one is made
+        current for the call."""
+        fn = getattr(self.lib, name)
+        if self.device.type != "cuda":
+            rc = fn(*args, 0)
+        elif torch.cuda.current_device() == self.device.index:
+            rc = fn(*args, torch.cuda.current_stream(self.device).cuda_stream)
+        else:
+            with torch.cuda.device(self.device):
+                rc = fn(*args, torch.cuda.current_stream(self.device).cuda_stream)
+        if rc:
+            _capi.check(self.lib, rc, name)
 
     def _dtype(self, name, t):
         if not isinstance(t, torch.Tensor) or t.dtype not in DTYPES:
             raise ValueError(f"{name} must be a float32, bfloat16 or float16 tensor")
         return t.dtype
 
-    def _output(self, name, t, like_shape, dtype):
+    def _output(self, name, t, like):
+        """The caller's output, or a new contiguous one of ``like``'s shape and dtype."""
         if t is None:
-            return torch.empty(like_shape, dtype=dtype, device=self.device)
-        _rows(name, t, self.device, dtype, len(like_shape))
-        if tuple(t.shape) != tuple(like_shape):
-            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(like_shape)}")
+            return like.new_empty(like.shape)
+        _rows(name, t, self.device, like.dtype, like.dim())
+        if t.shape != like.shape:
+            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(like.shape)}")
         return _writable(name, t)
 
     # ---- norm + rotation ------------------------------------------------------------------------------------------
-    def _norm_rope_dims(self, q, k, positions, freqs, eps, interleaved):
+    def _norm_rope_args(self, q, k, positions, freqs, q_weight, k_weight, eps, interleaved):
+        """The checked head of the record and the addresses of positions, freqs and weights."""
         dt = self._dtype("q", q)
         _rows("q", q, self.device, dt)
         _rows("k", k, self.device, dt)
-        if q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+        rows, hq, dim = q.shape
+        if k.shape[0] != rows or k.shape[2] != dim:
             raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} must have the same rows and head size")
-        pos = _vector("positions", positions, q.shape[0], torch.int32, self.device)
-        if freqs.dim() != 1:
-            raise ValueError("freqs must hold one angle per rotated pair")
-        fr = _vector("freqs", freqs, freqs.shape[0], torch.float64, self.device)
-        if 2 * freqs.shape[0] > q.shape[2]:
-            raise ValueError(f"{freqs.shape[0]} rotated pairs do not fit a head of {q.shape[2]}")
+        if not isinstance(freqs, torch.Tensor) or freqs.dim() != 1:
+            raise ValueError("freqs must be a tensor of one angle per rotated pair")
+        pairs = freqs.shape[0]
+        if 2 * pairs > dim:
+            raise ValueError(f"{pairs} rotated pairs do not fit a head of {dim}")
         if not eps >= 0.0:
             raise ValueError("eps must not be negative")
-        d = _capi.NormRope()
-        d.dtype, d.head_dim, d.rot_dim, d.interleaved = DTYPES[dt], q.shape[2], 2 * freqs.shape[0], int(bool(interleaved))
-        d.q_heads, d.k_heads, d.tokens, d.eps = q.shape[1], k.shape[1], q.shape[0], eps
-        d.q_stride[:], d.k_stride[:] = _st(q), _st(k)
-        return d, pos, fr
+        head = (DTYPES[dt], dim, 2 * pairs, 1 if interleaved else 0, hq, k.shape[1], rows, eps, 0)
+        return head, (_vector("positions", positions, rows, torch.int32, self.device),
+                      _vector("freqs", freqs, pairs, torch.float64, self.device),
+                      _vector("q_weight", q_weight, dim, torch.float32, self.device),
+                      _vector("k_weight", k_weight, dim, torch.float32, self.device))
 
     def norm_rope(self, q, k, positions, freqs, q_weight=None, k_weight=None, eps: float = 1e-6, interleaved: bool = False,
                   q_out=None, k_out=None):
         """-> (q', k').  q (rows, query heads, head_dim) and k (rows, key heads, head_dim): every head divided by its root mean
         square and multiplied by ``q_weight`` / ``k_weight`` (fp32, None: no norm), then its first ``2 len(freqs)`` elements
         rotated by ``positions[row] * freqs[pair]`` (positions int32; freqs float64, see :func:`rotary_frequencies`).
-        ``interleaved``: neighbouring elements are a pair; otherwise the pairs lie half the rotated part apart.  ``q_out`` /
-        ``k_out`` may be q / k themselves."""
-        d, pos, fr = self._norm_rope_dims(q, k, positions, freqs, eps, interleaved)
-        q_out = self._output("q_out", q_out, q.shape, q.dtype)
-        k_out = self._output("k_out", k_out, k.shape, k.dtype)
-        d.q_out_stride[:], d.k_out_stride[:] = _st(q_out), _st(k_out)
-        wq = _vector("q_weight", q_weight, q.shape[2], torch.float32, self.device)
-        wk = _vector("k_weight", k_weight, q.shape[2], torch.float32, self.device)
-        with self._on_device():
-            rc = self.lib.dof_norm_rope_forward(C.byref(d), q.data_ptr(), k.data_ptr(), pos, fr, wq, wk, q_out.data_ptr(),
-                                                k_out.data_ptr(), self._stream())
-        _capi.check(self.lib, rc, "dof_norm_rope_forward")
+        ``interleaved``: neighbouring elements are a pair; otherwise the pairs lie half the rotated part apart.  head_dim: even, up
+        to 256.  ``q_out`` / ``k_out`` may be q / k themselves."""
+        head, ptrs = self._norm_rope_args(q, k, positions, freqs, q_weight, k_weight, eps, interleaved)
+        q_out = self._output("q_out", q_out, q)
+        k_out = self._output("k_out", k_out, k)
+        rec = _capi.PACK_NORM_ROPE.pack(*head, *_st(q), *_st(k), *_st(q_out), *_st(k_out), 0, 0, 0, 0)
+        self._launch("dof_norm_rope_forward", rec, q.data_ptr(), k.data_ptr(), *ptrs, q_out.data_ptr(), k_out.data_ptr())
         return q_out, k_out
 
     def norm_rope_backward(self, dq_out, dk_out, q, k, positions, freqs, q_weight=None, k_weight=None, eps: float = 1e-6,
                            interleaved: bool = False):
         """-> (dq, dk, dq_weight, dk_weight) from the gradients at :meth:`norm_rope`'s outputs and its inputs (the weight gradients
         are None without a weight; they are the same bits on every run)."""
-        d, pos, fr = self._norm_rope_dims(q, k, positions, freqs, eps, interleaved)
+        head, ptrs = self._norm_rope_args(q, k, positions, freqs, q_weight, k_weight, eps, interleaved)
         for name, g, x in (("dq_out", dq_out, q), ("dk_out", dk_out, k)):
             _rows(name, g, self.device, q.dtype)
             if g.shape != x.shape:
                 raise ValueError(f"{name} has shape {tuple(g.shape)}, expected {tuple(x.shape)}")
-        d.gq_stride[:], d.gk_stride[:] = _st(dq_out), _st(dk_out)
-        dq = torch.empty(q.shape, dtype=q.dtype, device=self.device)
-        dk = torch.empty(k.shape, dtype=k.dtype, device=self.device)
-        d.q_out_stride[:], d.k_out_stride[:] = _st(dq), _st(dk)
-        wq = _vector("q_weight", q_weight, q.shape[2], torch.float32, self.device)
-        wk = _vector("k_weight", k_weight, q.shape[2], torch.float32, self.device)
-        f32 = dict(dtype=torch.float32, device=self.device)
-        dwq = torch.empty(q.shape[2], **f32) if wq else None
-        dwk = torch.empty(q.shape[2], **f32) if wk else None
-        ws = torch.empty(self._bytes("dof_norm_rope_workspace_bytes", C.byref(d)) if wq or wk else 0, dtype=torch.uint8,
-                         device=self.device)
-        with self._on_device():
-            rc = self.lib.dof_norm_rope_backward(C.byref(d), dq_out.data_ptr(), dk_out.data_ptr(), q.data_ptr(), k.data_ptr(),
-                                                 pos, fr, wq, wk, dq.data_ptr(), dk.data_ptr(),
-                                                 dwq.data_ptr() if wq else 0, dwk.data_ptr() if wk else 0, ws.data_ptr(),
-                                                 self._stream())
-        _capi.check(self.lib, rc, "dof_norm_rope_backward")
+        dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
+        dwq = None if q_weight is None else torch.empty_like(q_weight)
+        dwk = None if k_weight is None else torch.empty_like(k_weight)
+        rec = _capi.PACK_NORM_ROPE.pack(*head, *_st(q), *_st(k), *_st(dq), *_st(dk), *_st(dq_out), *_st(dk_out))
+        ws = None
+        if dwq is not None or dwk is not None:
+            ws = torch.empty(self._bytes("dof_norm_rope_workspace_bytes", rec), dtype=torch.uint8, device=self.device)
+        self._launch("dof_norm_rope_backward", rec, dq_out.data_ptr(), dk_out.data_ptr(), q.data_ptr(), k.data_ptr(), *ptrs,
+                     dq.data_ptr(), dk.data_ptr(), _ptr(dwq), _ptr(dwk), _ptr(ws))
         return dq, dk, dwq, dwk
 
     # ---- attention over packed documents ----------------------------------------------------------------------------
@@ -248,7 +247,7 @@ class AttentionOps:
         data (lists, arrays, CPU tensors).  Build it once per batch and use it for every layer, forward and backward."""
         return AttentionPlan(self, q_lengths, k_lengths, causal, prefix)
 
-    def _attention_dims(self, plan, q, k, v, scale, cap, slopes):
+    def _attention_args(self, plan, q, k, v, scale, cap, slopes):
         if not isinstance(plan, AttentionPlan) or plan.device != self.device:
             raise ValueError("plan must come from attention_plan() of these operators")
         dt = self._dtype("q", q)
@@ -261,11 +260,14 @@ class AttentionOps:
             raise ValueError(f"the plan covers {plan.q_rows} query and {plan.k_rows} key rows, the tensors have {q.shape[0]} and {k.shape[0]}")
         if k.shape[1] < 1 or q.shape[1] % k.shape[1] or q.shape[1] < 1:
             raise ValueError(f"{q.shape[1]} query heads are not a multiple of {k.shape[1]} key heads")
-        d = _capi.Attention()
-        d.dtype, d.head_dim, d.q_heads, d.k_heads = DTYPES[dt], q.shape[2], q.shape[1], k.shape[1]
-        d.scale = q.shape[2] ** -0.5 if scale is None else scale
-        d.cap = cap
-        return d, _vector("slopes", slopes, q.shape[1], torch.float32, self.device)
+        head = (DTYPES[dt], q.shape[2], q.shape[1], k.shape[1], q.shape[2] ** -0.5 if scale is None else scale, cap)
+        return head, _vector("slopes", slopes, q.shape[1], torch.float32, self.device)
+
+    def _lse(self, lse, q):
+        if not isinstance(lse, torch.Tensor) or lse.shape != q.shape[:2] or lse.dtype != torch.float32 or lse.device != self.device \
+                or not lse.is_contiguous():
+            raise ValueError(f"lse must be a contiguous float32 tensor of shape {tuple(q.shape[:2])} on {self.device}")
+        return lse
 
     def attention(self, plan, q, k, v, scale: Optional[float] = None, cap: float = 0.0, slopes=None, out=None, lse=None):
         """-> (o, lse).  q (rows, query heads, head_dim), k and v (rows, key heads, head_dim); query head h reads key head
@@ -273,23 +275,19 @@ class AttentionOps:
         ``slopes`` (fp32 per query head): minus ``slope * distance``.  lse (rows, query heads), fp32, natural log.  A row that sees no
         key gives zeros and -inf.  Rows behind the last document are left as they were in ``out`` / ``lse`` and are zeros in tensors
         allocated here.  head_dim: a multiple of 8 up to 128."""
-        d, sl = self._attention_dims(plan, q, k, v, scale, cap, slopes)
+        head, sl = self._attention_args(plan, q, k, v, scale, cap, slopes)
         tail = q.shape[0] > plan.q_rows
-        new = torch.zeros if tail else torch.empty
-        if out is None:
-            out = new(q.shape, dtype=q.dtype, device=self.device)
-        o = self._output("out", out, q.shape, q.dtype)
+        if out is None and tail:
+            out = q.new_zeros(q.shape)
+        o = self._output("out", out, q)
         if lse is None:
-            lse = new(q.shape[:2], dtype=torch.float32, device=self.device)
-        elif lse.shape != q.shape[:2] or lse.dtype != torch.float32 or lse.device != self.device or not lse.is_contiguous():
-            raise ValueError(f"lse must be a contiguous float32 tensor of shape {tuple(q.shape[:2])} on {self.device}")
+            lse = (torch.zeros if tail else torch.empty)(q.shape[:2], dtype=torch.float32, device=self.device)
+        self._lse(lse, q)
         q, k, v = _wide(q), _wide(k), _wide(v)
         ow = o if _is_wide(o) else o.clone(memory_format=torch.contiguous_format)
-        d.q_stride[:], d.k_stride[:], d.v_stride[:], d.o_stride[:] = _st(q), _st(k), _st(v), _st(ow)
-        with self._on_device():
-            rc = self.lib.dof_attention_forward(C.byref(plan.record), plan.table.data_ptr(), C.byref(d), q.data_ptr(), k.data_ptr(),
-                                                v.data_ptr(), sl, ow.data_ptr(), lse.data_ptr(), self._stream())
-        _capi.check(self.lib, rc, "dof_attention_forward")
+        rec = _capi.PACK_ATTENTION.pack(*head, *_st(q), *_st(k), *_st(v), *_st(ow), 0, 0, 0, 0, 0, 0, 0, 0)
+        self._launch("dof_attention_forward", C.byref(plan.record), plan.table.data_ptr(), rec, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                     sl, ow.data_ptr(), lse.data_ptr())
         if ow is not o:
             o.copy_(ow)
         return o, lse
@@ -298,26 +296,21 @@ class AttentionOps:
         """-> (dq, dk, dv) from the gradient at ``o`` and the forward's inputs and results; zeros in rows of no document.  The same
         bits on every run.  ``slopes`` are constants: they get no gradient.  float16: small gradients keep their precision down to
         about 1e-6 of the scores' gradient; scale the loss for smaller ones, as in any float16 training."""
-        d, sl = self._attention_dims(plan, q, k, v, scale, cap, slopes)
+        head, sl = self._attention_args(plan, q, k, v, scale, cap, slopes)
         for name, t in (("do", do), ("o", o)):
             _rows(name, t, self.device, q.dtype)
             if t.shape != q.shape:
                 raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(q.shape)}")
-        if lse.shape != q.shape[:2] or lse.dtype != torch.float32 or lse.device != self.device or not lse.is_contiguous():
-            raise ValueError(f"lse must be a contiguous float32 tensor of shape {tuple(q.shape[:2])} on {self.device}")
-        new_q = torch.zeros if q.shape[0] > plan.q_rows else torch.empty
-        new_k = torch.zeros if k.shape[0] > plan.k_rows else torch.empty
-        dq = new_q(q.shape, dtype=q.dtype, device=self.device)
-        dk, dv = (new_k(k.shape, dtype=q.dtype, device=self.device) for _ in range(2))
+        self._lse(lse, q)
+        dq = q.new_zeros(q.shape) if q.shape[0] > plan.q_rows else q.new_empty(q.shape)
+        new_k = k.new_zeros if k.shape[0] > plan.k_rows else k.new_empty
+        dk, dv = new_k(k.shape), new_k(k.shape)
         q, k, v, do, o = _wide(q), _wide(k), _wide(v), _wide(do), _wide(o)
-        d.q_stride[:], d.k_stride[:], d.v_stride[:], d.o_stride[:], d.g_stride[:] = _st(q), _st(k), _st(v), _st(o), _st(do)
-        d.dq_stride[:], d.dk_stride[:], d.dv_stride[:] = _st(dq), _st(dk), _st(dv)
-        ws = torch.empty(self._bytes("dof_attention_workspace_bytes", C.byref(plan.record), C.byref(d)), dtype=torch.uint8, device=self.device)
-        with self._on_device():
-            rc = self.lib.dof_attention_backward(C.byref(plan.record), plan.table.data_ptr(), C.byref(d), do.data_ptr(), q.data_ptr(),
-                                                 k.data_ptr(), v.data_ptr(), sl, o.data_ptr(), lse.data_ptr(), dq.data_ptr(),
-                                                 dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), self._stream())
-        _capi.check(self.lib, rc, "dof_attention_backward")
+        rec = _capi.PACK_ATTENTION.pack(*head, *_st(q), *_st(k), *_st(v), *_st(o), *_st(do), *_st(dq), *_st(dk), *_st(dv))
+        need = self._bytes("dof_attention_workspace_bytes", C.byref(plan.record), rec)
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        self._launch("dof_attention_backward", C.byref(plan.record), plan.table.data_ptr(), rec, do.data_ptr(), q.data_ptr(), k.data_ptr(),
+                     v.data_ptr(), sl, o.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(ws))
         return dq, dk, dv
 
     # ---- the new frames of live streams ------------------------------------------------------------------------------
@@ -352,26 +345,17 @@ class AttentionOps:
                 or not page_table.is_contiguous():
             raise ValueError(f"page_table must be a contiguous int32 tensor ({b}, pages of a stream) on {self.device}")
         ln = _vector("lengths", lengths, b, torch.int32, self.device)
-        d = _capi.AttnStep()
-        d.dtype, d.head_dim, d.q_heads, d.k_heads = DTYPES[dt], dim, hq, hk
-        d.streams, d.new_frames, d.n_pages, d.page_size, d.max_pages = b, new, k_cache.shape[0], k_cache.shape[1], page_table.shape[1]
-        d.scale = dim ** -0.5 if scale is None else scale
-        d.cap = cap
-        o = self._output("out", out, q.shape, dt)
-        ow = o
-        if not _is_wide(o):
-            ow = o.clone(memory_format=torch.contiguous_format)
-        q, k, v = _wide(q), _wide(k), _wide(v)
-        d.q_stride[:], d.k_stride[:], d.v_stride[:], d.o_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3], ow.stride()[:3]
-        d.kc_stride[:], d.vc_stride[:] = k_cache.stride()[:3], v_cache.stride()[:3]
         sl = _vector("slopes", slopes, hq, torch.float32, self.device)
-        need = self._bytes("dof_attention_step_workspace_bytes", C.byref(d))
+        o = self._output("out", out, q)
+        ow = o if _is_wide(o) else o.clone(memory_format=torch.contiguous_format)
+        q, k, v = _wide(q), _wide(k), _wide(v)
+        rec = _capi.PACK_ATTN_STEP.pack(DTYPES[dt], dim, hq, hk, b, new, k_cache.shape[0], k_cache.shape[1], page_table.shape[1], 0,
+                                        dim ** -0.5 if scale is None else scale, cap, *_st(q), *_st(k), *_st(v), *_st(ow),
+                                        *_st(k_cache), *_st(v_cache))
+        need = self._bytes("dof_attention_step_workspace_bytes", rec)
         ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-        with self._on_device():
-            rc = self.lib.dof_attention_step(C.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(),
-                                             v_cache.data_ptr(), page_table.data_ptr(), ln, sl, ow.data_ptr(),
-                                             ws.data_ptr() if need else 0, self._stream())
-        _capi.check(self.lib, rc, "dof_attention_step")
+        self._launch("dof_attention_step", rec, q.data_ptr(), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                     page_table.data_ptr(), ln, sl, ow.data_ptr(), _ptr(ws))
         if ow is not o:
             o.copy_(ow)
         return o
