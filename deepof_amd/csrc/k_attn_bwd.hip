@@ -123,9 +123,9 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_
           } else {
             float w = x[v] * sc.mul;
             if (sc.cap_l2 != 0.0f) {
-              const float th = dof_cap_tanh<T>(w);
+              const float th = dof_cap_tanh<T>(x[v], sc.mul);
               w = sc.cap_l2 * th;
-              c *= 1.0f - th * th;
+              c *= fmaf(-th, th, 1.0f);
             }
             if (A.slopes) w -= sc.slope_l2 * fabsf(base - (float)r);
             p = dof_exp2(w - lse2);
@@ -254,9 +254,9 @@ __global__ void __launch_bounds__(64, DP <= 32 ? 2 : 1) k_attn_bwd_one(DofAttnBw
       } else {
         float w = x[v] * A.score.mul;
         if (A.score.cap_l2 != 0.0f) {
-          const float th = dof_cap_tanh<T>(w);
+          const float th = dof_cap_tanh<T>(x[v], A.score.mul);
           w = A.score.cap_l2 * th;
-          c *= 1.0f - th * th;
+          c *= fmaf(-th, th, 1.0f);
         }
         if (A.slopes) w -= slope * fabsf(base + (float)r);
         p[v] = dof_exp2(w - ls);
@@ -433,9 +433,9 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_
         } else {
           float w = x[v] * A.score.mul;
           if (A.score.cap_l2 != 0.0f) {
-            const float th = dof_cap_tanh<T>(w);
+            const float th = dof_cap_tanh<T>(x[v], A.score.mul);
             w = A.score.cap_l2 * th;
-            c *= 1.0f - th * th;
+            c *= fmaf(-th, th, 1.0f);
           }
           if (A.slopes) w -= slope * fabsf(base + (float)r);
           p[v] = dof_exp2(w - lse2);

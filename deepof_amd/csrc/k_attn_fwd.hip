@@ -97,23 +97,24 @@ __global__ void __launch_bounds__(64 * NW, DP <= 32 ? (NW == 1 && sizeof(T) == 4
         for (int s = 0; s < KS; ++s) x[u] = dof_mma32<T>(sk[buf].rowfrag(32 * u + col, 2 * s + half), q[s], x[u]);
       }
       if constexpr (!PLAIN) {
+        const float base = (float)(pos - j0 - 4 * half);
         if (sc.cap_l2 != 0.0f) {
 #pragma unroll
           for (int u = 0; u < KU; ++u)
 #pragma unroll
-            for (int v = 0; v < 16; ++v) x[u][v] = sc.cap_l2 * dof_cap_tanh<T>(x[u][v] * sc.mul);
+            for (int v = 0; v < 16; ++v) x[u][v] = sc.cap_l2 * dof_cap_tanh<T>(x[u][v], sc.mul);
+          if (A.slopes) {
+#pragma unroll
+            for (int u = 0; u < KU; ++u)
+#pragma unroll
+              for (int v = 0; v < 16; ++v) x[u][v] -= sc.slope_l2 * fabsf(base - (float)(32 * u + 8 * (v / 4) + v % 4));
+          }
         } else {
 #pragma unroll
           for (int u = 0; u < KU; ++u)
 #pragma unroll
-            for (int v = 0; v < 16; ++v) x[u][v] *= sc.mul;
-        }
-        if (A.slopes) {
-          const float base = (float)(pos - j0 - 4 * half);
-#pragma unroll
-          for (int u = 0; u < KU; ++u)
-#pragma unroll
-            for (int v = 0; v < 16; ++v) x[u][v] -= sc.slope_l2 * fabsf(base - (float)(32 * u + 8 * (v / 4) + v % 4));
+            for (int v = 0; v < 16; ++v)
+              x[u][v] = fmaf(x[u][v], sc.mul, -sc.slope_l2 * fabsf(base - (float)(32 * u + 8 * (v / 4) + v % 4)));
         }
       }
       const float unit = PLAIN ? sc.mul : 1.0f;  // of x, in log 2

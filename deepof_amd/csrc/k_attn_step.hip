@@ -300,15 +300,16 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) k_attn
     // keys 16 u + 4 quad + e of the tile, e = 0 .. 3, sit in this lane's registers
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[i][u][e] *= A.score.mul;
       if (A.score.cap_l2 != 0.0f) {
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[i][u][e] = A.score.cap_l2 * dof_cap_tanh<T>(x[i][u][e]);
+          for (int e = 0; e < 4; ++e) x[i][u][e] = A.score.cap_l2 * dof_cap_tanh<T>(x[i][u][e], A.score.mul);
+      } else {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[i][u][e] *= A.score.mul;
       }
       if (A.slopes) {
         const float base = (float)(pos[i] - j0 - 4 * quad);

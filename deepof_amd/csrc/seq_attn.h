@@ -30,11 +30,11 @@ struct DofScore {
 };
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-// tanh for the cap: fp32 inputs take the library's, 16-bit ones the fast form (absolute error 2^-22, far below half a step of the
-// inputs the score is made of)
-template <class T> __device__ __forceinline__ float dof_cap_tanh(float x) {
-  if constexpr (sizeof(T) == 4) return tanhf(x);
-  else return dof_tanh(x);
+// tanh(raw mul) for the cap: fp32 inputs take the library's; 16-bit ones 1 - 2 / (1 + 2^(2 log2(e) mul raw)), whose absolute error of 2^-22
+// is far below half a step of the inputs the score is made of
+template <class T> __device__ __forceinline__ float dof_cap_tanh(float raw, float mul) {
+  if constexpr (sizeof(T) == 4) return tanhf(raw * mul);
+  else return fmaf(-2.0f, dof_rcp(1.0f + dof_exp2(raw * (mul * (2.0f * kLog2e)))), 1.0f);
 }
 
 // Blocks are dealt to the eight XCDs in turn, each with an L2 of its own.  Where the heads divide over the XCDs (or the XCDs over the
