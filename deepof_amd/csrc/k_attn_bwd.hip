@@ -8,8 +8,14 @@
 // Every gradient element is summed by one workgroup in a fixed order: no atomics, the same bits on every run.  The price is that S
 // and dP are computed twice (seven products of the size of S instead of five).  Both kernels keep their own rows' operands in
 // registers and stream the other side through LDS (two images); the second products take P and dS straight from the registers the
-// first ones left them in, as in the forward.  P and dS are rounded to the elements' type for their products; everything that is
-// summed is fp32.  fp16 has 5 exponent bits: there P is carried as 2^12 P and dS as 2^6 dS (exact factors, taken out at the end), so
+// first ones left them in, as in the forward.
+//
+// P is rounded to the elements' type for its product with g, as in the forward.  dS goes into its products as two 16-bit numbers, value
+// and rest: rounded once, its error alone would be as large as that of rounding dq and dk themselves (of short documents it came to 1.8
+// times that, together with delta from the rounded o).  The second product costs a fifth: 16384 causal frames, 16 / 4 heads of 128, bf16:
+// dq 1.75 -> 2.28 ms, dk 1.83 -> 2.22 ms.  The dq kernel starts from
+// delta = g.o, sums the unrounded P dP on its way and leaves that delta to the dk kernel.  Everything that is summed is fp32.
+// fp16 has 5 exponent bits: there P is carried as 2^12 P and dS as 2^6 dS (exact factors, taken out at the end), so
 // that weights of long documents and small gradients stay out of its subnormals.
 #include <cmath>
 
@@ -28,12 +34,54 @@ template <> struct Lift<DofF16> {
   static constexpr float p2 = 12.0f, p = 4096.0f, ds = 64.0f;
 };
 
-// PLAIN: neither cap nor bias (as in the forward)
-template <class T, int DP, int NW, bool PLAIN>
+// A row's log-sum-exp in log 2, as the value and (fp32 elements) what its rounding left: there the weights are to be good to fp32, and
+// one rounding of a number near 10 is not.  The lift is taken off.  +inf: the row takes no part (it has no keys).
+struct Lse { float value, rest; };
+template <class T> __device__ __forceinline__ Lse lse_of(float lse) {
+  Lse r = {INFINITY, 0.0f};
+  if (lse == -INFINITY) return r;
+  r.value = lse * kLog2e;
+  if constexpr (sizeof(T) == 4) r.rest = fmaf(lse, kLog2e, -r.value) + lse * 1.925963033500e-8f;  // log2(e) - kLog2e
+  r.value -= Lift<T>::p2;
+  return r;
+}
+// the weight: 2^(w - lse), w = x mul for plain scores
+template <class T, int KIND> __device__ __forceinline__ float weight(float x, float mul, float w, float value, float rest) {
+  const float e = KIND == 0 ? fmaf(x, mul, -value) : w - value;
+  return dof_exp2(sizeof(T) == 4 ? e - rest : e);
+}
+
+// Sixteen raw products x of a lane -> the exponents' arguments w (log 2, before the log-sum-exp is taken off) and c, the factor of dS from
+// P (dP - delta): the derivative of the cap and the lift.  dist(v): the distance of element v.
+template <class T, int KIND, class Dist>
+__device__ __forceinline__ void scores(const dof_f32x16& x, const DofScore& sc, bool bias, Dist dist, float* w, float* c) {
+#pragma unroll
+  for (int v = 0; v < 16; ++v) {
+    w[v] = x[v];
+    c[v] = Lift<T>::ds / Lift<T>::p;
+  }
+  if constexpr (KIND == 2) {
+    dof_cap_tanh<T, 16>(w, sc.mul);
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      c[v] *= fmaf(-w[v], w[v], 1.0f);
+      w[v] *= sc.cap_l2;
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < 16; ++v) w[v] *= sc.mul;
+  }
+  if (bias) {
+#pragma unroll
+    for (int v = 0; v < 16; ++v) w[v] -= sc.slope_l2 * fabsf(dist(v));
+  }
+}
+
+// KIND: the score function (dof_attn_kind)
+template <class T, int DP, int NW, int KIND>
 __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_attn_dq(DofAttnBwd B) {
   const DofAttnFwd& A = B.f;
-  // keys per step: 64 where two wavefronts per SIMD still fit (heads of 96: 162 us with 64, 174 with 32; of 128: 2.4 ms and 1.77)
-  constexpr int KU = NW == 4 && DP == 96 ? 2 : 1, kKeys = 32 * KU;
+  constexpr int kKeys = 32;  // per step: what leaves room for two wavefronts per SIMD
   using Tile = DofTile<T, kKeys, DP>;
   using Stage = DofStage<T, kKeys, DP, 64 * NW>;
   __shared__ Tile sk[2], sv[2];
@@ -77,77 +125,76 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_
   }
   delta += dof_swap32(delta);
   const int64_t srow = (t.q0 + row) * A.q_heads + h;
-  if (live && half == 0) B.delta[srow] = delta;
-  float lse2 = live ? A.lse[srow] * kLog2e : 0.0f;
-  if (lse2 == -INFINITY) lse2 = 0.0f;  // a row without keys: every score is masked below
-  lse2 -= Lift<T>::p2;
+  float sum = 0.0f;  // of P dP: delta again, without the rounding of o
+  const Lse lse = lse_of<T>(live ? A.lse[srow] : -INFINITY);
   const T* kp = static_cast<const T*>(A.k) + t.k0 * A.ks[0] + hk * A.ks[1];
   const T* vp = static_cast<const T*>(A.v) + t.k0 * A.vs[0] + hk * A.vs[1];
 
   dof_f32x16 dq[DT];
-#pragma unroll
-  for (int d = 0; d < DT; ++d) dq[d] = dof_zero16();
   Stage rk, rv;
-  if (kmax > 0) {
-    rk.load(kp, A.ks[0], t.lk, A.dim, tid);
-    rv.load(vp, A.vs[0], t.lk, A.dim, tid);
-    rk.store(sk[0], tid);
-    rv.store(sv[0], tid);
-  }
-  for (int j0 = 0, buf = 0; j0 < kmax; j0 += kKeys, buf ^= 1) {
-    __syncthreads();
-    const int next = j0 + kKeys;
-    if (next < kmax) {
-      rk.load(kp + next * A.ks[0], A.ks[0], t.lk - next, A.dim, tid);
-      rv.load(vp + next * A.vs[0], A.vs[0], t.lk - next, A.dim, tid);
-    }
-    if (j0 < wmax) {
-      const bool partial = j0 + kKeys > wmin;
+  // Rows of few keys: delta from the rounded o is off by as much as rounding all of dq once more; they go through their keys twice, the
+  // first time for the sum of P dP alone.
+  for (int pass = sizeof(T) == 2 && kmax <= 2 * kKeys ? 0 : 1; pass < 2; ++pass) {
 #pragma unroll
-      for (int u = 0; u < KU; ++u) {
+    for (int d = 0; d < DT; ++d) dq[d] = dof_zero16();
+    if (kmax > 0) {
+      rk.load(kp, A.ks[0], t.lk, A.dim, tid);
+      rv.load(vp, A.vs[0], t.lk, A.dim, tid);
+      rk.store(sk[0], tid);
+      rv.store(sv[0], tid);
+    }
+    sum = 0.0f;
+    for (int j0 = 0, buf = 0; j0 < kmax; j0 += kKeys, buf ^= 1) {
+      __syncthreads();
+      const int next = j0 + kKeys;
+      if (next < kmax) {
+        rk.load(kp + next * A.ks[0], A.ks[0], t.lk - next, A.dim, tid);
+        rv.load(vp + next * A.vs[0], A.vs[0], t.lk - next, A.dim, tid);
+      }
+      if (j0 < wmax) {
+        const bool partial = j0 + kKeys > wmin;
         dof_f32x16 x = dof_zero16(), y = dof_zero16();
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-          x = dof_mma32<T>(sk[buf].rowfrag(32 * u + col, 2 * s + half), q[s], x);
-          y = dof_mma32<T>(sv[buf].rowfrag(32 * u + col, 2 * s + half), g[s], y);
+          x = dof_mma32<T>(sk[buf].rowfrag(col, 2 * s + half), q[s], x);
+          y = dof_mma32<T>(sv[buf].rowfrag(col, 2 * s + half), g[s], y);
         }
-        float ds[16];
-        const float base = (float)(pos - j0 - 32 * u - 4 * half);
-        const int left = kend - j0 - 32 * u - 4 * half;
+        float ds[16], w[16], c[16];
+        const float base = (float)(pos - j0 - 4 * half);
+        const int left = kend - j0 - 4 * half;
+        if constexpr (KIND > 0) scores<T, KIND>(x, sc, A.slopes != nullptr, [&](int v) { return base - (float)(8 * (v / 4) + v % 4); }, w, c);
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
-          const int r = 8 * (v / 4) + v % 4;
-          float c = Lift<T>::ds / Lift<T>::p, p;
-          if constexpr (PLAIN) {
-            p = dof_exp2(fmaf(x[v], sc.mul, -lse2));
-          } else {
-            float w = x[v] * sc.mul;
-            if (sc.cap_l2 != 0.0f) {
-              const float th = dof_cap_tanh<T>(x[v], sc.mul);
-              w = sc.cap_l2 * th;
-              c *= fmaf(-th, th, 1.0f);
-            }
-            if (A.slopes) w -= sc.slope_l2 * fabsf(base - (float)r);
-            p = dof_exp2(w - lse2);
-          }
-          ds[v] = p * c * (y[v] - delta);
-          if (partial && r >= left) ds[v] = 0.0f;  // not 0 x (what a masked key holds)
+          const bool hidden = partial && 8 * (v / 4) + v % 4 >= left;  // not 0 x (what a hidden key holds)
+          const float p = weight<T, KIND>(x[v], sc.mul, w[v], lse.value, lse.rest);
+          ds[v] = hidden ? 0.0f : p * (KIND == 0 ? Lift<T>::ds / Lift<T>::p : c[v]) * (y[v] - delta);
+          sum += hidden ? 0.0f : p * y[v];
         }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          const DofFrag<T> f = dof_frag_pack<T>(ds + 8 * s);
-          const int r = 32 * u + 16 * s + 4 * half;
+          const DofFrag<T> f = dof_frag_pack<T>(ds + 8 * s), rest = dof_frag_rest<T>(ds + 8 * s, f);
+          const int r = 16 * s + 4 * half;
 #pragma unroll
-          for (int d = 0; d < DT; ++d) dq[d] = dof_mma32<T>(sk[buf].colfrag(r, r + 8, 32 * d + col), f, dq[d]);
+          for (int d = 0; d < DT; ++d) {
+            const DofFrag<T> k = sk[buf].colfrag(r, r + 8, 32 * d + col);
+            dq[d] = dof_mma32<T>(k, f, dq[d]);
+            if constexpr (sizeof(T) == 2) dq[d] = dof_mma32<T>(k, rest, dq[d]);
+          }
         }
       }
+      if (next < kmax) {
+        rk.store(sk[buf ^ 1], tid);
+        rv.store(sv[buf ^ 1], tid);
+      }
     }
-    if (next < kmax) {
-      rk.store(sk[buf ^ 1], tid);
-      rv.store(sv[buf ^ 1], tid);
+    sum = (sum + dof_swap32(sum)) / Lift<T>::p;
+    if (pass == 0) {
+      delta = sum;
+      __syncthreads();  // the second pass fills the images anew
     }
   }
   if (!live) return;
+  if (half == 0) B.delta[srow] = sum;
   const float out = B.scale / Lift<T>::ds;
   T* dqp = static_cast<T*>(B.dq) + (t.q0 + row) * B.dqs[0] + h * B.dqs[1];
 #pragma unroll
@@ -163,18 +210,18 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_
 }
 
 // Documents of at most 32 query rows and 32 keys: all three gradients from one pass of one wavefront per document and key head.  S and dP
-// are computed once (five products), q, k, v, o and g are read once and delta never leaves the workgroup.  dS turns from "lane = key"
+// are computed once (five products), q, k, v and g are read once, and delta is the sum of P dP over the lanes.  dS turns from "lane = key"
 // to "lane = query" through LDS for dq; dk and dv add up over the group's query heads in registers.
-template <class T, int DP, bool PLAIN>
+template <class T, int DP, int KIND>
 __global__ void __launch_bounds__(64, DP <= 32 ? 2 : 1) k_attn_bwd_one(DofAttnBwd B) {
   const DofAttnFwd& A = B.f;
   constexpr int KS = DP / 16, DT = (DP + 31) / 32;
   using Tile = DofTile<T, 32, 32 * DT>;
   using Stage = DofStage<T, 32, 32 * DT, 64>;
   __shared__ Tile sq, sg, sk;
-  __shared__ DofTile<T, 32, 32> sds;  // dS, [query][key]
+  __shared__ DofTile<T, 32, 32> sds[sizeof(T) == 2 ? 2 : 1];  // dS, [query][key], and what its rounding left
   alignas(16) __shared__ float sl[32];
-  alignas(16) __shared__ float sd[32];
+  alignas(16) __shared__ float sr[32];
   const int lane = threadIdx.x, col = lane & 31, half = lane >> 5;
   const int group = A.q_heads / A.k_heads;
   int tile, hk;
@@ -204,34 +251,13 @@ __global__ void __launch_bounds__(64, DP <= 32 ? 2 : 1) k_attn_bwd_one(DofAttnBw
   for (int h = hk * group; h < (hk + 1) * group; ++h) {
     rq.load(static_cast<const T*>(A.q) + t.q0 * A.qs[0] + h * A.qs[1], A.qs[0], t.lq, A.dim, lane);
     rg.load(static_cast<const T*>(B.g) + t.q0 * B.gs[0] + h * B.gs[1], B.gs[0], t.lq, A.dim, lane);
-    const T* op = static_cast<const T*>(A.o) + (t.q0 + col) * A.os[0] + h * A.os[1];
-    DofFrag<T> of[KS];
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const int e = 16 * s + 8 * half;
-      of[s] = dof_frag_zero<T>();
-      if (row && e < A.dim) of[s] = dof_frag_load<T>(op + e);
-    }
-    float lse2 = INFINITY;
-    if (row) lse2 = A.lse[(t.q0 + col) * A.q_heads + h] * kLog2e;
-    if (lse2 == -INFINITY) lse2 = INFINITY;  // a row without keys takes no part
+    const Lse lse = lse_of<T>(row ? A.lse[(t.q0 + col) * A.q_heads + h] : -INFINITY);
     __syncthreads();  // the previous head's reads are done
     rq.store(sq, lane);
     rg.store(sg, lane);
-    __syncthreads();
-    float delta = 0.0f;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      float a[8], b[8];
-      dof_frag_unpack<T>(sg.rowfrag(col, 2 * s + half), a);
-      dof_frag_unpack<T>(of[s], b);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) delta = fmaf(a[i], b[i], delta);
-    }
-    delta += dof_swap32(delta);
     if (half == 0) {
-      sl[col] = lse2 - Lift<T>::p2;
-      sd[col] = delta;
+      sl[col] = lse.value;
+      sr[col] = lse.rest;
     }
     __syncthreads();
     dof_f32x16 x = dof_zero16(), y = dof_zero16();
@@ -240,44 +266,44 @@ __global__ void __launch_bounds__(64, DP <= 32 ? 2 : 1) k_attn_bwd_one(DofAttnBw
       x = dof_mma32<T>(sq.rowfrag(col, 2 * s + half), sk.rowfrag(col, 2 * s + half), x);
       y = dof_mma32<T>(sg.rowfrag(col, 2 * s + half), vf[s], y);
     }
-    float p[16], ds[16];
-    const float slope = !PLAIN && A.slopes ? A.slopes[h] * kLog2e : 0.0f;
+    float p[16], ds[16], w[16], c[16];
     const float base = (float)(off + 4 * half - col);
     const int left = live ? mine - 4 * half : 32;
-#pragma unroll
-    for (int v = 0; v < 16; ++v) {
-      const int r = 8 * (v / 4) + v % 4;
-      float c = Lift<T>::ds / Lift<T>::p;
-      const float ls = sl[r + 4 * half];
-      if constexpr (PLAIN) {
-        p[v] = dof_exp2(fmaf(x[v], A.score.mul, -ls));
-      } else {
-        float w = x[v] * A.score.mul;
-        if (A.score.cap_l2 != 0.0f) {
-          const float th = dof_cap_tanh<T>(x[v], A.score.mul);
-          w = A.score.cap_l2 * th;
-          c *= fmaf(-th, th, 1.0f);
-        }
-        if (A.slopes) w -= slope * fabsf(base + (float)r);
-        p[v] = dof_exp2(w - ls);
-      }
-      ds[v] = p[v] * c * (y[v] - sd[r + 4 * half]);
-      if (r < left) p[v] = ds[v] = 0.0f;
-    }
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const DofFrag<T> pf = dof_frag_pack<T>(p + 8 * s), df = dof_frag_pack<T>(ds + 8 * s);
-      const int r = 16 * s + 4 * half;
-#pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        dv[d] = dof_mma32<T>(sg.colfrag(r, r + 8, 32 * d + col), pf, dv[d]);
-        dk[d] = dof_mma32<T>(sq.colfrag(r, r + 8, 32 * d + col), df, dk[d]);
-      }
+    if constexpr (KIND > 0) {
+      DofScore sc = A.score;
+      if (A.slopes) sc.slope_l2 = A.slopes[h] * kLog2e;
+      scores<T, KIND>(x, sc, A.slopes != nullptr, [&](int v) { return base + (float)(8 * (v / 4) + v % 4); }, w, c);
     }
 #pragma unroll
     for (int v = 0; v < 16; ++v) {
       const int r = 8 * (v / 4) + v % 4 + 4 * half;
-      DofElem<T>::put(reinterpret_cast<T*>(sds.mem + sds.offset(r, col / Tile::EPC)) + col % Tile::EPC, ds[v]);
+      p[v] = weight<T, KIND>(x[v], A.score.mul, w[v], sl[r], sr[r]);
+      const bool hidden = 8 * (v / 4) + v % 4 < left;
+      p[v] = hidden ? 0.0f : p[v];
+      // delta = the row's sum of P dP: over the 32 lanes that hold the row
+      float d = hidden ? 0.0f : p[v] * y[v];
+      d = dof_row16_sum(d);
+      d += __shfl_xor(d, 16);
+      ds[v] = hidden ? 0.0f : p[v] * (KIND == 0 ? Lift<T>::ds / Lift<T>::p : c[v]) * (y[v] - d / Lift<T>::p);
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const DofFrag<T> pf = dof_frag_pack<T>(p + 8 * s), df = dof_frag_pack<T>(ds + 8 * s), rest = dof_frag_rest<T>(ds + 8 * s, df);
+      const int r = 16 * s + 4 * half;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        dv[d] = dof_mma32<T>(sg.colfrag(r, r + 8, 32 * d + col), pf, dv[d]);
+        const DofFrag<T> q = sq.colfrag(r, r + 8, 32 * d + col);
+        dk[d] = dof_mma32<T>(q, df, dk[d]);
+        if constexpr (sizeof(T) == 2) dk[d] = dof_mma32<T>(q, rest, dk[d]);
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      const int to = sds[0].offset(8 * (v / 4) + v % 4 + 4 * half, col / Tile::EPC);
+      T* e = reinterpret_cast<T*>(sds[0].mem + to) + col % Tile::EPC;
+      DofElem<T>::put(e, ds[v]);
+      if constexpr (sizeof(T) == 2) DofElem<T>::put(reinterpret_cast<T*>(sds[1].mem + to) + col % Tile::EPC, ds[v] - DofElem<T>::get(e));
     }
     __syncthreads();
     // dq (queries in registers, d over the lanes) = dS K
@@ -287,10 +313,14 @@ __global__ void __launch_bounds__(64, DP <= 32 ? 2 : 1) k_attn_bwd_one(DofAttnBw
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       // the eight keys of an operand are rows 16 s + 8 half .. of K, four and four
-      const DofFrag<T> f = sds.rowfrag(col, 2 * s + half);
+      const DofFrag<T> f = sds[0].rowfrag(col, 2 * s + half);
       const int r = 16 * s + 8 * half;
 #pragma unroll
-      for (int d = 0; d < DT; ++d) dq[d] = dof_mma32<T>(f, sk.colfrag(r, r + 4, 32 * d + col), dq[d]);
+      for (int d = 0; d < DT; ++d) {
+        const DofFrag<T> k = sk.colfrag(r, r + 4, 32 * d + col);
+        dq[d] = dof_mma32<T>(f, k, dq[d]);
+        if constexpr (sizeof(T) == 2) dq[d] = dof_mma32<T>(sds[1].rowfrag(col, 2 * s + half), k, dq[d]);
+      }
     }
     const float out = B.scale / Lift<T>::ds;
     T* dqp = static_cast<T*>(B.dq) + t.q0 * B.dqs[0] + h * B.dqs[1];
@@ -323,7 +353,7 @@ __global__ void __launch_bounds__(64, DP <= 32 ? 2 : 1) k_attn_bwd_one(DofAttnBw
 // registers only one wavefront fits a SIMD, and one alone does not hide its own latencies (16384 frames, heads of 128: 6.4 ms in one
 // pass, 4 products; the two passes run 5).
 // A workgroup takes `heads_per` query heads of the group; several workgroups of one key tile leave fp32 parts for k_attn_join.
-template <class T, int DP, int NW, bool PLAIN, int WANT>
+template <class T, int DP, int NW, int KIND, int WANT>
 __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_attn_dkv(DofAttnBwd B) {
   const DofAttnFwd& A = B.f;
   constexpr bool DV = (WANT & 1) != 0, DK = (WANT & 2) != 0;
@@ -331,7 +361,8 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_
   using Tile = DofTile<T, kRows, DP>;
   using Stage = DofStage<T, kRows, DP, 64 * NW>;
   __shared__ Tile sq[2], sg[2];
-  alignas(16) __shared__ float sl[2][kRows];  // log-sum-exp in units of log 2 (+inf: the row takes no part)
+  alignas(16) __shared__ float sl[2][kRows];  // log-sum-exp, its rest
+  alignas(16) __shared__ float sr[2][kRows];
   alignas(16) __shared__ float sd[2][kRows];  // delta
   constexpr int KS = DP / 16, DT = DP / 32;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
@@ -377,18 +408,18 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_
   }
 
   Stage rq, rg;
-  float rl = 0.0f, rd = 0.0f;
+  Lse rl = {0.0f, 0.0f};
+  float rd = 0.0f;
   auto load = [&](int h, int i0) {
     rq.load(static_cast<const T*>(A.q) + (t.q0 + i0) * A.qs[0] + h * A.qs[1], A.qs[0], t.lq - i0, A.dim, tid);
     rg.load(static_cast<const T*>(B.g) + (t.q0 + i0) * B.gs[0] + h * B.gs[1], B.gs[0], t.lq - i0, A.dim, tid);
     if (tid < kRows) {
-      rl = INFINITY;
+      rl = lse_of<T>(-INFINITY);
       rd = 0.0f;
       if (i0 + tid < t.lq) {
         const int64_t srow = (t.q0 + i0 + tid) * A.q_heads + h;
-        rl = A.lse[srow] * kLog2e;
+        rl = lse_of<T>(A.lse[srow]);
         rd = B.delta[srow];
-        rl = rl == -INFINITY ? INFINITY : rl - Lift<T>::p2;
       }
     }
   };
@@ -396,7 +427,8 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_
     rq.store(sq[buf], tid);
     rg.store(sg[buf], tid);
     if (tid < kRows) {
-      sl[buf][tid] = rl;
+      sl[buf][tid] = rl.value;
+      if (sizeof(T) == 4) sr[buf][tid] = rl.rest;
       sd[buf][tid] = rd;
     }
   };
@@ -418,29 +450,20 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_
         x = dof_mma32<T>(sq[buf].rowfrag(col, 2 * s + half), kf[s], x);
         if constexpr (DK) y = dof_mma32<T>(sg[buf].rowfrag(col, 2 * s + half), vf[s], y);
       }
-      float p[16], ds[16];
-      const float slope = !PLAIN && A.slopes ? A.slopes[h] * kLog2e : 0.0f;
+      float p[16], ds[16], w[16], c[16];
       const float base = (float)(i0 + off + 4 * half - key);
       const bool partial = i0 < w_full;
       const int left = mine - i0 - 4 * half;  // rows before this one do not see the lane's key
+      if constexpr (KIND > 0) {
+        DofScore sc = A.score;
+        if (A.slopes) sc.slope_l2 = A.slopes[h] * kLog2e;
+        scores<T, KIND>(x, sc, A.slopes != nullptr, [&](int v) { return base + (float)(8 * (v / 4) + v % 4); }, w, c);
+      }
 #pragma unroll
       for (int v = 0; v < 16; ++v) {
-        const int r = 8 * (v / 4) + v % 4;
-        float c = Lift<T>::ds / Lift<T>::p;
-        const float lse2 = sl[buf][r + 4 * half];
-        if constexpr (PLAIN) {
-          p[v] = dof_exp2(fmaf(x[v], A.score.mul, -lse2));
-        } else {
-          float w = x[v] * A.score.mul;
-          if (A.score.cap_l2 != 0.0f) {
-            const float th = dof_cap_tanh<T>(x[v], A.score.mul);
-            w = A.score.cap_l2 * th;
-            c *= fmaf(-th, th, 1.0f);
-          }
-          if (A.slopes) w -= slope * fabsf(base + (float)r);
-          p[v] = dof_exp2(w - lse2);
-        }
-        if constexpr (DK) ds[v] = p[v] * c * (y[v] - sd[buf][r + 4 * half]);
+        const int r = 8 * (v / 4) + v % 4 + 4 * half;
+        p[v] = weight<T, KIND>(x[v], A.score.mul, w[v], sl[buf][r], sizeof(T) == 4 ? sr[buf][r] : 0.0f);
+        if constexpr (DK) ds[v] = p[v] * (KIND == 0 ? Lift<T>::ds / Lift<T>::p : c[v]) * (y[v] - sd[buf][r]);
       }
       if (partial) {
 #pragma unroll
@@ -459,9 +482,13 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_
           for (int d = 0; d < DT; ++d) dv[d] = dof_mma32<T>(sg[buf].colfrag(r, r + 8, 32 * d + col), f, dv[d]);
         }
         if constexpr (DK) {
-          const DofFrag<T> f = dof_frag_pack<T>(ds + 8 * s);
+          const DofFrag<T> f = dof_frag_pack<T>(ds + 8 * s), rest = dof_frag_rest<T>(ds + 8 * s, f);
 #pragma unroll
-          for (int d = 0; d < DT; ++d) dk[d] = dof_mma32<T>(sq[buf].colfrag(r, r + 8, 32 * d + col), f, dk[d]);
+          for (int d = 0; d < DT; ++d) {
+            const DofFrag<T> q = sq[buf].colfrag(r, r + 8, 32 * d + col);
+            dk[d] = dof_mma32<T>(q, f, dk[d]);
+            if constexpr (sizeof(T) == 2) dk[d] = dof_mma32<T>(q, rest, dk[d]);
+          }
         }
       }
     }
@@ -508,43 +535,35 @@ __global__ void __launch_bounds__(256) k_attn_join(DofAttnBwd B) {
   dof_store_vec<T, 4>(static_cast<T*>(blockIdx.y ? B.dv : B.dk) + row * st[0] + hk * st[1] + e, s);
 }
 
-template <class T, int DP, bool PLAIN>
-void launch_dq_as(const DofAttnBwd& B, int flat, hipStream_t stream) {
-  const unsigned blocks = (unsigned)((int64_t)B.f.n_tiles * B.f.q_heads);
-  if (flat) DOF_LAUNCH((k_attn_dq<T, DP, 1, PLAIN>), (blocks, 1, 1), (64, 1, 1), stream, B);
-  else DOF_LAUNCH((k_attn_dq<T, DP, 4, PLAIN>), (blocks, 1, 1), (256, 1, 1), stream, B);
-}
-template <class T, int DP, bool PLAIN, int WANT>
-void launch_dkv_want(const DofAttnBwd& B, int flat, hipStream_t stream) {
-  const unsigned blocks = (unsigned)((int64_t)B.f.n_tiles * B.f.k_heads * B.splits);
-  if (flat) DOF_LAUNCH((k_attn_dkv<T, DP, 1, PLAIN, WANT>), (blocks, 1, 1), (64, 1, 1), stream, B);
-  else DOF_LAUNCH((k_attn_dkv<T, DP, 4, PLAIN, WANT>), (blocks, 1, 1), (256, 1, 1), stream, B);
-}
-template <class T, int DP, bool PLAIN>
-void launch_dkv_as(const DofAttnBwd& B, int flat, hipStream_t stream) {
-  if constexpr (DP <= 64) {
-    launch_dkv_want<T, DP, PLAIN, 3>(B, flat, stream);
-  } else {
-    launch_dkv_want<T, DP, PLAIN, 1>(B, flat, stream);
-    launch_dkv_want<T, DP, PLAIN, 2>(B, flat, stream);
-  }
-}
 template <class T, int DP>
 void launch_dq(const DofAttnBwd& B, int flat, hipStream_t stream) {
-  if (dof_attn_plain(B.f)) launch_dq_as<T, DP, true>(B, flat, stream);
-  else launch_dq_as<T, DP, false>(B, flat, stream);
+  const unsigned blocks = (unsigned)((int64_t)B.f.n_tiles * B.f.q_heads);
+  DOF_ATTN_KIND(B.f, KIND, {
+    if (flat) DOF_LAUNCH((k_attn_dq<T, DP, 1, KIND>), (blocks, 1, 1), (64, 1, 1), stream, B);
+    else DOF_LAUNCH((k_attn_dq<T, DP, 4, KIND>), (blocks, 1, 1), (256, 1, 1), stream, B);
+  });
+}
+template <class T, int DP, int WANT>
+void launch_dkv_want(const DofAttnBwd& B, int flat, hipStream_t stream) {
+  const unsigned blocks = (unsigned)((int64_t)B.f.n_tiles * B.f.k_heads * B.splits);
+  DOF_ATTN_KIND(B.f, KIND, {
+    if (flat) DOF_LAUNCH((k_attn_dkv<T, DP, 1, KIND, WANT>), (blocks, 1, 1), (64, 1, 1), stream, B);
+    else DOF_LAUNCH((k_attn_dkv<T, DP, 4, KIND, WANT>), (blocks, 1, 1), (256, 1, 1), stream, B);
+  });
 }
 template <class T, int DP>
 void launch_dkv(const DofAttnBwd& B, int flat, hipStream_t stream) {
-  if (dof_attn_plain(B.f)) launch_dkv_as<T, DP, true>(B, flat, stream);
-  else launch_dkv_as<T, DP, false>(B, flat, stream);
+  if constexpr (DP <= 64) {
+    launch_dkv_want<T, DP, 3>(B, flat, stream);
+  } else {
+    launch_dkv_want<T, DP, 1>(B, flat, stream);
+    launch_dkv_want<T, DP, 2>(B, flat, stream);
+  }
 }
-
 template <class T, int DP>
 void launch_one(const DofAttnBwd& B, hipStream_t stream) {
   const unsigned blocks = (unsigned)((int64_t)B.f.n_tiles * B.f.k_heads);
-  if (dof_attn_plain(B.f)) DOF_LAUNCH((k_attn_bwd_one<T, DP, true>), (blocks, 1, 1), (64, 1, 1), stream, B);
-  else DOF_LAUNCH((k_attn_bwd_one<T, DP, false>), (blocks, 1, 1), (64, 1, 1), stream, B);
+  DOF_ATTN_KIND(B.f, KIND, DOF_LAUNCH((k_attn_bwd_one<T, DP, KIND>), (blocks, 1, 1), (64, 1, 1), stream, B));
 }
 
 }  // namespace

@@ -22,8 +22,8 @@ namespace {
 // Keys per step: 32, or 64 for heads over 64 (24 ragged recordings, heads of 64: 236 us with 64, 199 with 32, which leave room for four
 // wavefronts per SIMD; 16384 frames, heads of 128: 1.40 ms with 64, 1.48 with 32: two wavefronts either way).  A single wavefront takes
 // 32 and one LDS image: nobody else waits for it, and the smaller image lets more of them onto a CU.
-// PLAIN: neither cap nor bias, scale > 0 (its multiplication is part of the exponent's)
-template <class T, int DP, int NW, bool PLAIN>
+// KIND: the score function (dof_attn_kind)
+template <class T, int DP, int NW, int KIND>
 __global__ void __launch_bounds__(64 * NW, DP <= 32 ? (NW == 1 && sizeof(T) == 4 ? 3 : 4) : sizeof(T) == 4 && DP > 64 ? 1 : 2) k_attn_fwd(DofAttnFwd A) {
   constexpr int KU = NW == 1 || DP <= 64 ? 1 : 2, kKeys = 32 * KU, BUF = NW == 1 ? 1 : 2;
   constexpr int KS = DP / 16, DT = (DP + 31) / 32;  // DP = 16: half of the only 32-wide tile of d is padding
@@ -96,13 +96,18 @@ __global__ void __launch_bounds__(64 * NW, DP <= 32 ? (NW == 1 && sizeof(T) == 4
 #pragma unroll
         for (int s = 0; s < KS; ++s) x[u] = dof_mma32<T>(sk[buf].rowfrag(32 * u + col, 2 * s + half), q[s], x[u]);
       }
-      if constexpr (!PLAIN) {
+      if constexpr (KIND > 0) {
         const float base = (float)(pos - j0 - 4 * half);
-        if (sc.cap_l2 != 0.0f) {
+        if constexpr (KIND == 2) {
 #pragma unroll
-          for (int u = 0; u < KU; ++u)
+          for (int u = 0; u < KU; ++u) {
+            float th[16];
 #pragma unroll
-            for (int v = 0; v < 16; ++v) x[u][v] = sc.cap_l2 * dof_cap_tanh<T>(x[u][v], sc.mul);
+            for (int v = 0; v < 16; ++v) th[v] = x[u][v];
+            dof_cap_tanh<T, 16>(th, sc.mul);
+#pragma unroll
+            for (int v = 0; v < 16; ++v) x[u][v] = sc.cap_l2 * th[v];
+          }
           if (A.slopes) {
 #pragma unroll
             for (int u = 0; u < KU; ++u)
@@ -117,7 +122,7 @@ __global__ void __launch_bounds__(64 * NW, DP <= 32 ? (NW == 1 && sizeof(T) == 4
               x[u][v] = fmaf(x[u][v], sc.mul, -sc.slope_l2 * fabsf(base - (float)(32 * u + 8 * (v / 4) + v % 4)));
         }
       }
-      const float unit = PLAIN ? sc.mul : 1.0f;  // of x, in log 2
+      const float unit = KIND == 0 ? sc.mul : 1.0f;  // of x, in log 2
       if (j0 + kKeys > wmin) {
         const int left = kend - j0 - 4 * half;
 #pragma unroll
@@ -148,11 +153,13 @@ __global__ void __launch_bounds__(64 * NW, DP <= 32 ? (NW == 1 && sizeof(T) == 4
 #pragma unroll
       for (int u = 0; u < KU; ++u) {
         float p[16];
+        float part = 0.0f;  // a chain of one addition per step, not sixteen, for the long sum
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
           p[v] = dof_exp2(fmaf(x[u][v], unit, -mm));
-          l += p[v];
+          part += p[v];
         }
+        l += part;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           const DofFrag<T> pf = dof_frag_pack<T>(p + 8 * s);
@@ -198,16 +205,13 @@ __global__ void __launch_bounds__(64 * NW, DP <= 32 ? (NW == 1 && sizeof(T) == 4
   if (half == 0) A.lse[(t.q0 + row) * A.q_heads + h] = l == 0.0f ? -INFINITY : (m + dof_log2(l)) * kLn2;
 }
 
-template <class T, int DP, bool PLAIN>
-void launch_as(const DofAttnFwd& A, int flat, hipStream_t stream) {
-  const unsigned blocks = (unsigned)((int64_t)A.n_tiles * A.q_heads);
-  if (flat) DOF_LAUNCH((k_attn_fwd<T, DP, 1, PLAIN>), (blocks, 1, 1), (64, 1, 1), stream, A);
-  else DOF_LAUNCH((k_attn_fwd<T, DP, 4, PLAIN>), (blocks, 1, 1), (256, 1, 1), stream, A);
-}
 template <class T, int DP>
 void launch(const DofAttnFwd& A, int flat, hipStream_t stream) {
-  if (dof_attn_plain(A)) launch_as<T, DP, true>(A, flat, stream);
-  else launch_as<T, DP, false>(A, flat, stream);
+  const unsigned blocks = (unsigned)((int64_t)A.n_tiles * A.q_heads);
+  DOF_ATTN_KIND(A, KIND, {
+    if (flat) DOF_LAUNCH((k_attn_fwd<T, DP, 1, KIND>), (blocks, 1, 1), (64, 1, 1), stream, A);
+    else DOF_LAUNCH((k_attn_fwd<T, DP, 4, KIND>), (blocks, 1, 1), (256, 1, 1), stream, A);
+  });
 }
 
 }  // namespace

@@ -301,10 +301,12 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) k_attn
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
       if (A.score.cap_l2 != 0.0f) {
+        float th[8];
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int k = 0; k < 8; ++k) th[k] = x[i][k / 4][k % 4];
+        dof_cap_tanh<T, 8>(th, A.score.mul);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[i][u][e] = A.score.cap_l2 * dof_cap_tanh<T>(x[i][u][e], A.score.mul);
+        for (int k = 0; k < 8; ++k) x[i][k / 4][k % 4] = A.score.cap_l2 * th[k];
       } else {
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -347,14 +349,15 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) k_attn
           for (int e = 0; e < 4; ++e) o[i][d][e] *= a;
       }
       const float mm = m[i] == -INFINITY ? 0.0f : m[i];
-      float p[8];
+      float p[8], part = 0.0f;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           p[4 * u + e] = dof_exp2(x[i][u][e] - mm);
-          l[i] += p[4 * u + e];
+          part += p[4 * u + e];
         }
+      l[i] += part;
       const DofFrag<T> pf = dof_frag_pack<T>(p);
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[i][d] = dof_mma16<T>(sv[wave].colfrag(4 * quad, 16 + 4 * quad, 16 * d + col), pf, o[i][d]);

@@ -27,7 +27,20 @@ struct DofAttnBwd {
   float* part;
 };
 
-static inline bool dof_attn_plain(const DofAttnFwd& A) { return A.score.cap_l2 == 0.0f && !A.slopes && A.score.mul > 0.0f; }
+// The kernels' score function: 0 plain (scale > 0; its multiplication is part of the exponent's), 1 with a distance bias (or another
+// scale), 2 capped, with or without a bias.
+static inline int dof_attn_kind(const DofAttnFwd& A) {
+  if (A.score.cap_l2 != 0.0f) return 2;
+  return A.slopes || !(A.score.mul > 0.0f) ? 1 : 0;
+}
+// DOF_ATTN_KIND(A, KIND, expr): expr with KIND = that number
+#define DOF_ATTN_KIND(A, KIND, ...)                                       \
+  do {                                                                    \
+    const int _kind = dof_attn_kind(A);                                   \
+    if (_kind == 0) { constexpr int KIND = 0; __VA_ARGS__; }              \
+    else if (_kind == 1) { constexpr int KIND = 1; __VA_ARGS__; }         \
+    else { constexpr int KIND = 2; __VA_ARGS__; }                         \
+  } while (0)
 
 int dof_launch_attn_fwd(const DofAttnFwd& A, int dtype, int flat, hipStream_t stream);
 int dof_launch_attn_dq(const DofAttnBwd& A, int dtype, int flat, hipStream_t stream);

@@ -58,6 +58,15 @@ template <class T> __device__ __forceinline__ void dof_frag_unpack(const DofFrag
   }
 }
 
+// what rounding to `f` left of the eight values, as a second fragment: the two carry them to 16 (bf16) or 22 (fp16) bits
+template <class T> __device__ __forceinline__ DofFrag<T> dof_frag_rest(const float* v, const DofFrag<T>& f) {
+  float r[8];
+  dof_frag_unpack<T>(f, r);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = v[i] - r[i];
+  return dof_frag_pack<T>(r);
+}
+
 // Sixteen bytes of elements with zeros in the place of infinities and NaN; were there any?
 template <class T> __device__ __forceinline__ bool dof_make_finite(DofWords<4>& v) {
   bool any = false;
