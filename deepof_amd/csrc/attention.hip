@@ -29,36 +29,35 @@ int check_plan_args(int32_t n_docs, const int64_t* q_off, const int64_t* k_off, 
   return DOF_OK;
 }
 
-struct Listed {
-  DofAttnTile tile;
-  int64_t work;
-};
-
 // keys visible to row i, as dof_attn_kend
 int64_t kend(int64_t lq, int64_t lk, int64_t prefix, int causal, int64_t i) {
   if (!causal) return lk;
   return std::max<int64_t>(0, std::min(lk, std::max(prefix, i + lk - lq + 1)));
 }
 
-void list_tiles(const DofAttnPlan* p, const int64_t* q_off, const int64_t* k_off, const int32_t* prefix, bool keys, int rows,
-                std::vector<Listed>* out) {
+// The tiles of one list, longest first (documents and rows in order among equals).
+void list_tiles(const DofAttnPlan* p, const int64_t* q_off, const int64_t* k_off, const int32_t* prefix, bool keys, int rows, int64_t n,
+                DofAttnTile* out) {
+  std::vector<int64_t> work((size_t)n);
+  bool falling = true;
+  int64_t at = 0;
   for (int32_t d = 0; d < p->n_docs; ++d) {
     const int64_t lq = q_off[d + 1] - q_off[d], lk = k_off[d + 1] - k_off[d];
     const int64_t pre = prefix ? std::max(0, prefix[d]) : 0;
-    for (int64_t r = 0; r < (keys ? lk : lq); r += rows) {
-      Listed e;
-      e.tile.q0 = q_off[d];
-      e.tile.k0 = k_off[d];
-      e.tile.lq = (int32_t)lq;
-      e.tile.lk = (int32_t)lk;
-      e.tile.prefix = (int32_t)std::min(pre, lk);
-      e.tile.row0 = (int32_t)r;
-      if (keys) e.work = !p->causal || r < pre ? lq : lq - std::min(lq, std::max<int64_t>(0, r - (lk - lq)));
-      else e.work = kend(lq, lk, pre, p->causal, std::min(r + rows, lq) - 1);
-      out->push_back(e);
+    for (int64_t r = 0; r < (keys ? lk : lq); r += rows, ++at) {
+      out[at] = {q_off[d], k_off[d], (int32_t)lq, (int32_t)lk, (int32_t)std::min(pre, lk), (int32_t)r};
+      if (keys) work[at] = !p->causal || r < pre ? lq : lq - std::min(lq, std::max<int64_t>(0, r - (lk - lq)));
+      else work[at] = kend(lq, lk, pre, p->causal, std::min(r + rows, lq) - 1);
+      falling = falling && (at == 0 || work[at] <= work[at - 1]);
     }
   }
-  std::stable_sort(out->begin(), out->end(), [](const Listed& a, const Listed& b) { return a.work > b.work; });
+  if (falling) return;
+  std::vector<int64_t> order((size_t)n);
+  for (int64_t i = 0; i < n; ++i) order[i] = i;
+  std::stable_sort(order.begin(), order.end(), [&](int64_t a, int64_t b) { return work[a] > work[b]; });
+  std::vector<DofAttnTile> sorted((size_t)n);
+  for (int64_t i = 0; i < n; ++i) sorted[i] = out[order[i]];
+  std::copy(sorted.begin(), sorted.end(), out);
 }
 
 int64_t count_tiles(int32_t n_docs, const int64_t* off, int rows) {
@@ -100,11 +99,9 @@ int check(const DofAttnPlan* p, const void* table, const DofAttention* d, const 
   return DOF_OK;
 }
 
-// list 0: query tiles of 128 rows, 1: of 32; 2: key tiles of 64, 3: of 32
+// list 0: query tiles of 128 rows, 1: of 32; 2: key tiles of 128, 3: of 32
 const DofAttnTile* list_at(const DofAttnPlan* p, const void* table, int list) {
-  const DofAttnTile* t = static_cast<const DofAttnTile*>(table);
-  for (int i = 0; i < list; ++i) t += p->n_tiles[i];
-  return t;
+  return static_cast<const DofAttnTile*>(table) + p->first[list];
 }
 
 // Tiles of 128 rows (four wavefronts share what is staged) unless the documents are so short that most of such a tile is empty, or
@@ -130,8 +127,11 @@ Shares shares_of(const DofAttnPlan* p, const DofAttention* d) {
   return s;
 }
 
-// Small documents and heads up to 64: one kernel for all three gradients (4096 windows of 25 frames, 4 heads of 16, fp32)
-bool one_pass(const DofAttnPlan* p, const DofAttention* d) { return p->small && d->head_dim <= 64; }
+// Small documents: one kernel for all three gradients (4096 windows of 25 frames, 4 heads of 16, fp32: 84 us, dq and dk / dv kernels 138).
+// fp32 heads over 64 would not fit its registers.
+bool one_pass(const DofAttnPlan* p, const DofAttention* d) {
+  return p->small && d->head_dim <= (d->dtype == DOF_DTYPE_F32 ? 64 : 128);
+}
 
 int64_t delta_bytes(const DofAttnPlan* p, const DofAttention* d) { return (p->q_rows * d->q_heads * 4 + 15) / 16 * 16; }
 
@@ -188,8 +188,22 @@ extern "C" int dof_attn_plan_size(int32_t n_docs, const int64_t* q_off, const in
   plan->n_tiles[1] = count_tiles(n_docs, q_off, kAttnFlat);
   plan->n_tiles[2] = count_tiles(n_docs, k_off, kAttnTall);
   plan->n_tiles[3] = count_tiles(n_docs, k_off, kAttnFlat);
-  plan->table_bytes = 0;
-  for (int i = 0; i < 4; ++i) plan->table_bytes += plan->n_tiles[i] * (int64_t)sizeof(DofAttnTile);
+  // Equal lists are kept once: documents of one tile each (tall and flat), and queries and keys of the same rows whose work is the same
+  bool self = true;
+  int64_t with_rows = 0;
+  for (int32_t i = 0; i < n_docs; ++i) {
+    self = self && q_off[i + 1] - q_off[i] == k_off[i + 1] - k_off[i];
+    with_rows += q_off[i + 1] > q_off[i];
+  }
+  int64_t entries = 0;
+  for (int i = 0; i < 4; ++i) {
+    int same = -1;
+    if (i % 2 == 1 && plan->n_tiles[i] == plan->n_tiles[i - 1]) same = i - 1;
+    else if (i >= 2 && self && (!causal || plan->n_tiles[i] == with_rows)) same = i - 2;
+    plan->first[i] = same >= 0 ? plan->first[same] : entries;
+    if (same < 0) entries += plan->n_tiles[i];
+  }
+  plan->table_bytes = entries * (int64_t)sizeof(DofAttnTile);
   return DOF_OK;
 }
 
@@ -202,7 +216,7 @@ extern "C" int dof_attn_plan_table(const DofAttnPlan* plan, const int64_t* q_off
   DofAttnPlan again;
   const int rc = dof_attn_plan_size(plan->n_docs, q_off, k_off, plan->causal, &again);
   if (rc != DOF_OK) return rc;
-  if (memcmp(again.n_tiles, plan->n_tiles, sizeof(again.n_tiles)) || again.table_bytes != plan->table_bytes) {
+  if (memcmp(again.n_tiles, plan->n_tiles, sizeof(again.n_tiles)) || memcmp(again.first, plan->first, sizeof(again.first)) || again.table_bytes != plan->table_bytes) {
     dof_set_error("dof_attn_plan_table: the offsets are not those the plan was sized for");
     return DOF_ERR_ARG;
   }
@@ -212,12 +226,12 @@ extern "C" int dof_attn_plan_table(const DofAttnPlan* plan, const int64_t* q_off
     return DOF_ERR_ARG;
   }
   try {
-    DofAttnTile* out = static_cast<DofAttnTile*>(table);
+    int64_t done = 0;
     for (int i = 0; i < 4; ++i) {
-      std::vector<Listed> list;
-      list.reserve((size_t)plan->n_tiles[i]);
-      list_tiles(plan, q_off, k_off, prefix, i >= 2, i % 2 ? kAttnFlat : kAttnTall, &list);
-      for (const Listed& e : list) *out++ = e.tile;
+      if (plan->first[i] < done || plan->n_tiles[i] == 0) continue;  // kept as an earlier list
+      list_tiles(plan, q_off, k_off, prefix, i >= 2, i % 2 ? kAttnFlat : kAttnTall, plan->n_tiles[i],
+                 static_cast<DofAttnTile*>(table) + plan->first[i]);
+      done = plan->first[i] + plan->n_tiles[i];
     }
   } catch (const std::bad_alloc&) {
     dof_set_error("dof_attn_plan_table: out of host memory");

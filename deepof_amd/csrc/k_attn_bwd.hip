@@ -594,7 +594,11 @@ int dof_launch_attn_bwd_one(const DofAttnBwd& B, int dtype, hipStream_t stream) 
   DOF_SEQ_DISPATCH(dtype, T, {
     if (B.f.dim <= 16) launch_one<T, 16>(B, stream);
     else if (B.f.dim <= 32) launch_one<T, 32>(B, stream);
-    else launch_one<T, 64>(B, stream);
+    else if (B.f.dim <= 64) launch_one<T, 64>(B, stream);
+    else if constexpr (sizeof(T) == 2) {
+      if (B.f.dim <= 96) launch_one<T, 96>(B, stream);
+      else launch_one<T, 128>(B, stream);
+    }
   });
   return dof_check_launch("k_attn_bwd_one");
 }

@@ -45,4 +45,4 @@ static inline int dof_attn_kind(const DofAttnFwd& A) {
 int dof_launch_attn_fwd(const DofAttnFwd& A, int dtype, int flat, hipStream_t stream);
 int dof_launch_attn_dq(const DofAttnBwd& A, int dtype, int flat, hipStream_t stream);
 int dof_launch_attn_dkv(const DofAttnBwd& A, int dtype, int flat, hipStream_t stream);
-int dof_launch_attn_bwd_one(const DofAttnBwd& B, int dtype, hipStream_t stream);  // heads of at most 64
+int dof_launch_attn_bwd_one(const DofAttnBwd& B, int dtype, hipStream_t stream);  // heads of at most 64 (fp32) or 128

@@ -524,7 +524,7 @@ typedef struct {
   int32_t n_docs, causal;
   int32_t small, reserved; /* 1: no document has more than 32 rows or keys, or rows without any key */
   int64_t q_rows, k_rows;  /* the last offsets */
-  int64_t n_tiles[4];
+  int64_t n_tiles[4], first[4]; /* lists of tiles in the table (equal lists are kept once) */
   int64_t table_bytes;
 } DofAttnPlan;
 int dof_attn_plan_size(int32_t n_docs, const int64_t* q_off, const int64_t* k_off, int32_t causal, DofAttnPlan* plan);

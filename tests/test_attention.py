@@ -104,6 +104,8 @@ CASES = [
     ([130, 35], None, 2, 1, 96, True, None, 0.0, False, "odd"),
     ([32, 7, 25], [32, 30, 25], 4, 2, 64, True, [0, 3, 9], 6.0, True, "packed"),  # small documents: one backward kernel
     ([3, 0, 31], [32, 4, 1], 6, 1, 40, False, None, 0.0, False, "plain"),
+    ([2, 19], None, 4, 1, 128, True, None, 0.0, False, "packed"),
+    ([11, 1, 30], None, 2, 2, 72, True, None, 4.0, True, "plain"),
 ]
 
 
