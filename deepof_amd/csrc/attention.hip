@@ -104,12 +104,11 @@ const DofAttnTile* list_at(const DofAttnPlan* p, const void* table, int list) {
   return static_cast<const DofAttnTile*>(table) + p->first[list];
 }
 
-// Tiles of 128 rows (four wavefronts share what is staged) unless the documents are so short that most of such a tile is empty, or
-// there are so few of them that most CUs would go without work.
-int flat_tiles(const DofAttnPlan* p, int which, int heads) {
-  const int64_t tall = p->n_tiles[which], flat = p->n_tiles[which + 1];
-  return flat * 2 < tall * 5 || (tall * heads < 256 && flat > tall);
-}
+// Tiles of 128 rows (four wavefronts share what is staged) unless the documents are so short that most of such a tile is empty
+// (fewer than 2.5 flat tiles of 32 rows per tall one).  Few tiles are no reason for flat ones: a lone wavefront that
+// stages for itself is slower than the CUs left empty cost (one recording of 5000 frames, 2 / 1 heads of 128, training: 0.83 ms tall,
+// 2.16 flat; of 300 frames, 4 heads of 64: 49 and 53 us).
+int flat_tiles(const DofAttnPlan* p, int which) { return p->n_tiles[which + 1] * 2 < p->n_tiles[which] * 5; }
 
 // dk / dv: a workgroup per key tile and key head goes through all query heads of the group.  Where those are too few to fill the chip
 // evenly (a causal tile's work ranges from nothing to all rows), the group's heads are shared out; the fp32 parts cost a write and a
@@ -118,7 +117,7 @@ struct Shares { int flat, splits, heads_per; };
 Shares shares_of(const DofAttnPlan* p, const DofAttention* d) {
   const int group = d->q_heads / d->k_heads;
   Shares s;
-  s.flat = flat_tiles(p, 2, d->q_heads);
+  s.flat = flat_tiles(p, 2);
   const int64_t items = p->n_tiles[2 + s.flat] * d->k_heads;
   int64_t want = items > 0 ? (2048 + items - 1) / items : 1;
   if (want > group) want = group;
@@ -256,7 +255,7 @@ extern "C" int dof_attention_forward(const DofAttnPlan* plan, const void* table,
     return DOF_ERR_UNSUPPORTED;
   }
   DofAttnFwd A = forward_args(d, q, k, v, slopes, o, lse);
-  const int flat = flat_tiles(plan, 0, d->q_heads);
+  const int flat = flat_tiles(plan, 0);
   set_tiles(&A, plan, table, 0, flat);
   return dof_launch_attn_fwd(A, d->dtype, flat, (hipStream_t)stream);
 }
@@ -308,7 +307,7 @@ extern "C" int dof_attention_backward(const DofAttnPlan* plan, const void* table
     return dof_launch_attn_bwd_one(B, d->dtype, (hipStream_t)stream);
   }
   if (rows) {
-    const int flat = flat_tiles(plan, 0, d->q_heads);
+    const int flat = flat_tiles(plan, 0);
     set_tiles(&B.f, plan, table, 0, flat);
     rc = dof_launch_attn_dq(B, d->dtype, flat, (hipStream_t)stream);
     if (rc != DOF_OK) return rc;
