@@ -15,8 +15,8 @@
 // times that, together with delta from the rounded o).  The second product costs a fifth: 16384 causal frames, 16 / 4 heads of 128, bf16:
 // dq 1.75 -> 2.28 ms, dk 1.83 -> 2.22 ms.  The dq kernel starts from
 // delta = g.o, sums the unrounded P dP on its way and leaves that delta to the dk kernel.  Everything that is summed is fp32.
-// fp16 has 5 exponent bits: there P is carried as 2^12 P and dS as 2^6 dS (exact factors, taken out at the end), so
-// that weights of long documents and small gradients stay out of its subnormals.
+// fp16 has 5 exponent bits: there P is carried as 2^12 P (an exact factor, taken out at the end), so that the weights of long
+// documents stay out of its subnormals.  dS is not lifted: gradients under a loss scale use the upper half of the range.
 #include <cmath>
 
 #include "deepof_hip.h"
@@ -31,7 +31,7 @@ template <class T> struct Lift {
   static constexpr float p2 = 0.0f, p = 1.0f, ds = 1.0f;  // log2 of P's factor, P's factor, dS's factor
 };
 template <> struct Lift<DofF16> {
-  static constexpr float p2 = 12.0f, p = 4096.0f, ds = 64.0f;
+  static constexpr float p2 = 12.0f, p = 4096.0f, ds = 1.0f;
 };
 
 // A row's log-sum-exp in log 2, as the value and (fp32 elements) what its rounding left: there the weights are to be good to fp32, and
