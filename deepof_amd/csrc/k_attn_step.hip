@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) k_attn
         for (int k = 0; k < 4; ++k) vreg[i].w[k] = here.page >= 0 ? vreg[i].w[k] : 0u;
         // several new frames: a later one's value is hidden from the earlier rows, whose zero weight must not meet an infinity or
         // NaN; finish() puts such values where they are seen
-        if (MULTI && j0 + kStepKeys > len + 1) dof_make_finite<T>(vreg[i]);
+        if (MULTI && j0 + (lane & 31) >= len) dof_make_finite<T>(vreg[i]);
       }
     }
 #pragma unroll

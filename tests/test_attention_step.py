@@ -162,6 +162,10 @@ def test_unseen_places_reach_nothing(device, bad):
     t2["k"][0, 2], t2["v"][0, 2] = bad, bad
     got, _, _ = run(ops, t2, table, lengths, kc, vc, slopes, 0.0, device)
     assert torch.equal(got[:, :2], want[:, :2]) and not bool(torch.isfinite(got[:, 2]).any())
+    vb = vc.clone()  # a cached frame on the new frames' page: every row sees it
+    vb[used[2], 3] = bad
+    got, _, _ = run(ops, t, table, lengths, kc, vb, slopes, 0.0, device)
+    assert not bool(torch.isfinite(got).any())
 
 
 @pytest.mark.parametrize("device", DEVICES)
