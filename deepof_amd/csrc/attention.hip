@@ -2,7 +2,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
-#include <new>
+#include <exception>
 #include <vector>
 
 #include "deepof_hip.h"
@@ -12,7 +12,8 @@
 
 namespace {
 
-constexpr int64_t kMaxRows = 1 << 30;  // of one document
+constexpr int64_t kMaxRows = 1 << 30;           // of one document
+constexpr int64_t kMaxBlocks = (1LL << 24) - 1;  // of 256 threads: a launch holds less than 2^32
 
 int check_plan_args(int32_t n_docs, const int64_t* q_off, const int64_t* k_off, const void* out) {
   if (n_docs < 0 || (n_docs > 0 && (!q_off || !k_off)) || !out) {
@@ -92,7 +93,7 @@ int check(const DofAttnPlan* p, const void* table, const DofAttention* d, const 
     return DOF_ERR_ARG;
   }
   for (int i = 0; i < 4; ++i)
-    if (p->n_tiles[i] < 0 || p->n_tiles[i] * d->q_heads > 0x7FFFFFFF) {
+    if (p->n_tiles[i] < 0 || p->n_tiles[i] > kMaxBlocks / d->q_heads) {
       dof_set_error("%s: too many tiles for one launch (%lld tiles, %d heads)", who, (long long)p->n_tiles[i], (int)d->q_heads);
       return DOF_ERR_UNSUPPORTED;
     }
@@ -232,8 +233,8 @@ extern "C" int dof_attn_plan_table(const DofAttnPlan* plan, const int64_t* q_off
                  static_cast<DofAttnTile*>(table) + plan->first[i]);
       done = plan->first[i] + plan->n_tiles[i];
     }
-  } catch (const std::bad_alloc&) {
-    dof_set_error("dof_attn_plan_table: out of host memory");
+  } catch (const std::exception& e) {
+    dof_set_error("dof_attn_plan_table: %s", e.what());
     return DOF_ERR_STATE;
   }
   return DOF_OK;

@@ -566,7 +566,7 @@ extern "C" int dof_attention_step(const DofAttnStep* d, const void* q, const voi
   }
   const int64_t blocks = s.parts * d->k_heads * s.row_blocks;
   const int64_t rows = (int64_t)d->streams * d->k_heads * s.rows;
-  if (blocks > 0x7FFFFFFF || rows > 0x7FFFFFFF) {
+  if (blocks >= 1 << 24 || rows >= 1 << 24) {  // of 256 threads: a launch holds less than 2^32
     dof_set_error("dof_attention_step: too many streams and heads for one launch");
     return DOF_ERR_UNSUPPORTED;
   }

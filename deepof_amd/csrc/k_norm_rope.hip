@@ -369,7 +369,7 @@ int launch(Args A, hipStream_t stream) {
   A.chunks = (A.tokens + tb - 1) / tb;
   int64_t blocks = A.chunks;
   if (BWD && blocks > kBwdBlocks) blocks = kBwdBlocks;
-  if (blocks > 1 << 30) blocks = 1 << 30;
+  if (blocks > 1 << 20) blocks = 1 << 20;  // a launch holds less than 2^32 threads; the kernel goes through the chunks in strides
   const dim3 grid((unsigned)blocks, 2, 1);
   if constexpr (sizeof(T) == 2) {
     if (vec == 8) { launch_vec<T, 8, BWD>(A, grid, stream); return (int)blocks; }
