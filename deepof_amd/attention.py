@@ -7,6 +7,9 @@ causal / prefix masks, tanh cap, distance bias) -- both with their backward pass
 frames of live streams against a paged key / value cache.  Elements are float32, bfloat16 or float16; sums, norms and softmax
 statistics are fp32.
 
+Gradients are explicit: every ``*_backward`` takes the gradients at the outputs and returns those at the inputs; autograd does not
+record these calls.
+
 ``AttentionOps`` issues the C-ABI calls (include/deepof_hip.h) on the current HIP stream of its device; product code obtains it
 through :func:`create_attention_ops`, which requires a ROCm device and the compiled library and raises otherwise.  Workspaces and
 outputs come from torch's allocator, one per call, so calls on different streams and captured graphs never share memory.
@@ -14,6 +17,7 @@ outputs come from torch's allocator, one per call, so calls on different streams
 from __future__ import annotations
 
 import ctypes as C
+import math
 from typing import Optional, Sequence
 
 import numpy as np
@@ -93,9 +97,33 @@ def _is_wide(t: torch.Tensor) -> bool:
     bits = t.data_ptr()
     for s in t.stride()[:-1]:
         bits |= s * e
-    if not bits & 15:
-        return True
-    return t.data_ptr() % 16 == 0 and all(s * e % 16 == 0 for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n > 1)
+    return not bits & 15
+
+
+def _apart(name: str, out: Optional[torch.Tensor], **inputs):
+    """An output the caller gave may not lie in an input's memory: other workgroups still read it.  Both may be slices of one
+    buffer's rows (a packed q | k | v): rows of a common pitch are compared by their place in the pitch."""
+    if not isinstance(out, torch.Tensor) or out.numel() == 0:
+        return
+    for other, t in inputs.items():
+        if not isinstance(t, torch.Tensor) or t.numel() == 0:
+            continue
+        lo, inner, whole, outer = _extent(out)
+        lo2, inner2, whole2, outer2 = _extent(t)
+        if lo >= lo2 + whole2 or lo2 >= lo + whole:
+            continue
+        pitch = math.gcd(*outer, *outer2)
+        at = (lo2 - lo) % pitch if pitch else 0
+        if not (inner <= at and at + inner2 <= pitch):
+            raise ValueError(f"{name} must not share memory with {other}")
+
+
+def _extent(t: torch.Tensor):
+    """First byte, bytes from there of one (head, element) plane and of the whole, and the outer strides in bytes."""
+    e = t.element_size()
+    spans = [(n - 1) * s * e for n, s in zip(t.shape, t.stride())]
+    outer = [s * e for n, s in zip(t.shape[:-2], t.stride()[:-2]) if n > 1]
+    return t.data_ptr(), sum(spans[-2:]) + e, sum(spans) + e, outer
 
 
 def _wide(t: torch.Tensor) -> torch.Tensor:
@@ -212,6 +240,13 @@ class AttentionOps:
         ``interleaved``: neighbouring elements are a pair; otherwise the pairs lie half the rotated part apart.  head_dim: even, up
         to 256.  ``q_out`` / ``k_out`` may be q / k themselves."""
         head, ptrs = self._norm_rope_args(q, k, positions, freqs, q_weight, k_weight, eps, interleaved)
+        _apart("q_out", q_out, k=k)
+        _apart("k_out", k_out, q=q)
+        for name, out, x in (("q_out", q_out, q), ("k_out", k_out, k)):
+            if out is not None and (out.data_ptr() != x.data_ptr() or out.stride() != x.stride()):
+                _apart(name, out, **{name[0]: x})
+        if q_out is not None and k_out is not None:
+            _apart("q_out", q_out, k_out=k_out)
         q_out = self._output("q_out", q_out, q)
         k_out = self._output("k_out", k_out, k)
         rec = _capi.PACK_NORM_ROPE.pack(*head, *_st(q), *_st(k), *_st(q_out), *_st(k_out), 0, 0, 0, 0)
@@ -274,8 +309,9 @@ class AttentionOps:
         ``h // (query heads / key heads)``.  Scores ``scale q.k`` (default ``head_dim ** -0.5``), ``cap``: ``cap tanh(score / cap)``,
         ``slopes`` (fp32 per query head): minus ``slope * distance``.  lse (rows, query heads), fp32, natural log.  A row that sees no
         key gives zeros and -inf.  Rows behind the last document are left as they were in ``out`` / ``lse`` and are zeros in tensors
-        allocated here.  head_dim: a multiple of 8 up to 128."""
+        allocated here.  ``out`` may not lie in q, k or v.  head_dim: a multiple of 8 up to 128."""
         head, sl = self._attention_args(plan, q, k, v, scale, cap, slopes)
+        _apart("out", out, q=q, k=k, v=v)
         tail = q.shape[0] > plan.q_rows
         if out is None and tail:
             out = q.new_zeros(q.shape)
@@ -339,6 +375,9 @@ class AttentionOps:
             raise ValueError(f"caches {tuple(k_cache.shape)} / {tuple(v_cache.shape)} must be (pages, page size, {hk}, {dim})")
         if hk < 1 or hq % hk or hq < 1:
             raise ValueError(f"{hq} query heads are not a multiple of {hk} key heads")
+        _apart("out", out, q=q, k=k, v=v, k_cache=k_cache, v_cache=v_cache)
+        if k_cache.data_ptr() == v_cache.data_ptr() and k_cache.numel():
+            raise ValueError("k_cache and v_cache must be two tensors")
         if not (_is_wide(k_cache) and _is_wide(v_cache)):
             raise ValueError("the caches' address and strides must be multiples of 16 bytes")
         if page_table.dim() != 2 or page_table.shape[0] != b or page_table.dtype != torch.int32 or page_table.device != self.device \

@@ -237,7 +237,7 @@ def test_refusals(device):
         with pytest.raises(ValueError):
             ops.attention(*args)
     for kw in (dict(slopes=torch.zeros(3, device=device)), dict(out=torch.zeros(12, 4, 8, device=device)),
-               dict(lse=torch.zeros(12, 4, dtype=torch.float64, device=device)), dict(out=q[:1].expand(12, 4, 16))):
+               dict(lse=torch.zeros(12, 4, dtype=torch.float64, device=device)), dict(out=q[:1].expand(12, 4, 16)), dict(out=q)):
         with pytest.raises(ValueError):
             ops.attention(plan, q, k, v, **kw)
     for kw in (dict(cap=-1.0), dict(cap=float("nan")), dict(scale=float("inf"))):
@@ -320,3 +320,27 @@ def test_large_float16_gradients(device, lens):
     err = (P * (G.abs() @ V.abs().T + (P * dP.abs()).sum(1, keepdim=True)) * (n + 16) * 2.0 ** -24 + 2.0 ** -11 * dS.abs()) @ K.abs() / 4
     assert bool(((dq.cpu().double()[:, 0] - want).abs() <= 2.0 ** -11 * want.abs() + (1 + 2.0 ** -11) * err + 2.0 ** -25).all())
     assert bool((dk.cpu() == 0).all()) and bool(torch.isfinite(dv.cpu().float()).all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_outputs_beside_and_over_inputs(device):
+    """Slices of one buffer's rows are apart; anything that shares bytes is refused."""
+    ops = make_ops(device)
+    gen = torch.Generator().manual_seed(6)
+    rows = torch.randn(9, 4, 3, 16, generator=gen).to(device)  # o | q | k | v of a row, three heads
+    o, q, k, v = rows.unbind(1)
+    plan = ops.attention_plan([4, 5])
+    want, _ = ops.attention(plan, q.contiguous(), k.contiguous(), v.contiguous())
+    got, _ = ops.attention(plan, q, k, v, out=o)
+    assert got is o and torch.equal(o, want)
+    for bad in (q, k, v, rows.view(9, 12, 16)[:, 2:5], rows.view(9, 12, 16)[:, 9:12]):
+        with pytest.raises(ValueError, match="share memory"):
+            ops.attention(plan, q, k, v, out=bad)
+    pos = torch.arange(9, dtype=torch.int32, device=device)
+    freqs = torch.ones(8, dtype=torch.float64, device=device)
+    a, b = ops.norm_rope(q.clone(), k.clone(), pos, freqs)
+    ops.norm_rope(q, k, pos, freqs, q_out=q, k_out=k)  # in place, slices of one buffer
+    assert torch.equal(q, a) and torch.equal(k, b)
+    for kw in (dict(q_out=k), dict(k_out=q), dict(q_out=o, k_out=o)):
+        with pytest.raises(ValueError, match="share memory"):
+            ops.norm_rope(q, k, pos, freqs, **kw)

@@ -182,6 +182,10 @@ def test_refusals(device):
                  (q, k, v, kc[:1].expand(9, 8, 2, 16), kc[:1].expand(9, 8, 2, 16), tb, ln)):
         with pytest.raises(ValueError):
             ops.attention_step(*args)
+    with pytest.raises(ValueError, match="two tensors"):
+        ops.attention_step(q, k, v, kc, kc, tb, ln)
+    with pytest.raises(ValueError, match="share memory"):
+        ops.attention_step(q, k, v, kc, vc, tb, ln, out=q)
     with pytest.raises(DofError, match="new frames"):
         ops.attention_step(q[:, :1].expand(2, 17, 4, 16), k[:, :1].expand(2, 17, 2, 16), v[:, :1].expand(2, 17, 2, 16), kc, vc, tb, ln)
     with pytest.raises(DofError, match="head_dim"):

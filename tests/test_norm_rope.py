@@ -154,6 +154,9 @@ def test_refusals(device):
         ops.norm_rope(q, k, pd, fd, q_weight=torch.ones(15, device=device))
     with pytest.raises(ValueError):
         ops.norm_rope(q, k, pd, fd, q_out=q[:1].expand(4, 2, 16))
+    with pytest.raises(ValueError, match="share memory"):
+        buf = torch.zeros(5, 2, 16, device=device)
+        ops.norm_rope(buf[:4], k, pd, fd, q_out=buf[1:])
     with pytest.raises(ValueError):
         ops.norm_rope(q, k, pd, fd, eps=-1.0)
     with pytest.raises(DofError, match="head_dim"):
