@@ -350,8 +350,8 @@ __global__ void __launch_bounds__(64, DP <= 32 ? 2 : 1) k_attn_bwd_one(DofAttnBw
 }
 
 // WANT: 1 = dv, 2 = dk, 3 = both in one pass.  Heads over 64 take two passes: with both accumulators (and their operands) in
-// registers only one wavefront fits a SIMD, and one alone does not hide its own latencies (16384 frames, heads of 128: 6.4 ms in one
-// pass, 4 products; the two passes run 5).
+// registers only one wavefront fits a SIMD, and one alone does not hide its own latencies (16384 causal frames, 16 / 4
+// heads of 128, before dS took its second product: 6.4 ms in one pass of 4 products, 3.3 in two of 5; with it, 2 + 4: 3.65 ms).
 // A workgroup takes `heads_per` query heads of the group; several workgroups of one key tile leave fp32 parts for k_attn_join.
 template <class T, int DP, int NW, int KIND, int WANT>
 __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_attn_dkv(DofAttnBwd B) {

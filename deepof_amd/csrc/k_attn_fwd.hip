@@ -2,8 +2,8 @@
 //
 //   s_ij = scale q_i.k_j ; s = cap tanh(s / cap) ; s -= slope |pos_i - j| ; softmax over the visible keys ; o_i = sum_j p_ij v_j
 //
-// A workgroup owns a tile of query rows of one document and head (32 rows per wavefront) and walks the document's visible keys, 64
-// at a time, with a running maximum and sum; K and V pass through LDS (two images, the next one's loads in flight under the present
+// A workgroup owns a tile of query rows of one document and head (32 rows per wavefront) and walks the document's visible keys, 32
+// or 64 at a time, with a running maximum and sum; K and V pass through LDS (two images, the next one's loads in flight under the present
 // one's products).  The products are transposed -- S^T = K Q^T, O^T = V^T P^T -- so that a lane owns one query: its maximum, sum and
 // rescaling are lane-local but for one exchange with the other half-wavefront, and P^T leaves the first product in just the registers
 // the second one wants it in (the key order inside a fragment is permuted, the same on both operands).  V^T is read from row-major
