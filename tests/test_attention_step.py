@@ -106,6 +106,23 @@ def test_step(device, dtype, case):
     assert torch.equal(kd, kw) and torch.equal(vd, vw)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_more_streams_than_threads(device):
+    """300 streams on pages of 5, the long one at 280 in parts, some idle."""
+    ops = make_ops(device)
+    lens = [(7 * s) % 11 for s in range(300)]
+    lens[280] = 700
+    case = (lens, 1, 2, 1, 16, 5, 0.0, False)
+    t, table, lengths, kc, vc, slopes = build(case, torch.float32, device)
+    lengths[3], lengths[299] = -1, -1
+    out = torch.full((300, 1, 2, 16), 7.0, device=device)
+    o, kd, vd = run(ops, t, table, lengths, kc, vc, slopes, 0.0, device, out=out)
+    want, bound, kw, vw = reference(t, table, lengths, 5, kc.shape[0], 0.0, None, torch.float32, kc, vc)
+    live = lengths >= 0
+    assert_within("o", o.cpu()[live], want[live], bound[live])
+    assert bool((o.cpu()[~live] == 7).all()) and torch.equal(kd, kw) and torch.equal(vd, vw)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("case", [([20011, 3], 1, 8, 2, 128, 16, 0.0, False), ([9000] * 3 + [40] * 30, 2, 4, 4, 64, 32, 10.0, True)],
