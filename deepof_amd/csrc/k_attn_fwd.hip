@@ -8,7 +8,8 @@
 // rescaling are lane-local but for one exchange with the other half-wavefront, and P^T leaves the first product in just the registers
 // the second one wants it in (the key order inside a fragment is permuted, the same on both operands).  V^T is read from row-major
 // LDS by the transposing LDS read.  Statistics and accumulators are fp32; P is rounded to the elements' type for its product (relative
-// half a step per weight, as the inputs' own), the sum l is taken of the unrounded weights.
+// half a step per weight, as the inputs' own; fp16 weights are lifted out of their subnormals, see DofSoftmax), the sum l is taken of
+// the unrounded weights.
 #include <cmath>
 
 #include "deepof_hip.h"
@@ -137,9 +138,9 @@ __global__ void __launch_bounds__(64 * NW, DP <= 32 ? (NW == 1 && sizeof(T) == 4
 #pragma unroll
         for (int v = 0; v < 16; ++v) mt = fmaxf(mt, x[u][v]);
       mt = fmaxf(mt, dof_swap32(mt)) * unit;
-      // The running maximum follows only when a tile's exceeds it by 2^8: until then the weights stay below 256, which costs the
+      // The running maximum follows only when a tile's exceeds it by 2^kLag: until then the weights stay below that, which costs the
       // fp32 sums nothing, and the accumulators need no rescaling pass.
-      if (dof_wave_any(mt > m + 8.0f)) {
+      if (dof_wave_any(mt > m + DofSoftmax<T>::kLag)) {
         const float mn = fmaxf(m, mt);
         const float a = mn == -INFINITY ? 1.0f : dof_exp2(m - mn);
         m = mn;
@@ -149,7 +150,7 @@ __global__ void __launch_bounds__(64 * NW, DP <= 32 ? (NW == 1 && sizeof(T) == 4
 #pragma unroll
           for (int v = 0; v < 16; ++v) o[d][v] *= a;
       }
-      const float mm = m == -INFINITY ? 0.0f : m;
+      const float mm = m == -INFINITY ? 0.0f : m - DofSoftmax<T>::kUp;
 #pragma unroll
       for (int u = 0; u < KU; ++u) {
         float p[16];
@@ -202,7 +203,7 @@ __global__ void __launch_bounds__(64 * NW, DP <= 32 ? (NW == 1 && sizeof(T) == 4
         dof_store_vec<T, 4>(op + e, r);
       }
     }
-  if (half == 0) A.lse[(t.q0 + row) * A.q_heads + h] = l == 0.0f ? -INFINITY : (m + dof_log2(l)) * kLn2;
+  if (half == 0) A.lse[(t.q0 + row) * A.q_heads + h] = l == 0.0f ? -INFINITY : (m - DofSoftmax<T>::kUp + dof_log2(l)) * kLn2;
 }
 
 template <class T, int DP>

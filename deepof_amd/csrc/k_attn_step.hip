@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) k_attn
         for (int e = 0; e < 4; ++e) mt = fmaxf(mt, x[i][u][e]);
       mt = fmaxf(mt, __shfl_xor(mt, 16));
       mt = fmaxf(mt, dof_swap32(mt));
-      if (dof_wave_any(mt > m[i] + 8.0f)) {  // as in the forward pass: the maximum follows in steps of 2^8
+      if (dof_wave_any(mt > m[i] + DofSoftmax<T>::kLag)) {  // as in the forward pass: the maximum follows in steps
         const float mn = fmaxf(m[i], mt);
         const float a = mn == -INFINITY ? 1.0f : dof_exp2(m[i] - mn);
         m[i] = mn;
@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) k_attn
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[i][d][e] *= a;
       }
-      const float mm = m[i] == -INFINITY ? 0.0f : m[i];
+      const float mm = m[i] == -INFINITY ? 0.0f : m[i] - DofSoftmax<T>::kUp;  // a factor of the sums as of the weights
       float p[8], part = 0.0f;
 #pragma unroll
       for (int u = 0; u < 2; ++u)

@@ -30,6 +30,17 @@ struct DofScore {
 };
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
+// The running maximum of a softmax follows a new tile's only when that exceeds it by 2^kLag; weights are kept as 2^kUp times themselves
+// (products and sum alike, so that the factor leaves with the division).  fp16 has 5 exponent bits: without a factor a weight
+// below 2^-25 of the maximum is zero in the products while the sum counts it, and many such weights are a recording's tail.  With
+// 2^11 what a weight loses is at most 2^-36 of the largest, and the largest, 2^(4 + 11), stays below 65504.
+template <class T> struct DofSoftmax {
+  static constexpr float kLag = 8.0f, kUp = 0.0f;
+};
+template <> struct DofSoftmax<DofF16> {
+  static constexpr float kLag = 4.0f, kUp = 11.0f;
+};
+
 // t[i] = tanh(t[i] mul) of N scores of a lane.  Capped scores mostly lie well inside the cap: while all of the wavefront's are below 0.6 of
 // it, an odd polynomial (fitted to tanh(x) / x on [0, 0.6], relative error 1.1e-8) takes 8 instructions, none of them transcendental;
 // otherwise the library's tanh (fp32) or 1 - 2 / (1 + 2^(2 log2(e) x)), absolute error 2^-22.
