@@ -514,25 +514,30 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_
   if constexpr (DV) write(dv, ov, B.dv, B.dvs, B.part + B.splits * B.k_rows * A.k_heads * A.dim);
 }
 
-// dk and dv (blockIdx.y) from the parts of several workgroups per key tile, added in order.  Four elements a thread, rows of the tiles.
+// dk and dv (blockIdx.y) from the parts of several workgroups per key tile, added in order: a workgroup per 32 rows of a tile and key
+// head, four elements a thread.  Rows of no tile have no parts and stay.
+constexpr int kJoinRows = 32;
 template <class T>
-__global__ void __launch_bounds__(256) k_attn_join(DofAttnBwd B) {
+__global__ void __launch_bounds__(256) k_attn_join(DofAttnBwd B, int pieces) {
   const DofAttnFwd& A = B.f;
+  const int item = blockIdx.x / A.k_heads, hk = blockIdx.x - item * A.k_heads, tile = item / pieces;
+  const DofAttnTile t = A.tiles[tile];
+  const int first = t.row0 + (item - tile * pieces) * kJoinRows, rows = t.lk - first < kJoinRows ? t.lk - first : kJoinRows;
   const int quads = A.dim / 4;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t rh = i / quads, row = rh / A.k_heads;
-  if (row >= B.k_rows) return;
-  const int e = (int)(i - rh * quads) * 4, hk = (int)(rh - row * A.k_heads);
   const float* part = B.part + (blockIdx.y ? B.splits * B.k_rows * A.k_heads * A.dim : 0);
-  float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int k = 0; k < B.splits; ++k) {
-    float v[4];
-    dof_load_vec<float, 4>(part + ((k * B.k_rows + row) * A.k_heads + hk) * A.dim + e, v);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) s[j] += v[j];
-  }
   const int64_t* st = blockIdx.y ? B.dvs : B.dks;
-  dof_store_vec<T, 4>(static_cast<T*>(blockIdx.y ? B.dv : B.dk) + row * st[0] + hk * st[1] + e, s);
+  for (int i = threadIdx.x; i < rows * quads; i += 256) {
+    const int r = i / quads, e = 4 * (i - r * quads);
+    const int64_t row = t.k0 + first + r;
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k = 0; k < B.splits; ++k) {
+      float v[4];
+      dof_load_vec<float, 4>(part + ((k * B.k_rows + row) * A.k_heads + hk) * A.dim + e, v);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[j] += v[j];
+    }
+    dof_store_vec<T, 4>(static_cast<T*>(blockIdx.y ? B.dv : B.dk) + row * st[0] + hk * st[1] + e, s);
+  }
 }
 
 template <class T, int DP>
@@ -584,8 +589,10 @@ int dof_launch_attn_dkv(const DofAttnBwd& B, int dtype, int flat, hipStream_t st
     else if (B.f.dim <= 64) launch_dkv<T, 64>(B, flat, stream);
     else if (B.f.dim <= 96) launch_dkv<T, 96>(B, flat, stream);
     else launch_dkv<T, 128>(B, flat, stream);
-    if (B.splits > 1)
-      DOF_LAUNCH((k_attn_join<T>), (dof_cdiv(B.k_rows * B.f.k_heads * (B.f.dim / 4), 256), 2, 1), (256, 1, 1), stream, B);
+    if (B.splits > 1) {
+      const int pieces = (flat ? kAttnFlat : kAttnTall) / kJoinRows;
+      DOF_LAUNCH((k_attn_join<T>), ((unsigned)((int64_t)B.f.n_tiles * pieces * B.f.k_heads), 2, 1), (256, 1, 1), stream, B, pieces);
+    }
   });
   return dof_check_launch("k_attn_dkv");
 }

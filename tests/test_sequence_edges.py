@@ -1,10 +1,13 @@
 """Edges of the sequence operators: long tails of a softmax, long sums, what a row must not see, memory they may not touch, limits.
 Every bound is derived where it stands; u is half a step of the type, relative to the value."""
+import ctypes as C
 import math
 
+import numpy as np
 import pytest
 import torch
 
+from deepof_amd import _capi
 from sequence_common import DEVICES, DTYPES, TINY, U, U32, make_ops
 
 
@@ -58,3 +61,47 @@ def test_step_with_a_long_tail_behind_a_sink(device, dtype, n, gap):
     o = ops.attention_step(q[None].to(device), k[None, -1:].to(device), v[None, -1:].to(device), kc, vc, table,
                            torch.tensor([n - 1], dtype=torch.int32, device=device))
     assert float((o.cpu().double() - want).abs().max()) <= sink_bound(want, n, dtype)
+
+
+def plan_at(ops, q_off, k_off, causal, device):
+    """A plan through the C ABI, whose documents may begin behind row 0 -> the record and its table on the device."""
+    q_off, k_off = np.asarray(q_off, dtype=np.int64), np.asarray(k_off, dtype=np.int64)
+    plan = _capi.AttnPlan()
+    _capi.check(ops.lib, ops.lib.dof_attn_plan_size(len(q_off) - 1, q_off.ctypes.data, k_off.ctypes.data, causal, C.byref(plan)), "size")
+    host = torch.empty(max(16, plan.table_bytes), dtype=torch.uint8)
+    _capi.check(ops.lib, ops.lib.dof_attn_plan_table(C.byref(plan), q_off.ctypes.data, k_off.ctypes.data, 0, host.data_ptr()), "table")
+    return plan, host.to(device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("lens", [[40], [200, 33], [20]])  # flat key tiles, tall ones, a document of the small kernel's
+def test_rows_before_the_first_document_stay(device, dtype, lens):
+    """First offsets above 0: the rows before are neither read (NaN) nor written, the gradients are those of the batch alone."""
+    ops = make_ops(device)
+    lead, hq, hk, d = 8, 4, 1, 16
+    n = lead + sum(lens)
+    g = torch.Generator().manual_seed(2)
+    t = {x: torch.randn(n, h, d, generator=g).to(dtype).to(device) for x, h in (("q", hq), ("k", hk), ("v", hk), ("g", hq))}
+    alone = {x: y[lead:].contiguous() for x, y in t.items()}
+    whole = ops.attention_plan(lens, causal=True)
+    o, lse = ops.attention(whole, alone["q"], alone["k"], alone["v"])
+    want = dict(zip(("dq", "dk", "dv"), ops.attention_backward(whole, alone["g"], alone["q"], alone["k"], alone["v"], o, lse)), o=o, lse=lse)
+    for x in t.values():
+        x[:lead] = float("nan")
+    off = lead + np.concatenate(([0], np.cumsum(lens)))
+    plan, table = plan_at(ops, off, off, 1, device)
+    out = {x: torch.full((n, h, d), 7.0, dtype=dtype, device=device) for x, h in (("o", hq), ("dq", hq), ("dk", hk), ("dv", hk))}
+    out["lse"] = torch.full((n, hq), 7.0, device=device)
+    st = {x: (h * d, d) for x, h in (("q", hq), ("k", hk))}
+    rec = _capi.PACK_ATTENTION.pack(_capi.DTYPE_F32 + DTYPES.index(dtype), d, hq, hk, d ** -0.5, 0.0, *st["q"], *st["k"], *st["k"], *st["q"],
+                                    *st["q"], *st["q"], *st["k"], *st["k"])
+    p = {x: y.data_ptr() for x, y in (*t.items(), *out.items())}
+    ops._launch("dof_attention_forward", C.byref(plan), table.data_ptr(), rec, p["q"], p["k"], p["v"], 0, p["o"], p["lse"])
+    need = ops._bytes("dof_attention_workspace_bytes", C.byref(plan), rec)
+    ws = torch.full((max(16, need) // 4,), 123.0, device=device)
+    ops._launch("dof_attention_backward", C.byref(plan), table.data_ptr(), rec, p["g"], p["q"], p["k"], p["v"], 0, p["o"], p["lse"], p["dq"],
+                p["dk"], p["dv"], ws.data_ptr())
+    for x, y in out.items():
+        assert bool((y[:lead] == 7).all()), x
+        assert torch.equal(y[lead:], want[x]), x
