@@ -134,6 +134,11 @@ bool one_pass(const DofAttnPlan* p, const DofAttention* d) {
 }
 
 int64_t delta_bytes(const DofAttnPlan* p, const DofAttention* d) { return (p->q_rows * d->q_heads * 4 + 15) / 16 * 16; }
+int64_t workspace_bytes(const DofAttnPlan* p, const DofAttention* d) {  // 0: none (one kernel, or keys without any query row)
+  if (one_pass(p, d)) return 0;
+  const Shares s = shares_of(p, d);
+  return delta_bytes(p, d) + (s.splits > 1 ? 2 * s.splits * p->k_rows * d->k_heads * d->head_dim * 4 : 0);
+}
 
 DofAttnFwd forward_args(const DofAttention* d, const void* q, const void* k, const void* v, const float* slopes, void* o, float* lse) {
   DofAttnFwd A;
@@ -264,9 +269,7 @@ extern "C" int dof_attention_forward(const DofAttnPlan* plan, const void* table,
 extern "C" int64_t dof_attention_workspace_bytes(const DofAttnPlan* plan, const DofAttention* d) {
   static const char none = 0;
   if (check(plan, &none, d, "dof_attention_workspace_bytes") != DOF_OK) return -1;
-  if (one_pass(plan, d)) return 0;
-  const Shares s = shares_of(plan, d);
-  return delta_bytes(plan, d) + (s.splits > 1 ? 2 * s.splits * plan->k_rows * d->k_heads * d->head_dim * 4 : 0);
+  return workspace_bytes(plan, d);
 }
 
 extern "C" int dof_attention_backward(const DofAttnPlan* plan, const void* table, const DofAttention* d, const void* g, const void* q,
@@ -277,7 +280,7 @@ extern "C" int dof_attention_backward(const DofAttnPlan* plan, const void* table
   const bool rows = plan->n_tiles[0] > 0, keys = plan->n_tiles[2] > 0;
   if (!rows && !keys) return DOF_OK;
   const bool one = one_pass(plan, d);
-  if ((!one && !workspace) || (rows && (!g || !q || !o || !lse || !dq)) || (keys && (!k || !v || !dk || !dv))) {
+  if ((!workspace && workspace_bytes(plan, d) > 0) || (rows && (!g || !q || !o || !lse || !dq)) || (keys && (!k || !v || !dk || !dv))) {
     dof_set_error("dof_attention_backward: null tensor");
     return DOF_ERR_ARG;
   }

@@ -540,7 +540,7 @@ typedef struct {
 } DofAttention;
 int dof_attention_forward(const DofAttnPlan* plan, const void* table, const DofAttention* dims, const void* q, const void* k,
                           const void* v, const float* slopes, void* o, float* lse, void* stream);
-int64_t dof_attention_workspace_bytes(const DofAttnPlan* plan, const DofAttention* dims); /* of the backward call; -1: bad dims */
+int64_t dof_attention_workspace_bytes(const DofAttnPlan* plan, const DofAttention* dims); /* of the backward call; 0: none needed; -1: bad dims */
 int dof_attention_backward(const DofAttnPlan* plan, const void* table, const DofAttention* dims, const void* g, const void* q,
                            const void* k, const void* v, const float* slopes, const void* o, const float* lse, void* dq, void* dk,
                            void* dv, void* workspace, void* stream);

@@ -105,3 +105,16 @@ def test_rows_before_the_first_document_stay(device, dtype, lens):
     for x, y in out.items():
         assert bool((y[:lead] == 7).all()), x
         assert torch.equal(y[lead:], want[x]), x
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("hq,hk", [(2, 2), (4, 1)])  # a key head's query heads in one workgroup, and shared out
+@pytest.mark.parametrize("keys", [[50], [3], [0, 200]])
+def test_keys_without_any_query_row(device, hq, hk, keys):
+    ops = make_ops(device)
+    q, k, v = (torch.randn(n, h, 16).to(device) for n, h in ((0, hq), (sum(keys), hk), (sum(keys), hk)))
+    plan = ops.attention_plan([0] * len(keys), keys)
+    o, lse = ops.attention(plan, q, k, v)
+    dq, dk, dv = ops.attention_backward(plan, q, q, k, v, o, lse)
+    assert o.shape == dq.shape == (0, hq, 16) and lse.shape == (0, hq)
+    assert dk.shape == dv.shape == k.shape and bool((dk == 0).all()) and bool((dv == 0).all())
