@@ -133,7 +133,8 @@ def _wide(t: torch.Tensor) -> torch.Tensor:
 
 class AttentionPlan:
     """The tiles of one packed batch on the device (:meth:`AttentionOps.attention_plan`): serves any number of heads, head sizes,
-    dtypes and streams, forward and backward; never written after it is made."""
+    dtypes and streams, forward and backward; never written after it is made.  It may be dropped while calls that use it still
+    run; a captured graph reads it at every replay, so keep it as long as the graph."""
 
     def __init__(self, ops: "AttentionOps", q_lengths, k_lengths, causal, prefix):
         ql = self._host("q_lengths", q_lengths)
@@ -159,6 +160,13 @@ class AttentionPlan:
                                                          pre.ctypes.data if pre is not None else 0, host.data_ptr()),
                     "dof_attn_plan_table")
         self.table = host.to(self.device)
+
+    def on_current_stream(self) -> int:
+        """The table's address for a call on the current stream.  The allocator is told of that stream, so that a plan which is
+        dropped gives its memory back only behind the call, also where another stream made it."""
+        if self.table.is_cuda:
+            self.table.record_stream(torch.cuda.current_stream(self.device))
+        return self.table.data_ptr()
 
     @staticmethod
     def _host(name, lengths):
@@ -322,7 +330,7 @@ class AttentionOps:
         q, k, v = _wide(q), _wide(k), _wide(v)
         ow = o if _is_wide(o) else o.clone(memory_format=torch.contiguous_format)
         rec = _capi.PACK_ATTENTION.pack(*head, *_st(q), *_st(k), *_st(v), *_st(ow), 0, 0, 0, 0, 0, 0, 0, 0)
-        self._launch("dof_attention_forward", C.byref(plan.record), plan.table.data_ptr(), rec, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+        self._launch("dof_attention_forward", C.byref(plan.record), plan.on_current_stream(), rec, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                      sl, ow.data_ptr(), lse.data_ptr())
         if ow is not o:
             o.copy_(ow)
@@ -345,7 +353,7 @@ class AttentionOps:
         rec = _capi.PACK_ATTENTION.pack(*head, *_st(q), *_st(k), *_st(v), *_st(o), *_st(do), *_st(dq), *_st(dk), *_st(dv))
         need = self._bytes("dof_attention_workspace_bytes", C.byref(plan.record), rec)
         ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-        self._launch("dof_attention_backward", C.byref(plan.record), plan.table.data_ptr(), rec, do.data_ptr(), q.data_ptr(), k.data_ptr(),
+        self._launch("dof_attention_backward", C.byref(plan.record), plan.on_current_stream(), rec, do.data_ptr(), q.data_ptr(), k.data_ptr(),
                      v.data_ptr(), sl, o.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(ws))
         return dq, dk, dv
 

@@ -118,3 +118,25 @@ def test_keys_without_any_query_row(device, hq, hk, keys):
     dq, dk, dv = ops.attention_backward(plan, q, q, k, v, o, lse)
     assert o.shape == dq.shape == (0, hq, 16) and lse.shape == (0, hq)
     assert dk.shape == dv.shape == k.shape and bool((dk == 0).all()) and bool((dv == 0).all())
+
+
+@pytest.mark.gpu
+def test_a_dropped_plan_stays_until_the_streams_that_use_it_are_done():
+    """Made on the default stream, used on another one that is still busy: the block of its tiles is not handed out again before."""
+    ops = make_ops("cuda:0")
+    q, k, v = (torch.randn(75, 2, 32, device="cuda:0") for _ in range(3))
+    plan = ops.attention_plan([40, 35], causal=True)
+    want = [x.clone() for x in ops.attention(plan, q, k, v)]
+    big = torch.randn(8192, 8192, device="cuda:0")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            big = big @ big * 1e-4
+        got = ops.attention(plan, q, k, v)
+    at, size = plan.table.data_ptr(), plan.table.numel()
+    del plan
+    others = [torch.empty(size, dtype=torch.uint8, device="cuda:0") for _ in range(64)]
+    assert side.query() or all(x.data_ptr() != at for x in others)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
