@@ -140,3 +140,52 @@ def test_a_dropped_plan_stays_until_the_streams_that_use_it_are_done():
     assert side.query() or all(x.data_ptr() != at for x in others)
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES[:2], ids=str)
+@pytest.mark.parametrize("cap", [4.0])
+def test_a_row_depends_on_what_it_sees_alone(device, dtype, cap):
+    """To the last bit: a later frame's key and value, made large and not, reach no earlier row, and a row's query no other row --
+    forward, backward and step."""
+    ops = make_ops(device)
+    g = torch.Generator().manual_seed(4)
+    n, d = 62, 16
+    t = [(torch.randn(n, 2, d, generator=g) * 0.5).to(dtype).to(device) for _ in range(4)]
+    plan = ops.attention_plan([n], causal=True)
+
+    def run(q, k, v, do):
+        o, lse = ops.attention(plan, q, k, v, cap=cap)
+        return (o, lse) + ops.attention_backward(plan, do, q, k, v, o, lse, cap=cap)
+
+    want = run(*t)
+    last = n - 1
+    for which, factor in ((0, 60.0), (1, 60.0), (2, 30.0), (0, 9.0), (1, 9.0)):
+        x = [y.clone() for y in t]
+        x[which][last] *= factor
+        got = run(*x)
+        assert torch.equal(got[0][:last], want[0][:last]) and torch.equal(got[1][:last], want[1][:last])
+        assert torch.equal(got[2][:last], want[2][:last])  # dq
+
+    def step(q, k, v):
+        kc, vc = (torch.zeros(5, 16, 2, d, dtype=dtype, device=device) for _ in range(2))
+        kc.view(80, 2, d)[:50], vc.view(80, 2, d)[:50] = t[1][:50], t[2][:50]
+        return ops.attention_step(q, k, v, kc, vc, torch.arange(5, dtype=torch.int32, device=device)[None],
+                                  torch.tensor([50], dtype=torch.int32, device=device), cap=cap)
+
+    new = [x[None, 50:] for x in t[:3]]
+    want = step(*new)
+    for which in (0, 1, 2):
+        x = [y.clone() for y in new]
+        x[which][:, -1] *= 60.0
+        assert torch.equal(step(*x)[:, :-1], want[:, :-1])
+
+
+def test_cap_polynomial():
+    """The odd polynomial that stands for tanh below 0.6, with its coefficients as stored: relative error below 1.5e-8."""
+    x = np.linspace(1e-6, 0.6, 200001)
+    y = x * x
+    c = [float(np.float32(f)) for f in (-0.006276387721300125, 0.021116213873028755, -0.053875137120485306, 0.13332924246788025,
+                                        -0.3333333134651184)]
+    p = x * (1.0 + y * (c[4] + y * (c[3] + y * (c[2] + y * (c[1] + y * c[0])))))
+    assert np.abs(p / np.tanh(x) - 1.0).max() < 1.5e-8
