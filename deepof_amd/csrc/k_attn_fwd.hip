@@ -141,9 +141,10 @@ __global__ void __launch_bounds__(64 * NW, DP <= 32 ? (NW == 1 && sizeof(T) == 4
       // The running maximum follows only when a tile's exceeds it by 2^kLag: until then the weights stay below that, which costs the
       // fp32 sums nothing, and the accumulators need no rescaling pass.
       if (dof_wave_any(mt > m + DofSoftmax<T>::kLag)) {
-        const float mn = fmaxf(m, mt);
-        const float a = mn == -INFINITY ? 1.0f : dof_exp2(m - mn);
-        m = mn;
+        // only of the rows that exceed theirs: a row's bits do not depend on the other rows of its wavefront
+        const bool up = mt > m + DofSoftmax<T>::kLag;
+        const float a = up ? dof_exp2(m - mt) : 1.0f;
+        m = up ? mt : m;
         l *= a;
 #pragma unroll
         for (int d = 0; d < DT; ++d)

@@ -338,10 +338,10 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) k_attn
         for (int e = 0; e < 4; ++e) mt = fmaxf(mt, x[i][u][e]);
       mt = fmaxf(mt, __shfl_xor(mt, 16));
       mt = fmaxf(mt, dof_swap32(mt));
-      if (dof_wave_any(mt > m[i] + DofSoftmax<T>::kLag)) {  // as in the forward pass: the maximum follows in steps
-        const float mn = fmaxf(m[i], mt);
-        const float a = mn == -INFINITY ? 1.0f : dof_exp2(m[i] - mn);
-        m[i] = mn;
+      if (dof_wave_any(mt > m[i] + DofSoftmax<T>::kLag)) {  // as in the forward pass: the maximum follows in steps, row by row
+        const bool up = mt > m[i] + DofSoftmax<T>::kLag;
+        const float a = up ? dof_exp2(m[i] - mt) : 1.0f;
+        m[i] = up ? mt : m[i];
         l[i] *= a;
 #pragma unroll
         for (int d = 0; d < DT; ++d)

@@ -143,8 +143,8 @@ def test_a_dropped_plan_stays_until_the_streams_that_use_it_are_done():
 
 
 @pytest.mark.parametrize("device", DEVICES)
-@pytest.mark.parametrize("dtype", DTYPES[:2], ids=str)
-@pytest.mark.parametrize("cap", [4.0])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("cap", [0.0, 4.0])
 def test_a_row_depends_on_what_it_sees_alone(device, dtype, cap):
     """To the last bit: a later frame's key and value, made large and not, reach no earlier row, and a row's query no other row --
     forward, backward and step."""
