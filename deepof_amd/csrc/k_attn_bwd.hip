@@ -126,11 +126,14 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_
   delta += dof_swap32(delta);
   const int64_t srow = (t.q0 + row) * A.q_heads + h;
   float sum = 0.0f;  // of P dP: delta again, without the rounding of o
+  DofLongNumber<T> pdp;
   const Lse lse = lse_of<T>(live ? A.lse[srow] : -INFINITY);
   const T* kp = static_cast<const T*>(A.k) + t.k0 * A.ks[0] + hk * A.ks[1];
   const T* vp = static_cast<const T*>(A.v) + t.k0 * A.vs[0] + hk * A.vs[1];
 
   dof_f32x16 dq[DT];
+  DofLongSum<T, dof_f32x16, DT> ldq;
+  ldq.clear();
   Stage rk, rv;
   // Rows of few keys: delta from the rounded o is off by as much as rounding all of dq once more; they go through their keys twice, the
   // first time for the sum of P dP alone.
@@ -143,7 +146,7 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_
       rk.store(sk[0], tid);
       rv.store(sv[0], tid);
     }
-    sum = 0.0f;
+    pdp = DofLongNumber<T>();
     for (int j0 = 0, buf = 0; j0 < kmax; j0 += kKeys, buf ^= 1) {
       __syncthreads();
       const int next = j0 + kKeys;
@@ -162,14 +165,16 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_
         float ds[16], w[16], c[16];
         const float base = (float)(pos - j0 - 4 * half);
         const int left = kend - j0 - 4 * half;
+        float part = 0.0f;
         if constexpr (KIND > 0) scores<T, KIND>(x, sc, A.slopes != nullptr, [&](int v) { return base - (float)(8 * (v / 4) + v % 4); }, w, c);
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
           const bool hidden = partial && 8 * (v / 4) + v % 4 >= left;  // not 0 x (what a hidden key holds)
           const float p = weight<T, KIND>(x[v], sc.mul, w[v], lse.value, lse.rest);
           ds[v] = hidden ? 0.0f : p * (KIND == 0 ? Lift<T>::ds / Lift<T>::p : c[v]) * (y[v] - delta);
-          sum += hidden ? 0.0f : p * y[v];
+          part += hidden ? 0.0f : p * y[v];
         }
+        pdp.add(part);
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           const DofFrag<T> f = dof_frag_pack<T>(ds + 8 * s), rest = dof_frag_rest<T>(ds + 8 * s, f);
@@ -181,18 +186,21 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_
             if constexpr (sizeof(T) == 2) dq[d] = dof_mma32<T>(k, rest, dq[d]);
           }
         }
+        ldq.count(dq, kKeys);
       }
       if (next < kmax) {
         rk.store(sk[buf ^ 1], tid);
         rv.store(sv[buf ^ 1], tid);
       }
     }
+    sum = pdp.total();
     sum = (sum + dof_swap32(sum)) / Lift<T>::p;
     if (pass == 0) {
       delta = sum;
       __syncthreads();  // the second pass fills the images anew
     }
   }
+  ldq.finish(dq);
   if (!live) return;
   if (half == 0) B.delta[srow] = sum;
   const float out = B.scale / Lift<T>::ds;
@@ -401,6 +409,10 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_
     }
   }
   dof_f32x16 dk[DK ? DT : 1], dv[DV ? DT : 1];
+  DofLongSum<T, dof_f32x16, DK ? DT : 1> ldk;
+  DofLongSum<T, dof_f32x16, DV ? DT : 1> ldv;
+  if constexpr (DK) ldk.clear();
+  if constexpr (DV) ldv.clear();
 #pragma unroll
   for (int d = 0; d < DT; ++d) {
     if constexpr (DK) dk[d] = dof_zero16();
@@ -491,11 +503,15 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_
           }
         }
       }
+      if constexpr (DK) ldk.count(dk, kRows);
+      if constexpr (DV) ldv.count(dv, kRows);
     }
     if (next_h < h_lo + heads) store(buf ^ 1);
     h = next_h;
     i0 = next_i;
   }
+  if constexpr (DK) ldk.finish(dk);
+  if constexpr (DV) ldv.finish(dv);
   if (!live) return;
   const float ok = B.scale / Lift<T>::ds, ov = 1.0f / Lift<T>::p;
   auto write = [&](const dof_f32x16* acc, float f, void* out, const int64_t* st, float* part) {

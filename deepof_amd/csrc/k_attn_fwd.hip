@@ -63,7 +63,10 @@ __global__ void __launch_bounds__(64 * NW, DP <= 32 ? (NW == 1 && sizeof(T) == 4
   dof_f32x16 o[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) o[d] = dof_zero16();
-  float m = -INFINITY, l = 0.0f;
+  DofLongSum<T, dof_f32x16, DT> lo;
+  lo.clear();
+  DofLongNumber<T> l;
+  float m = -INFINITY;
 
   // In a step that some rows see only in part a hidden key's weight is zero, but zero times an infinity or NaN in V is not: such
   // values are left out of the products there (rare, and looked for in these steps only) and put where they are seen at the end.
@@ -145,7 +148,8 @@ __global__ void __launch_bounds__(64 * NW, DP <= 32 ? (NW == 1 && sizeof(T) == 4
         const bool up = mt > m + DofSoftmax<T>::kLag;
         const float a = up ? dof_exp2(m - mt) : 1.0f;
         m = up ? mt : m;
-        l *= a;
+        l.scale(a);
+        lo.scale(a);
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -155,13 +159,13 @@ __global__ void __launch_bounds__(64 * NW, DP <= 32 ? (NW == 1 && sizeof(T) == 4
 #pragma unroll
       for (int u = 0; u < KU; ++u) {
         float p[16];
-        float part = 0.0f;  // a chain of one addition per step, not sixteen, for the long sum
+        float part = 0.0f;  // one addition per step, not sixteen, to the long sum
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
           p[v] = dof_exp2(fmaf(x[u][v], unit, -mm));
           part += p[v];
         }
-        l += part;
+        l.add(part);
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           const DofFrag<T> pf = dof_frag_pack<T>(p + 8 * s);
@@ -170,6 +174,7 @@ __global__ void __launch_bounds__(64 * NW, DP <= 32 ? (NW == 1 && sizeof(T) == 4
           for (int d = 0; d < DT; ++d) o[d] = dof_mma32<T>(sv[buf].colfrag(r, r + 8, 32 * d + col), pf, o[d]);
         }
       }
+      lo.count(o, kKeys);
     }
     if (next < kmax) {
       if (BUF == 1) __syncthreads();
@@ -178,7 +183,9 @@ __global__ void __launch_bounds__(64 * NW, DP <= 32 ? (NW == 1 && sizeof(T) == 4
     }
   }
 
-  l += dof_swap32(l);
+  lo.finish(o);
+  float sum = l.total();
+  sum += dof_swap32(sum);
   __syncthreads();
   if (!live) return;
   if (found) {
@@ -192,7 +199,7 @@ __global__ void __launch_bounds__(64 * NW, DP <= 32 ? (NW == 1 && sizeof(T) == 4
           if (!(fabsf(x) < INFINITY)) o[d][v] += x;
         }
   }
-  const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // no visible key: zeros; NaN stays NaN
+  const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);  // no visible key: zeros; NaN stays NaN
   T* op = static_cast<T*>(A.o) + (t.q0 + row) * A.os[0] + h * A.os[1];
 #pragma unroll
   for (int d = 0; d < DT; ++d)
@@ -204,7 +211,7 @@ __global__ void __launch_bounds__(64 * NW, DP <= 32 ? (NW == 1 && sizeof(T) == 4
         dof_store_vec<T, 4>(op + e, r);
       }
     }
-  if (half == 0) A.lse[(t.q0 + row) * A.q_heads + h] = l == 0.0f ? -INFINITY : (m - DofSoftmax<T>::kUp + dof_log2(l)) * kLn2;
+  if (half == 0) A.lse[(t.q0 + row) * A.q_heads + h] = sum == 0.0f ? -INFINITY : (m - DofSoftmax<T>::kUp + dof_log2(sum)) * kLn2;
 }
 
 template <class T, int DP>

@@ -30,8 +30,9 @@ namespace {
 
 constexpr int kStepKeys = 32;   // frames per wavefront and round
 constexpr int kMinTiles = 16;   // rounds of a part at least: four per wavefront
+constexpr int kMaxTiles = 256;  // and at most: 64 rounds per wavefront, a chain of 512 additions of fp32 products
 constexpr int kWhole = 32;      // streams whose table holds no more rounds stay whole: a second kernel for the join costs more
-constexpr int kTarget = 1024;   // parts of a call in all: two rounds of two workgroups per CU
+constexpr int kTarget = 1024;   // parts of a call in all, unless kMaxTiles makes them more: two rounds of two workgroups per CU
 
 struct Step {
   DofAttnStep d;
@@ -93,7 +94,7 @@ __device__ __forceinline__ Part find_part(const Step& A, int unit) {
   }
   const int64_t share = (all * A.d.k_heads * A.row_blocks + kTarget - 1) / kTarget;
   Part p;
-  p.per = share > A.min_tiles ? (int)share : A.min_tiles;
+  p.per = share > kMaxTiles ? kMaxTiles : share > A.min_tiles ? (int)share : A.min_tiles;
   int before = 0;
   for (int b0 = 0; b0 < A.d.streams; b0 += 256) {
     if (b0 > 0) __syncthreads();
@@ -508,7 +509,7 @@ int check(const DofAttnStep* d, const char* who) {
 }
 
 // Row tiles of 16 per workgroup (1 or 2), blocks of them, and the most parts that find_part can make of the streams: each at most
-// one more than its share, and no more than its table holds.
+// one more than its share (of kTarget, or of kMaxTiles each), and no more than its table holds.
 struct Shape { int rows, rt, row_blocks, min_tiles; int64_t parts; };
 Shape shape_of(const DofAttnStep* d) {
   Shape s;
@@ -517,7 +518,8 @@ Shape shape_of(const DofAttnStep* d) {
   s.row_blocks = (s.rows + 16 * s.rt - 1) / (16 * s.rt);
   const int64_t tiles = ((int64_t)d->max_pages * d->page_size + kStepKeys - 1) / kStepKeys;
   s.min_tiles = tiles <= kWhole ? kWhole : kMinTiles;
-  s.parts = d->streams + kTarget / ((int64_t)d->k_heads * s.row_blocks);
+  const int64_t target = kTarget / ((int64_t)d->k_heads * s.row_blocks), longest = d->streams * tiles / kMaxTiles;
+  s.parts = d->streams + (target > longest ? target : longest);
   const int64_t most = (tiles + s.min_tiles - 1) / s.min_tiles * d->streams;
   if (s.parts > most) s.parts = most;
   return s;

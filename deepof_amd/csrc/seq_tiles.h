@@ -123,6 +123,81 @@ __device__ __forceinline__ dof_f32x4 dof_zero4() {
   return z;
 }
 
+// sum += x with what the addition rounded off collected in `rest` (Knuth's two-sum); an infinite sum stays one
+__device__ __forceinline__ void dof_add_rest(float& sum, float& rest, float x) {
+  const float s = sum + x, b = s - sum, lost = (sum - (s - b)) + (x - b);
+  sum = s;
+  rest += fabsf(s) < INFINITY ? lost : 0.0f;
+}
+
+// Accumulators of N registers of V for long sums.  A chain of products rounds once per instruction, and where the terms have one sign
+// those errors add up: fp32 elements, 65536 equal weights and values, 6e-4 of the result.  There the chain is cut every kTerms
+// terms (kTerms / 2 additions of a 32x32x2 product) and added to a sum of such blocks: n terms are off by at most
+// (kTerms / 2 + n / kTerms) 2^-24 of the sum of their sizes.  (Keeping the blocks' own rounding errors besides would make that
+// independent of n, but its registers cost the kernels for heads of 16 to 64 a wavefront per SIMD.)  16-bit elements have 16 or 32 terms per
+// addition and results of 8 or 11 bits: n / 16 additions stay below half a step of bf16 to n = 2^19 terms of one sign, of fp16 to 2^17;
+// nothing is kept for them.
+template <class T, class V, int N> struct DofLongSum {
+  static constexpr bool kOn = sizeof(T) == 4;
+  static constexpr int kTerms = 256, kLanes = (int)(sizeof(V) / 4);
+  V sum[kOn ? N : 1];
+  int n;
+  __device__ __forceinline__ void clear() {
+    if constexpr (kOn) {
+      n = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int v = 0; v < kLanes; ++v) sum[i][v] = 0.0f;
+    }
+  }
+  __device__ __forceinline__ void scale(float a) {
+    if constexpr (kOn) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int v = 0; v < kLanes; ++v) sum[i][v] *= a;
+    }
+  }
+  // `terms` more are in the chain
+  __device__ __forceinline__ void count(V* chain, int terms) {
+    if constexpr (kOn) {
+      n += terms;
+      if (n < kTerms) return;
+      n = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int v = 0; v < kLanes; ++v) {
+          sum[i][v] += chain[i][v];
+          chain[i][v] = 0.0f;
+        }
+    }
+  }
+  // the whole sum, into the chain's registers
+  __device__ __forceinline__ void finish(V* chain) {
+    if constexpr (kOn) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int v = 0; v < kLanes; ++v) chain[i][v] += sum[i][v];
+    }
+  }
+};
+// one number that grows once per step; fp32 elements: with its own rounding errors
+template <class T> struct DofLongNumber {
+  float sum = 0.0f, rest = 0.0f;
+  __device__ __forceinline__ void add(float x) {
+    if constexpr (sizeof(T) == 4) dof_add_rest(sum, rest, x);
+    else sum += x;
+  }
+  __device__ __forceinline__ void scale(float a) {
+    sum *= a;
+    if constexpr (sizeof(T) == 4) rest *= a;
+  }
+  __device__ __forceinline__ float total() const { return sizeof(T) == 4 ? sum + rest : sum; }
+};
+
 // An LDS image of ROWS rows x DP elements, read both ways: eight consecutive elements of a row (rowfrag, the operand whose k runs
 // along the row) and eight rows of one column (colfrag, the operand whose k runs down the rows).
 //

@@ -189,3 +189,68 @@ def test_cap_polynomial():
                                         -0.3333333134651184)]
     p = x * (1.0 + y * (c[4] + y * (c[3] + y * (c[2] + y * (c[1] + y * c[0])))))
     assert np.abs(p / np.tanh(x) - 1.0).max() < 1.5e-8
+
+
+def equal_terms(n, d=8, heads=1):
+    """Equal weights and values whose products and sums fp32 cannot hold: every rounding has the same sign over long stretches."""
+    gen = torch.Generator().manual_seed(12)
+    return 0.1 + 0.01 * torch.rand(1, heads, d, generator=gen).expand(n, heads, d)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("n,d", [(4096, 8), (16384, 16), (3001, 72)])
+def test_long_float32_sums_of_one_sign(device, n, d):
+    """o, dq and the sum behind it over n keys; dk and dv over n rows."""
+    ops = make_ops(device)
+    # a chain of at most 128 additions (256 where they take one term each, as in the emulation), n / 256 of those in a second one, and
+    # 64 for weights, scores and the division, all of one sign
+    rel = (256 + n / 256 + 64) * U32
+    q, k, v = torch.zeros(1, 1, d), torch.zeros(n, 1, d), equal_terms(n, d).contiguous()
+    plan = ops.attention_plan([1], [n])
+    o, lse = ops.attention(plan, q.to(device), k.to(device), v.to(device))
+    assert float((o.cpu().double() / v[:1].double() - 1).abs().max()) <= rel
+    assert abs(float(lse) - math.log(n)) <= 4 * U32 * math.log(n)
+    # keys whose first half carries values 1 + v and the second v: dP differs by one between the halves, dS = +- 1 / (4 n) as the
+    # weights are equal; k = +- (0.1 ..) makes every term of dq positive
+    v2 = torch.zeros_like(v)
+    half = n // 2
+    v2[:half, :, 0] = 1.0
+    kk = equal_terms(n, d).contiguous()
+    kk[half:] *= -1.0
+    g = torch.zeros(1, 1, d)
+    g[..., 0] = 1.0
+    f = half / n  # dS of the first half: (1 - f) / n, of the second: - f / n
+    o2, lse2 = ops.attention(plan, q.to(device), kk.to(device), v2.to(device))
+    dq = ops.attention_backward(plan, g.to(device), q.to(device), kk.to(device), v2.to(device), o2, lse2)[0]
+    want = (f * (1 - f) + (1 - f) * f) * kk[:1].double() * d ** -0.5
+    # dS itself: 1 - delta, delta good to rel, so relative 2 rel; the weights to 64 roundings
+    assert float((dq.cpu().double() / want - 1).abs().max()) <= 4 * rel
+    # n rows over two keys: dv = sum of g / 2, dk = sum of dS q scale with dS = +- (g . (v0 - v1)) / 4
+    q3, g3 = equal_terms(n, d).contiguous(), equal_terms(n, d).contiguous()
+    k3, v3 = torch.zeros(2, 1, d), torch.zeros(2, 1, d)
+    v3[0, 0, 0] = 1.0
+    plan = ops.attention_plan([n], [2])
+    args = [x.to(device) for x in (q3, k3, v3)]
+    o3, lse3 = ops.attention(plan, *args)
+    dq3, dk3, dv3 = ops.attention_backward(plan, g3.to(device), *args, o3, lse3)
+    want = g3[:1].double() * n / 2
+    assert float((dv3.cpu().double() / want - 1).abs().max()) <= rel
+    want = g3[0, 0, 0].double() / 4 * n * q3[:1].double() * d ** -0.5
+    for at, sign in ((0, 1), (1, -1)):
+        assert float((dk3[at].cpu().double() * sign / want - 1).abs().max()) <= 4 * rel
+
+
+@pytest.mark.gpu
+def test_step_over_millions_of_frames():
+    """16 million frames that lie on two pages, listed over and over; equal weights, values of one sign."""
+    ops = make_ops("cuda:0")
+    page, n, hk, d = 1024, 16384 * 1024, 8, 8
+    kc = torch.zeros(2, page, hk, d, device="cuda:0")
+    vc = equal_terms(2 * page, d, hk).reshape(2, page, hk, d).contiguous().cuda()
+    table = torch.zeros(1, n // page + 1, dtype=torch.int32, device="cuda:0")
+    table[0, -1] = 1
+    q = torch.zeros(1, 1, hk, d, device="cuda:0")
+    o = ops.attention_step(q, torch.zeros_like(q), vc[:1, :1].clone(), kc, vc, table, torch.tensor([n], dtype=torch.int32, device="cuda:0"))
+    # a chain of 512 additions in a wavefront, four wavefronts, at most n / 8192 parts in a chain of their own, 64 for the weights
+    rel = (512 + 4 + n / 8192 / 8 + 64) * U32
+    assert float((o.cpu().double() / vc[0, :1].cpu().double() - 1).abs().max()) <= rel
