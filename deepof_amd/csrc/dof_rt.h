@@ -166,6 +166,16 @@ __device__ __forceinline__ void dof_sincos_turns(double turns, float* s, float* 
 }
 #endif
 
+// a value the compiler takes for another one: work on it is not shared with other branches (and its registers not held for them)
+#ifdef DOF_EMU
+__device__ __forceinline__ float dof_opaque(float v) { return v; }
+#else
+__device__ __forceinline__ float dof_opaque(float v) {
+  asm("" : "+v"(v));
+  return v;
+}
+#endif
+
 // 1: the HIP runtime is underneath (RCCL can be opened); 0: the host-only emulation build
 #ifdef DOF_EMU
 #define DOF_HAS_DEVICE_RUNTIME 0

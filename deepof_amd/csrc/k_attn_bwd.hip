@@ -61,7 +61,7 @@ __device__ __forceinline__ void scores(const dof_f32x16& x, const DofScore& sc, 
     c[v] = Lift<T>::ds / Lift<T>::p;
   }
   if constexpr (KIND == 2) {
-    dof_cap_tanh<T, 16>(w, sc.mul);
+    dof_cap_tanh<16>(w, sc.mul);
 #pragma unroll
     for (int v = 0; v < 16; ++v) {
       c[v] *= fmaf(-w[v], w[v], 1.0f);

@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(64 * NW, DP <= 32 ? (NW == 1 && sizeof(T) == 4
             float th[16];
 #pragma unroll
             for (int v = 0; v < 16; ++v) th[v] = x[u][v];
-            dof_cap_tanh<T, 16>(th, sc.mul);
+            dof_cap_tanh<16>(th, sc.mul);
 #pragma unroll
             for (int v = 0; v < 16; ++v) x[u][v] = sc.cap_l2 * th[v];
           }

@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) k_attn
         float th[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) th[k] = x[i][k / 4][k % 4];
-        dof_cap_tanh<T, 8>(th, A.score.mul);
+        dof_cap_tanh<8>(th, A.score.mul);
 #pragma unroll
         for (int k = 0; k < 8; ++k) x[i][k / 4][k % 4] = A.score.cap_l2 * th[k];
       } else {

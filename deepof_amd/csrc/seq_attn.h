@@ -42,31 +42,34 @@ template <> struct DofSoftmax<DofF16> {
 };
 
 // t[i] = tanh(t[i] mul) of N scores of a lane.  Below 0.6 of the cap, where capped scores mostly lie, an odd polynomial (fitted to
-// tanh(x) / x on [0, 0.6], relative error 1.5e-8) takes 8 instructions, none of them transcendental; from there on the library's
-// tanh (fp32) or 1 - 2 / (1 + 2^(2 log2(e) x)), absolute error 2^-22.  Which of them a score takes depends on it alone: what other
+// tanh(x) / x on [0, 0.6], relative error 1.5e-8) takes 8 instructions, none of them transcendental; from there on
+// 1 - 2 / (1 + 2^(2 log2(e) x)), whose quotient is below 0.47: off by 3 roundings of that and one of the result.  Which of them a score takes depends on it alone: what other
 // rows and hidden keys hold only decides whether the wavefront computes the second at all.
-template <class T, int N> __device__ __forceinline__ void dof_cap_tanh(float* t, float mul) {
+__device__ __forceinline__ float dof_tanh_near(float x) {
+  const float y = x * x;
+  float c = fmaf(y, -0.006276387721300125f, 0.021116213873028755f);
+  c = fmaf(y, c, -0.053875137120485306f);
+  c = fmaf(y, c, 0.13332924246788025f);
+  c = fmaf(y, c, -0.3333333134651184f);
+  return fmaf(x * y, c, x);
+}
+template <int N> __device__ __forceinline__ void dof_cap_tanh(float* t, float mul) {
   float top = 0.0f;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     t[i] *= mul;
     top = fmaxf(top, fabsf(t[i]));
   }
-  const bool far = dof_wave_any(!(top < 0.6f));
+  if (dof_wave_any(!(top < 0.6f))) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float x = t[i], y = x * x;
-    float c = fmaf(y, -0.006276387721300125f, 0.021116213873028755f);
-    c = fmaf(y, c, -0.053875137120485306f);
-    c = fmaf(y, c, 0.13332924246788025f);
-    c = fmaf(y, c, -0.3333333134651184f);
-    t[i] = fmaf(x * y, c, x);
-    if (far) {
-      float f;
-      if constexpr (sizeof(T) == 4) f = tanhf(x);
-      else f = fmaf(-2.0f, dof_rcp(1.0f + dof_exp2(x * (2.0f * kLog2e))), 1.0f);
-      t[i] = fabsf(x) < 0.6f ? t[i] : f;
+    for (int i = 0; i < N; ++i) {
+      const float x = dof_opaque(t[i]);  // the squares of both branches, computed before them, took 16 registers
+      const float far = fmaf(-2.0f, dof_rcp(1.0f + dof_exp2(x * (2.0f * kLog2e))), 1.0f);
+      t[i] = fabsf(x) < 0.6f ? dof_tanh_near(x) : far;
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) t[i] = dof_tanh_near(t[i]);
   }
 }
 
