@@ -84,7 +84,7 @@ class NormRope(C.Structure):
 
 
 class AttnPlan(C.Structure):
-    _fields_ = [("n_docs", C.c_int32), ("causal", C.c_int32), ("small", C.c_int32), ("reserved", C.c_int32),
+    _fields_ = [("n_docs", C.c_int32), ("causal", C.c_int32), ("small", C.c_int32), ("longest", C.c_int32),
                 ("q_rows", C.c_int64), ("k_rows", C.c_int64), ("n_tiles", C.c_int64 * 4),
                 ("first", C.c_int64 * 4), ("table_bytes", C.c_int64)]
 

@@ -169,6 +169,7 @@ DofAttnFwd forward_args(const DofAttention* d, const void* q, const void* k, con
 
 int set_tiles(DofAttnFwd* A, const DofAttnPlan* p, const void* table, int which, int flat) {
   A->causal = p->causal;
+  A->longest = p->longest;
   A->n_tiles = (int32_t)p->n_tiles[which + flat];
   A->tiles = list_at(p, table, which + flat);
   return A->n_tiles;
@@ -182,9 +183,10 @@ extern "C" int dof_attn_plan_size(int32_t n_docs, const int64_t* q_off, const in
   plan->n_docs = n_docs;
   plan->causal = causal != 0;
   plan->small = 1;
-  plan->reserved = 0;
+  plan->longest = 0;
   for (int32_t i = 0; i < n_docs; ++i) {
     const int64_t lq = q_off[i + 1] - q_off[i], lk = k_off[i + 1] - k_off[i];
+    plan->longest = (int32_t)std::max<int64_t>(plan->longest, std::max(lq, lk));
     if (lq > kAttnFlat || lk > kAttnFlat || (lq > 0 && lk == 0)) plan->small = 0;
   }
   plan->q_rows = n_docs ? q_off[n_docs] : 0;

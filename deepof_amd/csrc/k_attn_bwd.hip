@@ -77,8 +77,8 @@ __device__ __forceinline__ void scores(const dof_f32x16& x, const DofScore& sc, 
   }
 }
 
-// KIND: the score function (dof_attn_kind)
-template <class T, int DP, int NW, int KIND>
+// KIND: the score function (dof_attn_kind).  LONG: long sums are made of blocks (fp32; always in tall tiles)
+template <class T, int DP, int NW, int KIND, bool LONG>
 __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_attn_dq(DofAttnBwd B) {
   const DofAttnFwd& A = B.f;
   constexpr int kKeys = 32;  // per step: what leaves room for two wavefronts per SIMD
@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_
   const T* vp = static_cast<const T*>(A.v) + t.k0 * A.vs[0] + hk * A.vs[1];
 
   dof_f32x16 dq[DT];
-  DofLongSum<T, dof_f32x16, DT> ldq;
+  DofLongSum<T, dof_f32x16, DT, LONG> ldq;
   ldq.clear();
   Stage rk, rv;
   // Rows of few keys: delta from the rounded o is off by as much as rounding all of dq once more; they go through their keys twice, the
@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(64, DP <= 32 ? 2 : 1) k_attn_bwd_one(DofAttnBw
 // registers only one wavefront fits a SIMD, and one alone does not hide its own latencies (16384 causal frames, 16 / 4
 // heads of 128, before dS took its second product: 6.4 ms in one pass of 4 products, 3.3 in two of 5; with it, 2 + 4: 3.65 ms).
 // A workgroup takes `heads_per` query heads of the group; several workgroups of one key tile leave fp32 parts for k_attn_join.
-template <class T, int DP, int NW, int KIND, int WANT>
+template <class T, int DP, int NW, int KIND, bool LONG, int WANT>
 __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_attn_dkv(DofAttnBwd B) {
   const DofAttnFwd& A = B.f;
   constexpr bool DV = (WANT & 1) != 0, DK = (WANT & 2) != 0;
@@ -409,8 +409,8 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_
     }
   }
   dof_f32x16 dk[DK ? DT : 1], dv[DV ? DT : 1];
-  DofLongSum<T, dof_f32x16, DK ? DT : 1> ldk;
-  DofLongSum<T, dof_f32x16, DV ? DT : 1> ldv;
+  DofLongSum<T, dof_f32x16, DK ? DT : 1, LONG> ldk;
+  DofLongSum<T, dof_f32x16, DV ? DT : 1, LONG> ldv;
   if constexpr (DK) ldk.clear();
   if constexpr (DV) ldv.clear();
 #pragma unroll
@@ -560,16 +560,18 @@ template <class T, int DP>
 void launch_dq(const DofAttnBwd& B, int flat, hipStream_t stream) {
   const unsigned blocks = (unsigned)((int64_t)B.f.n_tiles * B.f.q_heads);
   DOF_ATTN_KIND(B.f, KIND, {
-    if (flat) DOF_LAUNCH((k_attn_dq<T, DP, 1, KIND>), (blocks, 1, 1), (64, 1, 1), stream, B);
-    else DOF_LAUNCH((k_attn_dq<T, DP, 4, KIND>), (blocks, 1, 1), (256, 1, 1), stream, B);
+    if (flat) DOF_ATTN_LONG(T, B.f.longest, LONG, DOF_LAUNCH((k_attn_dq<T, DP, 1, KIND, LONG>), (blocks, 1, 1), (64, 1, 1), stream, B));
+    else DOF_LAUNCH((k_attn_dq<T, DP, 4, KIND, sizeof(T) == 4>), (blocks, 1, 1), (256, 1, 1), stream, B);
   });
 }
 template <class T, int DP, int WANT>
 void launch_dkv_want(const DofAttnBwd& B, int flat, hipStream_t stream) {
   const unsigned blocks = (unsigned)((int64_t)B.f.n_tiles * B.f.k_heads * B.splits);
   DOF_ATTN_KIND(B.f, KIND, {
-    if (flat) DOF_LAUNCH((k_attn_dkv<T, DP, 1, KIND, WANT>), (blocks, 1, 1), (64, 1, 1), stream, B);
-    else DOF_LAUNCH((k_attn_dkv<T, DP, 4, KIND, WANT>), (blocks, 1, 1), (256, 1, 1), stream, B);
+    if (flat)
+      DOF_ATTN_LONG(T, (int64_t)B.f.longest * B.heads_per, LONG,
+                    DOF_LAUNCH((k_attn_dkv<T, DP, 1, KIND, LONG, WANT>), (blocks, 1, 1), (64, 1, 1), stream, B));
+    else DOF_LAUNCH((k_attn_dkv<T, DP, 4, KIND, sizeof(T) == 4, WANT>), (blocks, 1, 1), (256, 1, 1), stream, B);
   });
 }
 template <class T, int DP>

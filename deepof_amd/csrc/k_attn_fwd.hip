@@ -23,8 +23,8 @@ namespace {
 // Keys per step: 32, or 64 for heads over 64 (24 ragged recordings, heads of 64: 236 us with 64, 199 with 32, which leave room for four
 // wavefronts per SIMD; 16384 frames, heads of 128: 1.40 ms with 64, 1.48 with 32: two wavefronts either way).  A single wavefront takes
 // 32 and one LDS image: nobody else waits for it, and the smaller image lets more of them onto a CU.
-// KIND: the score function (dof_attn_kind)
-template <class T, int DP, int NW, int KIND>
+// KIND: the score function (dof_attn_kind).  LONG: long sums are made of blocks (fp32; always in tall tiles)
+template <class T, int DP, int NW, int KIND, bool LONG>
 __global__ void __launch_bounds__(64 * NW, DP <= 32 ? (NW == 1 && sizeof(T) == 4 ? 3 : 4) : sizeof(T) == 4 && DP > 64 ? 1 : 2) k_attn_fwd(DofAttnFwd A) {
   constexpr int KU = NW == 1 || DP <= 64 ? 1 : 2, kKeys = 32 * KU, BUF = NW == 1 ? 1 : 2;
   constexpr int KS = DP / 16, DT = (DP + 31) / 32;  // DP = 16: half of the only 32-wide tile of d is padding
@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(64 * NW, DP <= 32 ? (NW == 1 && sizeof(T) == 4
   dof_f32x16 o[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) o[d] = dof_zero16();
-  DofLongSum<T, dof_f32x16, DT> lo;
+  DofLongSum<T, dof_f32x16, DT, LONG> lo;
   lo.clear();
   DofLongNumber<T> l;
   float m = -INFINITY;
@@ -218,8 +218,8 @@ template <class T, int DP>
 void launch(const DofAttnFwd& A, int flat, hipStream_t stream) {
   const unsigned blocks = (unsigned)((int64_t)A.n_tiles * A.q_heads);
   DOF_ATTN_KIND(A, KIND, {
-    if (flat) DOF_LAUNCH((k_attn_fwd<T, DP, 1, KIND>), (blocks, 1, 1), (64, 1, 1), stream, A);
-    else DOF_LAUNCH((k_attn_fwd<T, DP, 4, KIND>), (blocks, 1, 1), (256, 1, 1), stream, A);
+    if (flat) DOF_ATTN_LONG(T, A.longest, LONG, DOF_LAUNCH((k_attn_fwd<T, DP, 1, KIND, LONG>), (blocks, 1, 1), (64, 1, 1), stream, A));
+    else DOF_LAUNCH((k_attn_fwd<T, DP, 4, KIND, sizeof(T) == 4>), (blocks, 1, 1), (256, 1, 1), stream, A);
   });
 }
 

@@ -5,6 +5,7 @@
 struct DofAttnFwd {
   const DofAttnTile* tiles;
   int32_t n_tiles, q_heads, k_heads, dim, causal;
+  int32_t longest;      // most rows or keys of a document
   DofScore score;
   const float* slopes;  // per query head, NULL: no bias
   const void *q, *k, *v;
@@ -40,6 +41,15 @@ static inline int dof_attn_kind(const DofAttnFwd& A) {
     if (_kind == 0) { constexpr int KIND = 0; __VA_ARGS__; }              \
     else if (_kind == 1) { constexpr int KIND = 1; __VA_ARGS__; }         \
     else { constexpr int KIND = 2; __VA_ARGS__; }                         \
+  } while (0)
+
+// DOF_ATTN_LONG(T, terms, LONG, expr): expr with LONG = whether sums of so many terms are made of blocks (fp32 elements)
+#define DOF_ATTN_LONG(T, terms, LONG, ...)                                                     \
+  do {                                                                                         \
+    if constexpr (sizeof(T) == 4) {                                                            \
+      if ((terms) > kLongTerms) { constexpr bool LONG = true; __VA_ARGS__; break; }            \
+    }                                                                                          \
+    { constexpr bool LONG = false; __VA_ARGS__; }                                              \
   } while (0)
 
 int dof_launch_attn_fwd(const DofAttnFwd& A, int dtype, int flat, hipStream_t stream);

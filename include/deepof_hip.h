@@ -522,7 +522,7 @@ int dof_norm_rope_backward(const DofNormRope* dims, const void* gq, const void* 
  * aligned) and passes both to the calls.  A plan serves any head count, head size and dtype. */
 typedef struct {
   int32_t n_docs, causal;
-  int32_t small, reserved; /* 1: no document has more than 32 rows or keys, or rows without any key */
+  int32_t small, longest;  /* small 1: no document has more than 32 rows or keys, or rows without any key; longest: most rows or keys */
   int64_t q_rows, k_rows;  /* the last offsets */
   int64_t n_tiles[4], first[4]; /* lists of tiles in the table (equal lists are kept once) */
   int64_t table_bytes;

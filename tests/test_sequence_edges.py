@@ -198,18 +198,18 @@ def equal_terms(n, d=8, heads=1):
 
 
 @pytest.mark.parametrize("device", DEVICES)
-@pytest.mark.parametrize("n,d", [(4096, 8), (16384, 16), (3001, 72)])
-def test_long_float32_sums_of_one_sign(device, n, d):
-    """o, dq and the sum behind it over n keys; dk and dv over n rows."""
+@pytest.mark.parametrize("n,d,few", [(4096, 8, 1), (16384, 16, 1), (3001, 72, 1), (1500, 40, 130)])
+def test_long_float32_sums_of_one_sign(device, n, d, few):
+    """o, dq and the sum behind it over n keys; dk and dv over n rows; few: rows (keys) on the other side, flat tiles or tall ones."""
     ops = make_ops(device)
     # a chain of at most 128 additions (256 where they take one term each, as in the emulation), n / 256 of those in a second one, and
     # 64 for weights, scores and the division, all of one sign
     rel = (256 + n / 256 + 64) * U32
-    q, k, v = torch.zeros(1, 1, d), torch.zeros(n, 1, d), equal_terms(n, d).contiguous()
-    plan = ops.attention_plan([1], [n])
+    q, k, v = torch.zeros(few, 1, d), torch.zeros(n, 1, d), equal_terms(n, d).contiguous()
+    plan = ops.attention_plan([few], [n])
     o, lse = ops.attention(plan, q.to(device), k.to(device), v.to(device))
     assert float((o.cpu().double() / v[:1].double() - 1).abs().max()) <= rel
-    assert abs(float(lse) - math.log(n)) <= 4 * U32 * math.log(n)
+    assert float((lse.cpu().double() - math.log(n)).abs().max()) <= 4 * U32 * math.log(n)
     # keys whose first half carries values 1 + v and the second v: dP differs by one between the halves, dS = +- 1 / (4 n) as the
     # weights are equal; k = +- (0.1 ..) makes every term of dq positive
     v2 = torch.zeros_like(v)
@@ -217,7 +217,7 @@ def test_long_float32_sums_of_one_sign(device, n, d):
     v2[:half, :, 0] = 1.0
     kk = equal_terms(n, d).contiguous()
     kk[half:] *= -1.0
-    g = torch.zeros(1, 1, d)
+    g = torch.zeros(few, 1, d)
     g[..., 0] = 1.0
     f = half / n  # dS of the first half: (1 - f) / n, of the second: - f / n
     o2, lse2 = ops.attention(plan, q.to(device), kk.to(device), v2.to(device))
@@ -225,18 +225,18 @@ def test_long_float32_sums_of_one_sign(device, n, d):
     want = (f * (1 - f) + (1 - f) * f) * kk[:1].double() * d ** -0.5
     # dS itself: 1 - delta, delta good to rel, so relative 2 rel; the weights to 64 roundings
     assert float((dq.cpu().double() / want - 1).abs().max()) <= 4 * rel
-    # n rows over two keys: dv = sum of g / 2, dk = sum of dS q scale with dS = +- (g . (v0 - v1)) / 4
+    # n rows over 2 few keys: dv = sum of g / (2 few), dk = sum of dS q scale with dS = +- g . (v0 - v1) / (4 few)
     q3, g3 = equal_terms(n, d).contiguous(), equal_terms(n, d).contiguous()
-    k3, v3 = torch.zeros(2, 1, d), torch.zeros(2, 1, d)
-    v3[0, 0, 0] = 1.0
-    plan = ops.attention_plan([n], [2])
+    k3, v3 = torch.zeros(2 * few, 1, d), torch.zeros(2 * few, 1, d)
+    v3[:few, 0, 0] = 1.0
+    plan = ops.attention_plan([n], [2 * few])
     args = [x.to(device) for x in (q3, k3, v3)]
     o3, lse3 = ops.attention(plan, *args)
     dq3, dk3, dv3 = ops.attention_backward(plan, g3.to(device), *args, o3, lse3)
-    want = g3[:1].double() * n / 2
+    want = g3[:1].double() * n / (2 * few)
     assert float((dv3.cpu().double() / want - 1).abs().max()) <= rel
-    want = g3[0, 0, 0].double() / 4 * n * q3[:1].double() * d ** -0.5
-    for at, sign in ((0, 1), (1, -1)):
+    want = g3[0, 0, 0].double() / (4 * few) * n * q3[:1].double() * d ** -0.5
+    for at, sign in ((slice(0, few), 1), (slice(few, None), -1)):
         assert float((dk3[at].cpu().double() * sign / want - 1).abs().max()) <= 4 * rel
 
 
