@@ -338,8 +338,8 @@ class AttentionOps:
 
     def attention_backward(self, plan, do, q, k, v, o, lse, scale: Optional[float] = None, cap: float = 0.0, slopes=None):
         """-> (dq, dk, dv) from the gradient at ``o`` and the forward's inputs and results; zeros in rows of no document.  The same
-        bits on every run.  ``slopes`` are constants: they get no gradient.  float16: the scores' gradients pass through float16, so
-        scale the loss as in any float16 training (they overflow at 65504 and lose precision below 1e-4)."""
+        bits on every run.  ``slopes`` are constants: they get no gradient.  float16: the scores' gradients are carried with a power
+        of two of their own, so that gradients of any size keep their precision; dq, dk and dv themselves are float16 numbers."""
         head, sl = self._attention_args(plan, q, k, v, scale, cap, slopes)
         for name, t in (("do", do), ("o", o)):
             _rows(name, t, self.device, q.dtype)

@@ -16,7 +16,8 @@
 // dq 1.75 -> 2.28 ms, dk 1.83 -> 2.22 ms.  The dq kernel starts from
 // delta = g.o, sums the unrounded P dP on its way and leaves that delta to the dk kernel.  Everything that is summed is fp32.
 // fp16 has 5 exponent bits: there P is carried as 2^12 P (an exact factor, taken out at the end), so that the weights of long
-// documents stay out of its subnormals.  dS is not lifted: gradients under a loss scale use the upper half of the range.
+// documents stay out of its subnormals, and dS with a power of two that follows its largest value (Range): gradients of any size
+// reach dq and dk as they would without the rounding.
 #include <cmath>
 
 #include "deepof_hip.h"
@@ -28,10 +29,46 @@
 namespace {
 
 template <class T> struct Lift {
-  static constexpr float p2 = 0.0f, p = 1.0f, ds = 1.0f;  // log2 of P's factor, P's factor, dS's factor
+  static constexpr float p2 = 0.0f, p = 1.0f;  // log2 of P's factor, P's factor
 };
 template <> struct Lift<DofF16> {
-  static constexpr float p2 = 12.0f, p = 4096.0f, ds = 1.0f;
+  static constexpr float p2 = 12.0f, p = 4096.0f;
+};
+
+// The power of two that dS takes into its fp16 products.  A lane holds values of one query row (dq) or one key (dk), and so does its half
+// of the accumulators: the factor is the lane's own (and that of the lane 32 away), found as a running maximum is.  The largest value
+// lies between 2^13 and 2^15 when it is set; what a value and its rest lose is at most 2^-25 then, 2^-38 of the largest.
+// Values arrive times P's factor.
+template <class T> struct Range {
+  static constexpr bool kOn = std::is_same<T, DofF16>::value;
+  float f = kOn ? 1.2676506e30f : 1.0f;  // 2^100
+  // mx 2^k in [2^13, 2^14), k at most 100
+  __device__ __forceinline__ static float fit(float mx) {
+    const int k = 267 - (int)(__builtin_bit_cast(uint32_t, mx) >> 23);
+    return __builtin_bit_cast(float, (uint32_t)(k < 227 ? k : 227) << 23);
+  }
+  __device__ __forceinline__ static float top(const float* ds) {
+    float mx = 0.0f;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) mx = fmaxf(mx, fabsf(ds[v]));
+    return fmaxf(mx, dof_swap32(mx));
+  }
+  template <int N> __device__ __forceinline__ void follow(float mx, dof_f32x16 (&acc)[N]) {
+    const bool up = mx * f > 32768.0f;
+    if (!dof_wave_any(up)) return;
+    const float to = up ? fit(mx) : f, a = to / f;
+    f = to;
+#pragma unroll
+    for (int d = 0; d < N; ++d)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[d][v] *= a;
+  }
+  __device__ __forceinline__ void apply(float* ds) const {
+    if constexpr (kOn) {
+#pragma unroll
+      for (int v = 0; v < 16; ++v) ds[v] *= f;
+    }
+  }
 };
 
 // A row's log-sum-exp in log 2, as the value and (fp32 elements) what its rounding left: there the weights are to be good to fp32, and
@@ -52,13 +89,13 @@ template <class T, int KIND> __device__ __forceinline__ float weight(float x, fl
 }
 
 // Sixteen raw products x of a lane -> the exponents' arguments w (log 2, before the log-sum-exp is taken off) and c, the factor of dS from
-// P (dP - delta): the derivative of the cap and the lift.  dist(v): the distance of element v.
+// P (dP - delta): the derivative of the cap.  dist(v): the distance of element v.
 template <class T, int KIND, class Dist>
 __device__ __forceinline__ void scores(const dof_f32x16& x, const DofScore& sc, bool bias, Dist dist, float* w, float* c) {
 #pragma unroll
   for (int v = 0; v < 16; ++v) {
     w[v] = x[v];
-    c[v] = Lift<T>::ds / Lift<T>::p;
+    c[v] = 1.0f;
   }
   if constexpr (KIND == 2) {
     dof_cap_tanh<16>(w, sc.mul);
@@ -133,6 +170,7 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_
 
   dof_f32x16 dq[DT];
   DofLongSum<T, dof_f32x16, DT, LONG> ldq;
+  Range<T> range;
   ldq.clear();
   Stage rk, rv;
   // Rows of few keys: delta from the rounded o is off by as much as rounding all of dq once more; they go through their keys twice, the
@@ -171,10 +209,14 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_
         for (int v = 0; v < 16; ++v) {
           const bool hidden = partial && 8 * (v / 4) + v % 4 >= left;  // not 0 x (what a hidden key holds)
           const float p = weight<T, KIND>(x[v], sc.mul, w[v], lse.value, lse.rest);
-          ds[v] = hidden ? 0.0f : p * (KIND == 0 ? Lift<T>::ds / Lift<T>::p : c[v]) * (y[v] - delta);
+          ds[v] = hidden ? 0.0f : p * (KIND == 0 ? 1.0f : c[v]) * (y[v] - delta);
           part += hidden ? 0.0f : p * y[v];
         }
         pdp.add(part);
+        if constexpr (Range<T>::kOn) {
+          range.follow(Range<T>::top(ds), dq);
+          range.apply(ds);
+        }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           const DofFrag<T> f = dof_frag_pack<T>(ds + 8 * s), rest = dof_frag_rest<T>(ds + 8 * s, f);
@@ -203,7 +245,7 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_
   ldq.finish(dq);
   if (!live) return;
   if (half == 0) B.delta[srow] = sum;
-  const float out = B.scale / Lift<T>::ds;
+  const float out = B.scale / Lift<T>::p / range.f;
   T* dqp = static_cast<T*>(B.dq) + (t.q0 + row) * B.dqs[0] + h * B.dqs[1];
 #pragma unroll
   for (int d = 0; d < DT; ++d)
@@ -253,6 +295,7 @@ __global__ void __launch_bounds__(64, DP <= 32 ? 2 : 1) k_attn_bwd_one(DofAttnBw
   dof_f32x16 dk[DT], dv[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) dk[d] = dv[d] = dof_zero16();
+  Range<T> range;
   // the first row that sees the lane's key
   const int mine = !A.causal || col < t.prefix || col - off < 0 ? 0 : col - off;
 
@@ -292,11 +335,23 @@ __global__ void __launch_bounds__(64, DP <= 32 ? 2 : 1) k_attn_bwd_one(DofAttnBw
       float d = hidden ? 0.0f : p[v] * y[v];
       d = dof_row16_sum(d);
       d += __shfl_xor(d, 16);
-      ds[v] = hidden ? 0.0f : p[v] * (KIND == 0 ? Lift<T>::ds / Lift<T>::p : c[v]) * (y[v] - d / Lift<T>::p);
+      ds[v] = hidden ? 0.0f : p[v] * (KIND == 0 ? 1.0f : c[v]) * (y[v] - d / Lift<T>::p);
+    }
+    // for dk the lanes' own factors; for dq, whose operand holds rows of all lanes, one for the document and head
+    float dsk[16], whole = 1.0f;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) dsk[v] = ds[v];
+    if constexpr (Range<T>::kOn) {
+      float mx = Range<T>::top(ds);
+      range.follow(mx, dk);
+      range.apply(dsk);
+#pragma unroll
+      for (int m = 1; m < 32; m <<= 1) mx = fmaxf(mx, __shfl_xor(mx, m));
+      whole = Range<T>::fit(mx);
     }
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const DofFrag<T> pf = dof_frag_pack<T>(p + 8 * s), df = dof_frag_pack<T>(ds + 8 * s), rest = dof_frag_rest<T>(ds + 8 * s, df);
+      const DofFrag<T> pf = dof_frag_pack<T>(p + 8 * s), df = dof_frag_pack<T>(dsk + 8 * s), rest = dof_frag_rest<T>(dsk + 8 * s, df);
       const int r = 16 * s + 4 * half;
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
@@ -310,8 +365,9 @@ __global__ void __launch_bounds__(64, DP <= 32 ? 2 : 1) k_attn_bwd_one(DofAttnBw
     for (int v = 0; v < 16; ++v) {
       const int to = sds[0].offset(8 * (v / 4) + v % 4 + 4 * half, col / Tile::EPC);
       T* e = reinterpret_cast<T*>(sds[0].mem + to) + col % Tile::EPC;
-      DofElem<T>::put(e, ds[v]);
-      if constexpr (sizeof(T) == 2) DofElem<T>::put(reinterpret_cast<T*>(sds[1].mem + to) + col % Tile::EPC, ds[v] - DofElem<T>::get(e));
+      const float x = ds[v] * whole;
+      DofElem<T>::put(e, x);
+      if constexpr (sizeof(T) == 2) DofElem<T>::put(reinterpret_cast<T*>(sds[1].mem + to) + col % Tile::EPC, x - DofElem<T>::get(e));
     }
     __syncthreads();
     // dq (queries in registers, d over the lanes) = dS K
@@ -330,7 +386,7 @@ __global__ void __launch_bounds__(64, DP <= 32 ? 2 : 1) k_attn_bwd_one(DofAttnBw
         if constexpr (sizeof(T) == 2) dq[d] = dof_mma32<T>(sds[1].rowfrag(col, 2 * s + half), k, dq[d]);
       }
     }
-    const float out = B.scale / Lift<T>::ds;
+    const float out = B.scale / Lift<T>::p / whole;
     T* dqp = static_cast<T*>(B.dq) + t.q0 * B.dqs[0] + h * B.dqs[1];
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -343,7 +399,7 @@ __global__ void __launch_bounds__(64, DP <= 32 ? 2 : 1) k_attn_bwd_one(DofAttnBw
   if (!live) return;
   T* dkp = static_cast<T*>(B.dk) + (t.k0 + col) * B.dks[0] + hk * B.dks[1];
   T* dvp = static_cast<T*>(B.dv) + (t.k0 + col) * B.dvs[0] + hk * B.dvs[1];
-  const float ok = B.scale / Lift<T>::ds, ov = 1.0f / Lift<T>::p;
+  const float ok = B.scale / Lift<T>::p / range.f, ov = 1.0f / Lift<T>::p;
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -411,6 +467,7 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_
   dof_f32x16 dk[DK ? DT : 1], dv[DV ? DT : 1];
   DofLongSum<T, dof_f32x16, DK ? DT : 1, LONG> ldk;
   DofLongSum<T, dof_f32x16, DV ? DT : 1, LONG> ldv;
+  Range<T> range;  // of dS
   if constexpr (DK) ldk.clear();
   if constexpr (DV) ldv.clear();
 #pragma unroll
@@ -475,7 +532,7 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_
       for (int v = 0; v < 16; ++v) {
         const int r = 8 * (v / 4) + v % 4 + 4 * half;
         p[v] = weight<T, KIND>(x[v], A.score.mul, w[v], sl[buf][r], sizeof(T) == 4 ? sr[buf][r] : 0.0f);
-        if constexpr (DK) ds[v] = p[v] * (KIND == 0 ? Lift<T>::ds / Lift<T>::p : c[v]) * (y[v] - sd[buf][r]);
+        if constexpr (DK) ds[v] = p[v] * (KIND == 0 ? 1.0f : c[v]) * (y[v] - sd[buf][r]);
       }
       if (partial) {
 #pragma unroll
@@ -484,6 +541,10 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_
           if constexpr (DV) p[v] = hidden ? 0.0f : p[v];
           if constexpr (DK) ds[v] = hidden ? 0.0f : ds[v];
         }
+      }
+      if constexpr (DK && Range<T>::kOn) {
+        range.follow(Range<T>::top(ds), dk);
+        range.apply(ds);
       }
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
@@ -513,7 +574,7 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_
   if constexpr (DK) ldk.finish(dk);
   if constexpr (DV) ldv.finish(dv);
   if (!live) return;
-  const float ok = B.scale / Lift<T>::ds, ov = 1.0f / Lift<T>::p;
+  const float ok = B.scale / Lift<T>::p / range.f, ov = 1.0f / Lift<T>::p;
   auto write = [&](const dof_f32x16* acc, float f, void* out, const int64_t* st, float* part) {
 #pragma unroll
     for (int d = 0; d < DT; ++d)

@@ -254,3 +254,39 @@ def test_step_over_millions_of_frames():
     # a chain of 512 additions in a wavefront, four wavefronts, at most n / 8192 parts in a chain of their own, 64 for the weights
     rel = (512 + 4 + n / 8192 / 8 + 64) * U32
     assert float((o.cpu().double() / vc[0, :1].cpu().double() - 1).abs().max()) <= rel
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("side", ["dq", "dk"])
+# documents, size of the gradients, of the values, of the keys (queries)
+@pytest.mark.parametrize("lens,gs,vs,ks", [([512], 2.0 ** -10, 1.0, 256.0), ([100, 300], 2.0 ** -13, 1.0, 1024.0), ([30, 17], 2.0 ** -13, 0.25, 512.0),
+                                           ([40], 1.0, 1.0, 1.0), ([40], 2048.0, 1024.0, 2.0 ** -7), ([5, 20], 2048.0, 1024.0, 2.0 ** -7)])
+def test_float16_score_gradients_of_any_size(device, side, lens, gs, vs, ks):
+    """Equal weights 1 / n: with q = 0 dq is dS k / 4, with k = 0 dk is dS^T q / 4, dS = (g v - delta) / n between 1e-7 and 1e6."""
+    ops = make_ops(device)
+    gen = torch.Generator().manual_seed(8)
+    n, d = sum(lens), 16
+    q, k, v, g = ((torch.randn(n, 1, d, generator=gen) * x).half() for x in (ks, ks, vs, gs))
+    (q if side == "dq" else k).zero_()
+    plan = ops.attention_plan(lens)
+    dev = [x.to(device) for x in (q, k, v)]
+    o, lse = ops.attention(plan, *dev)
+    got = dict(zip(("dq", "dk", "dv"), ops.attention_backward(plan, g.to(device), *dev, o, lse)))[side].cpu().double()[:, 0]
+    u, at = U[torch.float16], 0
+    for m in lens:
+        s = slice(at, at + m)
+        at += m
+        Q, K, V, G = (x[s, 0].double() for x in (q, k, v, g))
+        dP, O = G @ V.T, V.mean(0)
+        delta = (dP / m).sum(1, keepdim=True)
+        dS = (dP - delta) / m
+        # dS: the weights to 64 roundings; dP a product of 16 terms; delta from the rounded o (dq) or a sum of m; what its two parts lose
+        err = 64 * U32 * dS.abs() + (G.abs() @ V.abs().T * 18 * U32 + G.abs() @ O.abs()[:, None] * (u + 18 * U32)
+                                    + (dP.abs() / m).sum(1, keepdim=True) * (m + 16) * U32) / m
+        err = err + 2.0 ** -38 * (dS.abs().max() if max(lens) <= 32 else dS.abs().amax(1, keepdim=True) if side == "dq" else dS.abs().amax(0, keepdim=True))
+        if side == "dq":
+            want, e, size = dS @ K / 4, err @ K.abs() / 4, dS.abs() @ K.abs() / 4
+        else:
+            want, e, size = dS.T @ Q / 4, err.T @ Q.abs() / 4, dS.abs().T @ Q.abs() / 4
+        bound = u * want.abs() + (1 + u) * (e + (m / 16 + 16) * U32 * size) + 2.0 ** -25
+        assert bool(torch.isfinite(got[s]).all()) and bool(((got[s] - want).abs() <= bound).all()), float(((got[s] - want).abs() / bound).max())
