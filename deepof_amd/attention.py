@@ -17,7 +17,6 @@ outputs come from torch's allocator, one per call, so calls on different streams
 from __future__ import annotations
 
 import ctypes as C
-import math
 from typing import Optional, Sequence
 
 import numpy as np
@@ -100,30 +99,50 @@ def _is_wide(t: torch.Tensor) -> bool:
     return not bits & 15
 
 
-def _apart(name: str, out: Optional[torch.Tensor], **inputs):
-    """An output the caller gave may not lie in an input's memory: other workgroups still read it.  Both may be slices of one
-    buffer's rows (a packed q | k | v): rows of a common pitch are compared by their place in the pitch."""
-    if not isinstance(out, torch.Tensor) or out.numel() == 0:
+def _apart(name: str, out: Optional[torch.Tensor], /, **inputs):
+    """An output the caller gave may not share a byte with an input: other workgroups still read it.  Both may be slices of one
+    buffer in any order (a packed q | k | v, heads side by side)."""
+    if not isinstance(out, torch.Tensor):
         return
     for other, t in inputs.items():
-        if not isinstance(t, torch.Tensor) or t.numel() == 0:
-            continue
-        lo, inner, whole, outer = _extent(out)
-        lo2, inner2, whole2, outer2 = _extent(t)
-        if lo >= lo2 + whole2 or lo2 >= lo + whole:
-            continue
-        pitch = math.gcd(*outer, *outer2)
-        at = (lo2 - lo) % pitch if pitch else 0
-        if not (inner <= at and at + inner2 <= pitch):
+        if isinstance(t, torch.Tensor) and _share(out, t):
             raise ValueError(f"{name} must not share memory with {other}")
 
 
-def _extent(t: torch.Tensor):
-    """First byte, bytes from there of one (head, element) plane and of the whole, and the outer strides in bytes."""
-    e = t.element_size()
-    spans = [(n - 1) * s * e for n, s in zip(t.shape, t.stride())]
-    outer = [s * e for n, s in zip(t.shape[:-2], t.stride()[:-2]) if n > 1]
-    return t.data_ptr(), sum(spans[-2:]) + e, sum(spans) + e, outer
+def _share(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Do two tensors have a byte in common?  Exact for slices of one buffer; tensors whose strides have so little to do with
+    each other that the search grows long count as sharing."""
+    apart = b.data_ptr() - a.data_ptr()
+    if apart < 0:
+        a, b, apart = b, a, -apart
+    if a.is_contiguous() and apart >= a.nbytes or a.numel() == 0 or b.numel() == 0:
+        return False
+    ea, eb = a.element_size(), b.element_size()
+    if apart >= ea + ea * sum((n - 1) * s for n, s in zip(a.shape, a.stride())):
+        return False
+    # is `apart` a sum of i * stride over a's dimensions, less one over b's, plus the place of a byte in either's element?
+    range_of = {1: [1 - eb, ea - 1]}
+    for t, e, sign in ((a, ea, 0), (b, eb, 1)):
+        for n, s in zip(t.shape, t.stride()):
+            if n > 1 and s > 0:
+                r = range_of.setdefault(s * e, [0, 0])
+                r[1 - sign] += (1 - 2 * sign) * (n - 1)
+    dims = sorted(((s, lo, hi) for s, (lo, hi) in range_of.items()), reverse=True)
+    reach = [(0, 0)]  # what the dimensions from the k-th on can add up to
+    for s, lo, hi in reversed(dims):
+        reach.insert(0, (reach[0][0] + s * lo, reach[0][1] + s * hi))
+    left = [10000]
+
+    def found(k, want):
+        if k == len(dims):
+            return want == 0
+        left[0] -= 1
+        if left[0] < 0:
+            return True
+        (s, lo, hi), (least, most) = dims[k], reach[k + 1]
+        return any(found(k + 1, want - i * s) for i in range(max(lo, -((most - want) // s)), min(hi, (want - least) // s) + 1))
+
+    return found(0, apart)
 
 
 def _wide(t: torch.Tensor) -> torch.Tensor:
@@ -317,7 +336,7 @@ class AttentionOps:
         ``h // (query heads / key heads)``.  Scores ``scale q.k`` (default ``head_dim ** -0.5``), ``cap``: ``cap tanh(score / cap)``,
         ``slopes`` (fp32 per query head): minus ``slope * distance``.  lse (rows, query heads), fp32, natural log.  A row that sees no
         key gives zeros and -inf.  Rows behind the last document are left as they were in ``out`` / ``lse`` and are zeros in tensors
-        allocated here.  ``out`` may not lie in q, k or v.  head_dim: a multiple of 8 up to 128."""
+        allocated here.  ``out`` and ``lse`` may not lie in q, k, v or each other.  head_dim: a multiple of 8 up to 128."""
         head, sl = self._attention_args(plan, q, k, v, scale, cap, slopes)
         _apart("out", out, q=q, k=k, v=v)
         tail = q.shape[0] > plan.q_rows
@@ -326,6 +345,8 @@ class AttentionOps:
         o = self._output("out", out, q)
         if lse is None:
             lse = (torch.zeros if tail else torch.empty)(q.shape[:2], dtype=torch.float32, device=self.device)
+        else:
+            _apart("lse", lse, q=q, k=k, v=v, out=out)
         self._lse(lse, q)
         q, k, v = _wide(q), _wide(k), _wide(v)
         ow = o if _is_wide(o) else o.clone(memory_format=torch.contiguous_format)
@@ -384,8 +405,8 @@ class AttentionOps:
         if hk < 1 or hq % hk or hq < 1:
             raise ValueError(f"{hq} query heads are not a multiple of {hk} key heads")
         _apart("out", out, q=q, k=k, v=v, k_cache=k_cache, v_cache=v_cache)
-        if k_cache.data_ptr() == v_cache.data_ptr() and k_cache.numel():
-            raise ValueError("k_cache and v_cache must be two tensors")
+        if _share(k_cache, v_cache):
+            raise ValueError("k_cache and v_cache must be two tensors that share no memory")
         if not (_is_wide(k_cache) and _is_wide(v_cache)):
             raise ValueError("the caches' address and strides must be multiples of 16 bytes")
         if page_table.dim() != 2 or page_table.shape[0] != b or page_table.dtype != torch.int32 or page_table.device != self.device \

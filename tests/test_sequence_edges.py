@@ -290,3 +290,62 @@ def test_float16_score_gradients_of_any_size(device, side, lens, gs, vs, ks):
             want, e, size = dS.T @ Q / 4, err.T @ Q.abs() / 4, dS.abs().T @ Q.abs() / 4
         bound = u * want.abs() + (1 + u) * (e + (m / 16 + 16) * U32 * size) + 2.0 ** -25
         assert bool(torch.isfinite(got[s]).all()) and bool(((got[s] - want).abs() <= bound).all()), float(((got[s] - want).abs() / bound).max())
+
+
+def test_shared_memory_is_found_and_nothing_else():
+    """Against a set of the bytes that each of two views of one small buffer addresses."""
+    from deepof_amd.attention import _share
+    gen = np.random.default_rng(3)
+    buf = torch.zeros(300, dtype=torch.float16)
+    wide = buf.view(torch.float32)
+
+    def view():
+        base, size = (buf, 2) if gen.random() < 0.7 else (wide, 4)
+        shape = tuple(int(x) for x in gen.integers(1, 5, 3))
+        stride = tuple(int(x) for x in gen.choice([0, 1, 2, 3, 4, 6, 8, 12, 24, 36], 3))
+        room = base.numel() - 1 - sum((n - 1) * s for n, s in zip(shape, stride))
+        if room < 0:
+            return view()
+        at = int(gen.integers(0, room + 1))
+        t = torch.as_strided(base, shape, stride, at)
+        idx = at + sum(s * np.arange(n).reshape([-1 if k == d else 1 for k in range(3)]) for d, (n, s) in enumerate(zip(shape, stride)))
+        return t, {int(i) * size + b for i in idx.ravel() for b in range(size)}
+
+    seen = [0, 0]
+    for _ in range(3000):
+        (a, bytes_a), (b, bytes_b) = view(), view()
+        want = bool(bytes_a & bytes_b)
+        seen[want] += 1
+        assert _share(a, b) == want, (a.shape, a.stride(), a.storage_offset(), b.shape, b.stride(), b.storage_offset())
+    assert min(seen) > 300
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_slices_of_one_buffer(device):
+    """Outputs whose heads or elements lie between those of the inputs are taken; an lse in the output's memory, and caches that
+    overlap without beginning together, are not."""
+    ops = make_ops(device)
+    gen = torch.Generator().manual_seed(6)
+    plan = ops.attention_plan([4, 5])
+    for buf, at in ((torch.randn(9, 3, 4, 16, generator=gen), lambda b, i: b[:, :, i]), (torch.randn(4, 3, 9, 16, generator=gen), lambda b, i: b[i].transpose(0, 1)),
+                    (torch.randn(3, 4, 9, 16, generator=gen), lambda b, i: b[:, i].transpose(0, 1))):
+        buf = buf.to(device)
+        o, q, k, v = (at(buf, i) for i in range(4))
+        want, _ = ops.attention(plan, q.contiguous(), k.contiguous(), v.contiguous())
+        got, _ = ops.attention(plan, q, k, v, out=o)
+        assert got is o and torch.equal(o, want)
+        with pytest.raises(ValueError, match="share memory"):
+            ops.attention(plan, q, k, v, out=q)
+    q = torch.randn(9, 3, 16, generator=gen).to(device)
+    o = torch.zeros(9, 3, 16, device=device)
+    with pytest.raises(ValueError, match="share memory"):
+        ops.attention(plan, q, q, q, out=o, lse=o.view(-1)[:27].view(9, 3))
+    with pytest.raises(ValueError, match="share memory"):
+        ops.attention(plan, q, q, q, lse=q.view(-1)[:27].view(9, 3))
+    kv = torch.randn(6, 8, 4, 16, generator=gen).to(device)
+    new, table, lengths = torch.randn(1, 1, 2, 16, device=device), torch.zeros(1, 1, dtype=torch.int32, device=device), torch.zeros(1, dtype=torch.int32, device=device)
+    for a, b in ((kv[:4, :, :2], kv[1:5, :, :2]), (kv[:, :, :2], kv[:, :, 1:3])):
+        with pytest.raises(ValueError, match="share"):
+            ops.attention_step(new, new, new, a, b, table, lengths)
+    ops.attention_step(new, new, new, kv[:, :, :2], kv[:, :, 2:], table, lengths)
+    assert torch.equal(kv[0, 0], torch.cat((new, new), 2)[0, 0])
