@@ -117,13 +117,21 @@ def _share(a: torch.Tensor, b: torch.Tensor) -> bool:
         a, b, apart = b, a, -apart
     if a.is_contiguous() and apart >= a.nbytes or a.numel() == 0 or b.numel() == 0:
         return False
-    ea, eb = a.element_size(), b.element_size()
-    if apart >= ea + ea * sum((n - 1) * s for n, s in zip(a.shape, a.stride())):
+    ea, eb, sa, sb = a.element_size(), b.element_size(), a.stride(), b.stride()
+    inner_a, inner_b = ea, eb  # bytes from the first to the last of one row
+    for n, s in zip(a.shape[1:], sa[1:]):
+        inner_a += (n - 1) * s * ea
+    for n, s in zip(b.shape[1:], sb[1:]):
+        inner_b += (n - 1) * s * eb
+    if apart >= inner_a + (a.shape[0] - 1) * sa[0] * ea:
         return False
+    pitch = sa[0] * ea
+    if pitch == sb[0] * eb and pitch and inner_a <= apart % pitch <= pitch - inner_b:
+        return False  # side by side in rows of one buffer
     # is `apart` a sum of i * stride over a's dimensions, less one over b's, plus the place of a byte in either's element?
     range_of = {1: [1 - eb, ea - 1]}
-    for t, e, sign in ((a, ea, 0), (b, eb, 1)):
-        for n, s in zip(t.shape, t.stride()):
+    for t, st, e, sign in ((a, sa, ea, 0), (b, sb, eb, 1)):
+        for n, s in zip(t.shape, st):
             if n > 1 and s > 0:
                 r = range_of.setdefault(s * e, [0, 0])
                 r[1 - sign] += (1 - 2 * sign) * (n - 1)
