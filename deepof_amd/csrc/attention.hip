@@ -13,7 +13,6 @@
 namespace {
 
 constexpr int64_t kMaxRows = 1 << 30;           // of one document
-constexpr int64_t kMaxBlocks = (1LL << 24) - 1;  // of 256 threads: a launch holds less than 2^32
 
 int check_plan_args(int32_t n_docs, const int64_t* q_off, const int64_t* k_off, const void* out) {
   if (n_docs < 0 || (n_docs > 0 && (!q_off || !k_off)) || !out) {
@@ -93,10 +92,19 @@ int check(const DofAttnPlan* p, const void* table, const DofAttention* d, const 
     return DOF_ERR_ARG;
   }
   for (int i = 0; i < 4; ++i)
-    if (p->n_tiles[i] < 0 || p->n_tiles[i] > kMaxBlocks / d->q_heads) {
-      dof_set_error("%s: too many tiles for one launch (%lld tiles, %d heads)", who, (long long)p->n_tiles[i], (int)d->q_heads);
-      return DOF_ERR_UNSUPPORTED;
+    if (p->n_tiles[i] < 0) {
+      dof_set_error("%s: bad plan", who);
+      return DOF_ERR_ARG;
     }
+  return DOF_OK;
+}
+
+// a launch holds less than 2^32 threads: a wavefront per flat tile and head, four per tall one
+int check_launch(int64_t tiles, int64_t heads, int flat, const char* who) {
+  if (tiles > ((1LL << 32) - 1) / (flat ? 64 : 256) / heads) {
+    dof_set_error("%s: too many tiles for one launch (%lld tiles, %lld heads)", who, (long long)tiles, (long long)heads);
+    return DOF_ERR_UNSUPPORTED;
+  }
   return DOF_OK;
 }
 
@@ -264,6 +272,8 @@ extern "C" int dof_attention_forward(const DofAttnPlan* plan, const void* table,
   }
   DofAttnFwd A = forward_args(d, q, k, v, slopes, o, lse);
   const int flat = flat_tiles(plan, 0);
+  rc = check_launch(plan->n_tiles[flat], d->q_heads, flat, "dof_attention_forward");
+  if (rc != DOF_OK) return rc;
   set_tiles(&A, plan, table, 0, flat);
   return dof_launch_attn_fwd(A, d->dtype, flat, (hipStream_t)stream);
 }
@@ -308,18 +318,24 @@ extern "C" int dof_attention_backward(const DofAttnPlan* plan, const void* table
     B.dks[i] = d->dk_stride[i];
     B.dvs[i] = d->dv_stride[i];
   }
+  static const char who[] = "dof_attention_backward";
   if (one) {
+    rc = check_launch(plan->n_tiles[3], d->k_heads, 1, who);
+    if (rc != DOF_OK) return rc;
     set_tiles(&B.f, plan, table, 2, 1);
     return dof_launch_attn_bwd_one(B, d->dtype, (hipStream_t)stream);
   }
+  const int flat = flat_tiles(plan, 0);
+  const Shares s = shares_of(plan, d);
+  rc = check_launch(plan->n_tiles[flat], d->q_heads, flat, who);
+  if (rc == DOF_OK) rc = check_launch(plan->n_tiles[2 + s.flat], (int64_t)d->k_heads * s.splits, s.flat, who);
+  if (rc != DOF_OK) return rc;
   if (rows) {
-    const int flat = flat_tiles(plan, 0);
     set_tiles(&B.f, plan, table, 0, flat);
     rc = dof_launch_attn_dq(B, d->dtype, flat, (hipStream_t)stream);
     if (rc != DOF_OK) return rc;
   }
   if (keys) {
-    const Shares s = shares_of(plan, d);
     B.splits = s.splits;
     B.heads_per = s.heads_per;
     B.k_rows = plan->k_rows;

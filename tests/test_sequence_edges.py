@@ -349,3 +349,28 @@ def test_slices_of_one_buffer(device):
             ops.attention_step(new, new, new, a, b, table, lengths)
     ops.attention_step(new, new, new, kv[:, :, :2], kv[:, :, 2:], table, lengths)
     assert torch.equal(kv[0, 0], torch.cat((new, new), 2)[0, 0])
+
+
+def test_launch_limits():
+    """Less than 2^32 threads in a launch: counted for the tiles that are launched, at 256 threads for a tall one and 64 for a flat
+    one.  Refused before anything is launched; nothing of the (absent) tensors is touched."""
+    ops = make_ops("cpu")
+
+    def record(lens, heads):
+        off = np.concatenate(([0], np.cumsum(np.asarray(lens, dtype=np.int64))))
+        plan = _capi.AttnPlan()
+        _capi.check(ops.lib, ops.lib.dof_attn_plan_size(len(lens), off.ctypes.data, off.ctypes.data, 0, C.byref(plan)), "size")
+        st = (heads * 64, 64)
+        return plan, _capi.PACK_ATTENTION.pack(_capi.DTYPE_BF16, 64, heads, heads, 0.125, 0.0, *(st * 8))
+
+    # one document of 2^29 rows, 2 heads: 2^23 tall tiles are launched, the 2^25 flat ones are not
+    plan, rec = record([2 ** 29], 2)
+    assert ops._bytes("dof_attention_workspace_bytes", C.byref(plan), rec) >= 2 ** 29 * 2 * 4
+    hold = torch.zeros(64)
+    some = hold.data_ptr() // 64 * 64 + 64
+    for lens, heads in (([2 ** 30] * 2, 1), ([2 ** 30], 4), ([20] * 70000, 1000)):
+        plan, rec = record(lens, heads)
+        rc = ops.lib.dof_attention_forward(C.byref(plan), some, rec, some, some, some, 0, some, some, 0)
+        assert rc < 0 and b"too many tiles" in ops.lib.dof_last_error_string()
+        rc = ops.lib.dof_attention_backward(C.byref(plan), some, rec, some, some, some, some, 0, some, some, some, some, some, some, 0)
+        assert rc < 0 and b"too many tiles" in ops.lib.dof_last_error_string()
