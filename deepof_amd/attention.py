@@ -8,7 +8,7 @@ frames of live streams against a paged key / value cache.  Elements are float32,
 statistics are fp32.
 
 Gradients are explicit: every ``*_backward`` takes the gradients at the outputs and returns those at the inputs; autograd does not
-record these calls.
+record these calls.  Tensors of the caller that a call writes to are marked as changed, as torch's own in-place operations mark them.
 
 ``AttentionOps`` issues the C-ABI calls (include/deepof_hip.h) on the current HIP stream of its device; product code obtains it
 through :func:`create_attention_ops`, which requires a ROCm device and the compiled library and raises otherwise.  Workspaces and
@@ -21,6 +21,7 @@ from typing import Optional, Sequence
 
 import numpy as np
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _capi
 
@@ -71,6 +72,13 @@ def _writable(name: str, t: torch.Tensor):
         if n > 1 and s == 0:
             raise ValueError(f"{name} is an expanded view; its elements must be distinct")
     return t
+
+
+def _changed(*tensors: Optional[torch.Tensor]):
+    """The caller's tensors that the call writes to: autograd then refuses a backward pass which needs what they held."""
+    for t in tensors:
+        if t is not None:
+            increment_version(t)
 
 
 def _vector(name: str, t: Optional[torch.Tensor], n: int, dtype, device):
@@ -282,8 +290,10 @@ class AttentionOps:
                 _apart(name, out, **{name[0]: x})
         if q_out is not None and k_out is not None:
             _apart("q_out", q_out, k_out=k_out)
+        given = q_out, k_out
         q_out = self._output("q_out", q_out, q)
         k_out = self._output("k_out", k_out, k)
+        _changed(*given)
         rec = _capi.PACK_NORM_ROPE.pack(*head, *_st(q), *_st(k), *_st(q_out), *_st(k_out), 0, 0, 0, 0)
         self._launch("dof_norm_rope_forward", rec, q.data_ptr(), k.data_ptr(), *ptrs, q_out.data_ptr(), k_out.data_ptr())
         return q_out, k_out
@@ -347,7 +357,7 @@ class AttentionOps:
         allocated here.  ``out`` and ``lse`` may not lie in q, k, v or each other.  head_dim: a multiple of 8 up to 128."""
         head, sl = self._attention_args(plan, q, k, v, scale, cap, slopes)
         _apart("out", out, q=q, k=k, v=v)
-        tail = q.shape[0] > plan.q_rows
+        tail, given = q.shape[0] > plan.q_rows, (out, lse)
         if out is None and tail:
             out = q.new_zeros(q.shape)
         o = self._output("out", out, q)
@@ -356,6 +366,7 @@ class AttentionOps:
         else:
             _apart("lse", lse, q=q, k=k, v=v, out=out)
         self._lse(lse, q)
+        _changed(*given)
         q, k, v = _wide(q), _wide(k), _wide(v)
         ow = o if _is_wide(o) else o.clone(memory_format=torch.contiguous_format)
         rec = _capi.PACK_ATTENTION.pack(*head, *_st(q), *_st(k), *_st(v), *_st(ow), 0, 0, 0, 0, 0, 0, 0, 0)
@@ -423,6 +434,7 @@ class AttentionOps:
         ln = _vector("lengths", lengths, b, torch.int32, self.device)
         sl = _vector("slopes", slopes, hq, torch.float32, self.device)
         o = self._output("out", out, q)
+        _changed(k_cache, v_cache, out)
         ow = o if _is_wide(o) else o.clone(memory_format=torch.contiguous_format)
         q, k, v = _wide(q), _wide(k), _wide(v)
         rec = _capi.PACK_ATTN_STEP.pack(DTYPES[dt], dim, hq, hk, b, new, k_cache.shape[0], k_cache.shape[1], page_table.shape[1], 0,

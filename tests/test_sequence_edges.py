@@ -374,3 +374,33 @@ def test_launch_limits():
         assert rc < 0 and b"too many tiles" in ops.lib.dof_last_error_string()
         rc = ops.lib.dof_attention_backward(C.byref(plan), some, rec, some, some, some, some, 0, some, some, some, some, some, some, 0)
         assert rc < 0 and b"too many tiles" in ops.lib.dof_last_error_string()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_written_tensors_count_as_changed(device):
+    """A graph that saved a tensor which a call then writes over must not run backward on the new values."""
+    ops = make_ops(device)
+    pos, freqs = torch.arange(6, dtype=torch.int32, device=device), torch.ones(8, dtype=torch.float64, device=device)
+    w = torch.ones(6, 2, 16, device=device, requires_grad=True)
+    q, k = (torch.randn(6, 2, 16, device=device) for _ in range(2))
+    plan = ops.attention_plan([6])
+    lse = torch.zeros(6, 2, device=device)
+    kc, vc = (torch.zeros(2, 16, 2, 16, device=device) for _ in range(2))
+    new = q[None, :1]
+
+    def step():
+        ops.attention_step(new, new, new, kc, vc, torch.zeros(1, 1, dtype=torch.int32, device=device), torch.zeros(1, dtype=torch.int32, device=device),
+                           out=torch.zeros_like(new))
+
+    for held, call in ((q, lambda: ops.norm_rope(q, k, pos, freqs, q_out=q)), (k, lambda: ops.norm_rope(q, k, pos, freqs, k_out=k)),
+                       (k, lambda: ops.attention(plan, q, q, q, out=k)), (lse, lambda: ops.attention(plan, q, q, q, lse=lse)), (kc, step), (vc, step)):
+        y = ((w.flatten()[0] if held.shape != w.shape else w) * held).sum()
+        call()
+        with pytest.raises(RuntimeError, match="inplace operation"):
+            y.backward()
+    y = (w * q).sum()
+    ops.norm_rope(q, k, pos, freqs)  # writes to its own outputs only
+    y.backward()
+    with torch.inference_mode():
+        x = torch.randn(6, 2, 16, device=device)
+        ops.norm_rope(x, k, pos, freqs, q_out=x)
