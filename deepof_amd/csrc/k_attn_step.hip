@@ -234,7 +234,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) k_attn
     return w;
   };
   // Loads of a tile.  A frame that is nowhere reads the head's first one instead: its score is masked, its value made zero.  Elements
-  // behind the head size read its start: they meet zeros of q, or columns of the result that are not written.
+  // behind the head size read its start: those of keys are made zero before the product (an infinity there would meet q's zeros),
+  // those of values are columns of the result that are not written.
   auto load = [&](int tile, Where w) {
     const int key = tile * kStepKeys + (lane & 31);
     int64_t ko = w.page * A.d.kc_stride[0] + w.slot * A.d.kc_stride[1], vo = w.page * A.d.vc_stride[0] + w.slot * A.d.vc_stride[1];
@@ -283,6 +284,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) k_attn
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) sv[wave].put(lane & 31, (lane >> 5) + 2 * i, vreg[i]);
+    if (32 * (KS - 1) + 8 * quad >= dim) kf[0][KS - 1] = kf[1][KS - 1] = dof_frag_zero<T>();
     dof_f32x4 x[RT][2];
 #pragma unroll
     for (int i = 0; i < RT; ++i)

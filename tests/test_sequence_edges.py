@@ -404,3 +404,21 @@ def test_written_tensors_count_as_changed(device):
     with torch.inference_mode():
         x = torch.randn(6, 2, 16, device=device)
         ops.norm_rope(x, k, pos, freqs, q_out=x)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("d", [8, 32, 72])
+def test_step_with_infinite_keys(device, dtype, d):
+    """A cached key whose score is -inf has weight zero, as one whose score is far below the others'."""
+    ops = make_ops(device)
+    g = torch.Generator().manual_seed(9)
+    q, k, v = (torch.randn(1, 1, 2, d, generator=g).to(dtype).to(device) for _ in range(3))
+    q[..., 0] = 1.0
+    kc, vc = (torch.randn(3, 16, 2, d, generator=g).to(dtype).to(device) for _ in range(2))
+    table, lengths = torch.arange(3, dtype=torch.int32, device=device)[None], torch.tensor([40], dtype=torch.int32, device=device)
+    outs = []
+    for low in (-30000.0, -math.inf):
+        kc[0, 3, :, 0], kc[1, 7, 1, 0] = low, low
+        outs.append(ops.attention_step(q, k, v, kc, vc.clone(), table, lengths))
+    assert bool(torch.isfinite(outs[1]).all()) and torch.equal(*outs)
