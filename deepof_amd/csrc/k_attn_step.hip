@@ -18,6 +18,7 @@
 // frame of a round and loads half of that frame's value itself, so that a round's loads are one address and fixed offsets per lane
 // (with an address per load the address arithmetic took longer than the loads: 64 streams of up to 5000 frames 201 us).
 // New frames are read from k and v, not from the cache, so storing them (by the first workgroup of a stream's head) races with nobody.
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 
@@ -30,9 +31,8 @@ namespace {
 
 constexpr int kStepKeys = 32;   // frames per wavefront and round
 constexpr int kMinTiles = 16;   // rounds of a part at least: four per wavefront
-constexpr int kMaxTiles = 256;  // and at most: 64 rounds per wavefront, a chain of 512 additions of fp32 products
 constexpr int kWhole = 32;      // streams whose table holds no more rounds stay whole: a second kernel for the join costs more
-constexpr int kTarget = 1024;   // parts of a call in all, unless kMaxTiles makes them more: two rounds of two workgroups per CU
+constexpr int kTarget = 1024;   // parts of a call in all: two rounds of two workgroups per CU
 
 struct Step {
   DofAttnStep d;
@@ -94,7 +94,8 @@ __device__ __forceinline__ Part find_part(const Step& A, int unit) {
   }
   const int64_t share = (all * A.d.k_heads * A.row_blocks + kTarget - 1) / kTarget;
   Part p;
-  p.per = share > kMaxTiles ? kMaxTiles : share > A.min_tiles ? (int)share : A.min_tiles;
+  constexpr int64_t most = 1 << 30;  // more than the tiles of any stream
+  p.per = share > most ? (int)most : share > A.min_tiles ? (int)share : A.min_tiles;
   int before = 0;
   for (int b0 = 0; b0 < A.d.streams; b0 += 256) {
     if (b0 > 0) __syncthreads();
@@ -144,9 +145,9 @@ __device__ __forceinline__ void finish(const Step& A, const int32_t* table, int 
   dof_store_vec<T, 4>(static_cast<T*>(A.o) + b * A.d.o_stride[0] + t * A.d.o_stride[1] + (hk * group + g) * A.d.o_stride[2] + e, v);
 }
 
-// RT: tiles of 16 rows.  MULTI: more than one new frame.
-template <class T, int DP, int RT, bool MULTI>
-__global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) k_attn_step(Step A) {
+// RT: tiles of 16 rows.  MULTI: more than one new frame.  LONG: a wavefront's sums may grow long and are made of blocks (fp32)
+template <class T, int DP, int RT, bool MULTI, bool LONG>
+__global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 32 * (3 - RT) + 32 ? 1 : 2) k_attn_step(Step A) {
   using Tile = DofTile<T, kStepKeys, DP>;
   __shared__ Tile sv[4];
   __shared__ float sm[4][16 * RT], sl[4][16 * RT];
@@ -215,11 +216,13 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) k_attn
   const int64_t vfresh = reinterpret_cast<const char*>(static_cast<const T*>(A.v) + b * A.d.v_stride[0] + hk * A.d.v_stride[2]) - vbase;
 
   dof_f32x4 o[RT][DT];
-  float m[RT], l[RT];
+  DofLongSum<T, dof_f32x4, DT, LONG> lo[RT];
+  DofLongNumber<T> l[RT];
+  float m[RT];
 #pragma unroll
   for (int i = 0; i < RT; ++i) {
     m[i] = -INFINITY;
-    l[i] = 0.0f;
+    lo[i].clear();
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[i][d] = dof_zero4();
   }
@@ -345,7 +348,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) k_attn
         const bool up = mt > m[i] + DofSoftmax<T>::kLag;
         const float a = up ? dof_exp2(m[i] - mt) : 1.0f;
         m[i] = up ? mt : m[i];
-        l[i] *= a;
+        l[i].scale(a);
+        lo[i].scale(a);
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -360,10 +364,11 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) k_attn
           p[4 * u + e] = dof_exp2(x[i][u][e] - mm);
           part += p[4 * u + e];
         }
-      l[i] += part;
+      l[i].add(part);
       const DofFrag<T> pf = dof_frag_pack<T>(p);
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[i][d] = dof_mma16<T>(sv[wave].colfrag(4 * quad, 16 + 4 * quad, 16 * d + col), pf, o[i][d]);
+      lo[i].count(o[i], kStepKeys / 2);  // terms: kLongTerms allows for two per addition, a 16x16x4 product adds four
     }
     DOF_WAVE_LDS_ORDER();
   }
@@ -372,11 +377,13 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) k_attn
   // weighted to the rows' common maximum.
 #pragma unroll
   for (int i = 0; i < RT; ++i) {
-    l[i] += __shfl_xor(l[i], 16);
-    l[i] += dof_swap32(l[i]);
+    lo[i].finish(o[i]);
+    float sum = l[i].total();
+    sum += __shfl_xor(sum, 16);
+    sum += dof_swap32(sum);
     if (quad == 0) {
       sm[wave][16 * i + col] = m[i];
-      sl[wave][16 * i + col] = l[i];
+      sl[wave][16 * i + col] = sum;
     }
   }
   static_assert(sizeof(Tile) >= 16 * DP * sizeof(float), "a value tile holds sixteen rows of sums");
@@ -511,7 +518,7 @@ int check(const DofAttnStep* d, const char* who) {
 }
 
 // Row tiles of 16 per workgroup (1 or 2), blocks of them, and the most parts that find_part can make of the streams: each at most
-// one more than its share (of kTarget, or of kMaxTiles each), and no more than its table holds.
+// one more than its share, and no more than its table holds.
 struct Shape { int rows, rt, row_blocks, min_tiles; int64_t parts; };
 Shape shape_of(const DofAttnStep* d) {
   Shape s;
@@ -520,8 +527,7 @@ Shape shape_of(const DofAttnStep* d) {
   s.row_blocks = (s.rows + 16 * s.rt - 1) / (16 * s.rt);
   const int64_t tiles = ((int64_t)d->max_pages * d->page_size + kStepKeys - 1) / kStepKeys;
   s.min_tiles = tiles <= kWhole ? kWhole : kMinTiles;
-  const int64_t target = kTarget / ((int64_t)d->k_heads * s.row_blocks), longest = d->streams * tiles / kMaxTiles;
-  s.parts = d->streams + (target > longest ? target : longest);
+  s.parts = d->streams + kTarget / ((int64_t)d->k_heads * s.row_blocks);
   const int64_t most = (tiles + s.min_tiles - 1) / s.min_tiles * d->streams;
   if (s.parts > most) s.parts = most;
   return s;
@@ -533,13 +539,23 @@ bool aligned(const void* p, const int64_t* s, int size) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && s[0] * size % 16 == 0 && s[1] * size % 16 == 0 && s[2] * size % 16 == 0;
 }
 
-template <class T, int DP>
-void launch_rt(const Step& A, int rt, unsigned blocks, hipStream_t stream) {
+template <class T, int DP, int RT>
+void launch_rt(const Step& A, bool grows, unsigned blocks, hipStream_t stream) {
   const bool multi = A.d.new_frames > 1;
-  if (rt == 1 && !multi) DOF_LAUNCH((k_attn_step<T, DP, 1, false>), (blocks, 1, 1), (256, 1, 1), stream, A);
-  else if (rt == 1) DOF_LAUNCH((k_attn_step<T, DP, 1, true>), (blocks, 1, 1), (256, 1, 1), stream, A);
-  else if (!multi) DOF_LAUNCH((k_attn_step<T, DP, 2, false>), (blocks, 1, 1), (256, 1, 1), stream, A);
-  else DOF_LAUNCH((k_attn_step<T, DP, 2, true>), (blocks, 1, 1), (256, 1, 1), stream, A);
+  if constexpr (sizeof(T) == 4) {
+    if (grows) {
+      if (multi) DOF_LAUNCH((k_attn_step<T, DP, RT, true, true>), (blocks, 1, 1), (256, 1, 1), stream, A);
+      else DOF_LAUNCH((k_attn_step<T, DP, RT, false, true>), (blocks, 1, 1), (256, 1, 1), stream, A);
+      return;
+    }
+  }
+  if (multi) DOF_LAUNCH((k_attn_step<T, DP, RT, true, false>), (blocks, 1, 1), (256, 1, 1), stream, A);
+  else DOF_LAUNCH((k_attn_step<T, DP, RT, false, false>), (blocks, 1, 1), (256, 1, 1), stream, A);
+}
+template <class T, int DP>
+void launch(const Step& A, int rt, bool grows, unsigned blocks, hipStream_t stream) {
+  if (rt == 1) launch_rt<T, DP, 1>(A, grows, blocks, stream);
+  else launch_rt<T, DP, 2>(A, grows, blocks, stream);
 }
 
 }  // namespace
@@ -604,11 +620,14 @@ extern "C" int dof_attention_step(const DofAttnStep* d, const void* q, const voi
   A.page_shift = -1;
   if ((d->page_size & (d->page_size - 1)) == 0)
     while ((int64_t)1 << (A.page_shift + 1) <= d->page_size) ++A.page_shift;
+  // the most tiles that the streams' tables let a part have, four wavefronts to share them, kStepKeys / 4 additions each
+  const int64_t tiles = ((int64_t)d->max_pages * d->page_size + kStepKeys - 1) / kStepKeys, share = d->streams * tiles * d->k_heads * s.row_blocks / kTarget;
+  const bool grows = std::max<int64_t>(s.min_tiles, share) / 4 * (kStepKeys / 2) > kLongTerms;
   DOF_SEQ_DISPATCH(d->dtype, T, {
-    if (d->head_dim <= 32) launch_rt<T, 32>(A, s.rt, (unsigned)blocks, (hipStream_t)stream);
-    else if (d->head_dim <= 64) launch_rt<T, 64>(A, s.rt, (unsigned)blocks, (hipStream_t)stream);
-    else if (d->head_dim <= 96) launch_rt<T, 96>(A, s.rt, (unsigned)blocks, (hipStream_t)stream);
-    else launch_rt<T, 128>(A, s.rt, (unsigned)blocks, (hipStream_t)stream);
+    if (d->head_dim <= 32) launch<T, 32>(A, s.rt, grows, (unsigned)blocks, (hipStream_t)stream);
+    else if (d->head_dim <= 64) launch<T, 64>(A, s.rt, grows, (unsigned)blocks, (hipStream_t)stream);
+    else if (d->head_dim <= 96) launch<T, 96>(A, s.rt, grows, (unsigned)blocks, (hipStream_t)stream);
+    else launch<T, 128>(A, s.rt, grows, (unsigned)blocks, (hipStream_t)stream);
     if (joins(d, s)) DOF_LAUNCH((k_attn_step_join<T>), ((unsigned)rows, dof_cdiv(d->head_dim, 4 * A.join_lanes), 1), (256, 1, 1), (hipStream_t)stream, A);
   });
   return dof_check_launch("k_attn_step");

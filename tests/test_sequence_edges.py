@@ -240,6 +240,25 @@ def test_long_float32_sums_of_one_sign(device, n, d, few):
         assert float((dk3[at].cpu().double() * sign / want - 1).abs().max()) <= 4 * rel
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("d,new", [(8, 1), (72, 1), (40, 12), (128, 16)])
+def test_step_whose_table_is_far_longer_than_its_streams(device, d, new):
+    """The kernels for long sums, at lengths that need none of it."""
+    ops = make_ops(device)
+    g = torch.Generator().manual_seed(13)
+    q, k, v = (torch.randn(2, new, 2, d, generator=g).to(device) for _ in range(3))
+    kc, vc = (torch.randn(4, 256, 2, d, generator=g).to(device) for _ in range(2))
+    table = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32)
+    lengths = torch.tensor([300, 470], dtype=torch.int32, device=device)
+    outs = []
+    for columns in (2, 1 << 17):
+        t = torch.full((2, columns), -1, dtype=torch.int32)
+        t[:, :2] = table
+        outs.append(ops.attention_step(q, k, v, kc.clone(), vc.clone(), t.to(device), lengths))
+    # the same scores; 64 roundings of weights and division and a chain of at most 32 / 4 * 4 additions on either side, of what |v| bounds
+    assert float((outs[0] - outs[1]).abs().max()) <= 2 * (64 + 32) * U32 * max(float(v.abs().max()), float(vc.abs().max()))
+
+
 @pytest.mark.gpu
 def test_step_over_millions_of_frames():
     """16 million frames that lie on two pages, listed over and over; equal weights, values of one sign."""
@@ -251,8 +270,8 @@ def test_step_over_millions_of_frames():
     table[0, -1] = 1
     q = torch.zeros(1, 1, hk, d, device="cuda:0")
     o = ops.attention_step(q, torch.zeros_like(q), vc[:1, :1].clone(), kc, vc, table, torch.tensor([n], dtype=torch.int32, device="cuda:0"))
-    # a chain of 512 additions in a wavefront, four wavefronts, at most n / 8192 parts in a chain of their own, 64 for the weights
-    rel = (512 + 4 + n / 8192 / 8 + 64) * U32
+    # a wavefront's 32768 frames: blocks of 128 additions, 64 of them; four wavefronts, at most 128 parts; 64 for the weights
+    rel = (128 + 64 + 4 + 128 + 64) * U32
     assert float((o.cpu().double() / vc[0, :1].cpu().double() - 1).abs().max()) <= rel
 
 
