@@ -136,6 +136,7 @@ __global__ void __launch_bounds__(256) k_norm_rope(Args A) {
   Place at[NI];
   bool live[NI];
   float wa[NI][VEC], wb[NI][VEC], da[NI][VEC], db[NI][VEC];
+  float ta[NI][VEC], tb[NI][VEC];  // weight gradients of whole chunks: two short chains of additions in place of a long one
 #pragma unroll
   for (int n = 0; n < NI; ++n) {
     const int p = (lane + n * A.lpr) * VEC;
@@ -144,7 +145,7 @@ __global__ void __launch_bounds__(256) k_norm_rope(Args A) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       wa[n][i] = wb[n][i] = 1.0f;
-      da[n][i] = db[n][i] = 0.0f;
+      da[n][i] = db[n][i] = ta[n][i] = tb[n][i] = 0.0f;
       if (live[n] && normed) {
         wa[n][i] = S.w[at[n].apart ? at[n].a + i : at[n].a + 2 * i];
         wb[n][i] = S.w[at[n].apart ? at[n].b + i : at[n].a + 2 * i + 1];
@@ -247,6 +248,16 @@ __global__ void __launch_bounds__(256) k_norm_rope(Args A) {
       for (int n = 0; n < NI; ++n)
         if (inside && live[n]) store_pairs<T, VEC, INTER>(orow, at[n], BWD ? ga[n] : a[n], BWD ? gb[n] : b[n]);
     }
+    if (BWD && normed) {
+#pragma unroll
+      for (int n = 0; n < NI; ++n)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          ta[n][i] += da[n][i];
+          tb[n][i] += db[n][i];
+          da[n][i] = db[n][i] = 0.0f;
+        }
+    }
   }
 
   if constexpr (BWD) {
@@ -257,8 +268,8 @@ __global__ void __launch_bounds__(256) k_norm_rope(Args A) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i)
         for (int m = A.lpr; m < 64; m <<= 1) {
-          da[n][i] += __shfl_xor(da[n][i], m);
-          db[n][i] += __shfl_xor(db[n][i], m);
+          ta[n][i] += __shfl_xor(ta[n][i], m);
+          tb[n][i] += __shfl_xor(tb[n][i], m);
         }
     __syncthreads();
     if ((tid & 63) < A.lpr) {
@@ -267,8 +278,8 @@ __global__ void __launch_bounds__(256) k_norm_rope(Args A) {
         if (live[n]) {
 #pragma unroll
           for (int i = 0; i < VEC; ++i) {
-            tab[(tid >> 6) * kMaxDim + (at[n].apart ? at[n].a + i : at[n].a + 2 * i)] = da[n][i];
-            tab[(tid >> 6) * kMaxDim + (at[n].apart ? at[n].b + i : at[n].a + 2 * i + 1)] = db[n][i];
+            tab[(tid >> 6) * kMaxDim + (at[n].apart ? at[n].a + i : at[n].a + 2 * i)] = ta[n][i];
+            tab[(tid >> 6) * kMaxDim + (at[n].apart ? at[n].b + i : at[n].a + 2 * i + 1)] = tb[n][i];
           }
         }
     }

@@ -441,3 +441,23 @@ def test_step_with_infinite_keys(device, dtype, d):
         kc[0, 3, :, 0], kc[1, 7, 1, 0] = low, low
         outs.append(ops.attention_step(q, k, v, kc, vc.clone(), table, lengths))
     assert bool(torch.isfinite(outs[1]).all()) and torch.equal(*outs)
+
+
+@pytest.mark.gpu
+def test_long_weight_gradients_of_one_sign():
+    """33 million rows of equal positive terms (two million tokens of one memory, expanded)."""
+    ops = make_ops("cuda:0")
+    n, heads, d = 1 << 21, 16, 256
+    gen = torch.Generator().manual_seed(14)
+    x, g = ((0.5 + torch.rand(1, 1, d, generator=gen)).bfloat16().cuda() for _ in range(2))
+    wide = [t.expand(n, heads, d) for t in (x, g)]
+    few = [t.expand(n, 1, d) for t in (x, g)]
+    w = torch.ones(d, device="cuda:0")
+    dwq, dwk = ops.norm_rope_backward(wide[1], few[1], wide[0], few[0], torch.zeros(n, dtype=torch.int32, device="cuda:0"),
+                                      torch.zeros(0, dtype=torch.float64, device="cuda:0"), w, w)[2:]
+    X, G = x.cpu().double(), g.cpu().double()
+    want = (G * X / torch.sqrt((X * X).mean(-1, keepdim=True) + 1e-6))[0, 0] * n
+    # a thread's 64 rows of a chunk of 64 tokens, 32 chunks, 2 exchanges and 4 wavefronts, 1024 partial rows in 32 chains of 32; 40 for a term
+    rel = (64 + 32 + 6 + 64 + 40) * U32
+    assert float((dwq.cpu().double() / (want * heads) - 1).abs().max()) <= rel
+    assert float((dwk.cpu().double() / want - 1).abs().max()) <= rel
