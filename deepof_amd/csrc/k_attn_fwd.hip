@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(64 * NW, DP <= 32 ? (NW == 1 && sizeof(T) == 4
         dof_store_vec<T, 4>(op + e, r);
       }
     }
-  if (half == 0) A.lse[(t.q0 + row) * A.q_heads + h] = sum == 0.0f ? -INFINITY : (m - DofSoftmax<T>::kUp + dof_log2(sum)) * kLn2;
+  if (half == 0) A.lse[(t.q0 + row) * A.q_heads + h] = sum == 0.0f ? -INFINITY : (m + dof_log2(sum * DofSoftmax<T>::kDown)) * kLn2;
 }
 
 template <class T, int DP>

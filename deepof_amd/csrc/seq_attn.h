@@ -35,10 +35,10 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // below 2^-25 of the maximum is zero in the products while the sum counts it, and many such weights are a recording's tail.  With
 // 2^11 what a weight loses is at most 2^-36 of the largest, and the largest, 2^(4 + 11), stays below 65504.
 template <class T> struct DofSoftmax {
-  static constexpr float kLag = 8.0f, kUp = 0.0f;
+  static constexpr float kLag = 8.0f, kUp = 0.0f, kDown = 1.0f;
 };
 template <> struct DofSoftmax<DofF16> {
-  static constexpr float kLag = 4.0f, kUp = 11.0f;
+  static constexpr float kLag = 4.0f, kUp = 11.0f, kDown = 1.0f / 2048.0f;  // kDown: 2^-kUp, for the logarithm of a sum
 };
 
 // t[i] = tanh(t[i] mul) of N scores of a lane.  Below 0.6 of the cap, where capped scores mostly lie, an odd polynomial (fitted to

@@ -461,3 +461,14 @@ def test_long_weight_gradients_of_one_sign():
     rel = (64 + 32 + 6 + 64 + 40) * U32
     assert float((dwq.cpu().double() / (want * heads) - 1).abs().max()) <= rel
     assert float((dwk.cpu().double() / want - 1).abs().max()) <= rel
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_float16_log_sum_exp_of_a_lifted_sum(device):
+    """The factor of float16 weights leaves the sum before its logarithm: equal scores of 0 over n keys give log n to 4 roundings of
+    it (a logarithm good to one step, log 2 and the product with it), not of log(2048 n)."""
+    ops = make_ops(device)
+    for n in (3, 5, 7, 11, 13):
+        q, k = torch.zeros(1, 1, 16, dtype=torch.float16, device=device), torch.zeros(n, 1, 16, dtype=torch.float16, device=device)
+        _, lse = ops.attention(ops.attention_plan([1], [n]), q, k, k)
+        assert abs(float(lse) - math.log(n)) <= 4 * U32 * math.log(n), n
