@@ -472,3 +472,30 @@ def test_float16_log_sum_exp_of_a_lifted_sum(device):
         q, k = torch.zeros(1, 1, 16, dtype=torch.float16, device=device), torch.zeros(n, 1, 16, dtype=torch.float16, device=device)
         _, lse = ops.attention(ops.attention_plan([1], [n]), q, k, k)
         assert abs(float(lse) - math.log(n)) <= 4 * U32 * math.log(n), n
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES[1:], ids=str)
+@pytest.mark.parametrize("n,new", [(300, 1), (1500, 3)])
+def test_step_is_as_good_as_rounding_its_result(device, dtype, n, new):
+    """16-bit weights keep their rest: o is off by its own rounding and fp32 arithmetic."""
+    ops = make_ops(device)
+    gen = torch.Generator().manual_seed(15)
+    d, page = 64, 100
+    q, k, v = (torch.randn(1, new, 2, d, generator=gen).to(dtype) for _ in range(3))
+    pages = -(-(n + new) // page)
+    kc, vc = (torch.randn(pages, page, 2, d, generator=gen).to(dtype) for _ in range(2))
+    table = torch.arange(pages, dtype=torch.int32, device=device)[None]
+    o = ops.attention_step(*(x.to(device) for x in (q, k, v)), kc.to(device), vc.to(device), table, torch.tensor([n], dtype=torch.int32, device=device))
+    K, V = kc.reshape(-1, 2, d)[:n].double(), vc.reshape(-1, 2, d)[:n].double()
+    for t in range(new):
+        for h in range(2):
+            Kt, Vt = (torch.cat((c[:, h], x[0, :t + 1, h].double())) for c, x in ((K, k), (V, v)))
+            Q = q[0, t, h].double()
+            p = torch.softmax(Kt @ Q / 8, 0)
+            want = p @ Vt
+            # scores: chains of 64 / 8 + 8 roundings of |q||k|; twice that and 64 for the weights, 2 u^2 for what value and rest leave
+            es = float((Kt.abs() @ Q.abs()).max()) / 8 * 16 * U32
+            rel = 2 * es + (64 + n / 32) * U32 + 2 * U[dtype] ** 2
+            bound = U[dtype] * want.abs() + 1.01 * rel * (p @ Vt.abs()) + TINY[dtype]
+            assert bool(((o[0, t, h].cpu().double() - want).abs() <= bound).all())
