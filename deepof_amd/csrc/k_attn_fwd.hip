@@ -9,7 +9,8 @@
 // the second one wants it in (the key order inside a fragment is permuted, the same on both operands).  V^T is read from row-major
 // LDS by the transposing LDS read.  Statistics and accumulators are fp32; P is rounded to the elements' type for its product (relative
 // half a step per weight, as the inputs' own; fp16 weights are lifted out of their subnormals, see DofSoftmax), the sum l is taken of
-// the unrounded weights.
+// the unrounded weights.  As value and rest, two products, P would take o's error from 1.2 - 1.4 times that of rounding o once to 1.0:
+// 24 ragged recordings with a bias 204 -> 250 us, 16384 frames, heads of 128, training 7.2 -> 7.9 ms (with dv's).  Not taken.
 #include <cmath>
 
 #include "deepof_hip.h"

@@ -31,7 +31,9 @@ namespace {
 
 constexpr int kStepKeys = 32;   // frames per wavefront and round
 constexpr int kMinTiles = 16;   // rounds of a part at least: four per wavefront
-constexpr int kWhole = 32;      // streams whose table holds no more rounds stay whole: a second kernel for the join costs more
+// Streams whose table holds no more rounds stay whole, which saves the second kernel for the join.  Eager calls, heads of 64 (8 / 2), one
+// stream, whole against parts: 1024 frames 21 / 25 us, 1536 22 / 25, 2048 27 / 25; 128 streams: 21 / 25, 27 / 31, 32 / 34.
+constexpr int kWhole = 32;
 constexpr int kTarget = 1024;   // parts of a call in all: two rounds of two workgroups per CU
 
 struct Step {
