@@ -136,9 +136,11 @@ Shares shares_of(const DofAttnPlan* p, const DofAttention* d) {
 }
 
 // Small documents: one kernel for all three gradients (4096 windows of 25 frames, 4 heads of 16, fp32: 84 us, dq and dk / dv kernels 138).
-// fp32 heads over 64 would not fit its registers.
+// fp32 heads over 64 would not fit its registers, nor the blocks that fp32 sums over more rows and query heads than kLongTerms want.
 bool one_pass(const DofAttnPlan* p, const DofAttention* d) {
-  return p->small && d->head_dim <= (d->dtype == DOF_DTYPE_F32 ? 64 : 128);
+  if (!p->small) return false;
+  if (d->dtype != DOF_DTYPE_F32) return true;
+  return d->head_dim <= 64 && (int64_t)p->longest * (d->q_heads / d->k_heads) <= kLongTerms;
 }
 
 int64_t delta_bytes(const DofAttnPlan* p, const DofAttention* d) { return (p->q_rows * d->q_heads * 4 + 15) / 16 * 16; }

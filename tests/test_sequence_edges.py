@@ -499,3 +499,25 @@ def test_step_is_as_good_as_rounding_its_result(device, dtype, n, new):
             rel = 2 * es + (64 + n / 32) * U32 + 2 * U[dtype] ** 2
             bound = U[dtype] * want.abs() + 1.01 * rel * (p @ Vt.abs()) + TINY[dtype]
             assert bool(((o[0, t, h].cpu().double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("heads,n", [(8, 32), (64, 32), (16, 25), (48, 200)])
+def test_float32_sums_over_many_query_heads(device, heads, n):
+    """One key head under many query heads: dv and dk add up the rows of all of them."""
+    ops = make_ops(device)
+    d = 16
+    q, g = (equal_terms(n, d).expand(n, heads, d).contiguous() for _ in range(2))
+    k, v = torch.zeros(n, 1, d), torch.zeros(n, 1, d)
+    v[:1, 0, 0] = 1.0  # dS: g0 (1 - 1 / n) / n for key 0, - g0 / n^2 for the others
+    plan = ops.attention_plan([n])
+    args = [x.to(device) for x in (q, k, v)]
+    o, lse = ops.attention(plan, *args)
+    dq, dk, dv = (x.cpu().double() for x in ops.attention_backward(plan, g.to(device), *args, o, lse))
+    # a chain of 256 additions (where each takes one term, as in the emulation), blocks of 256, at most 64 workgroups' parts; 64 for weights
+    rel = (256 + heads * n / 256 + 64 + 64) * U32
+    assert float((dv / (g[:1, :1].double() * heads) - 1).abs().max()) <= rel
+    size = g[0, 0, 0].double() * q[:1, :1].double() * heads * d ** -0.5
+    want = torch.cat((size * (1 - 1 / n), (-size / n).expand(n - 1, 1, d)))
+    # dS of the other keys is the difference 0 - delta, delta to rel
+    assert float((dk / want - 1).abs().max()) <= 3 * rel
