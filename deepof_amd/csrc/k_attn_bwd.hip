@@ -591,15 +591,14 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DP > 32 ? 1 : 2) k_
   if constexpr (DV) write(dv, ov, B.dv, B.dvs, B.part + B.splits * B.k_rows * A.k_heads * A.dim);
 }
 
-// dk and dv (blockIdx.y) from the parts of several workgroups per key tile, added in order: a workgroup per 32 rows of a tile and key
-// head, four elements a thread.  Rows of no tile have no parts and stay.
-constexpr int kJoinRows = 32;
+// dk and dv (blockIdx.y) from the parts of several workgroups per key tile, added in order: a workgroup per `take` rows of a tile and key
+// head (8, 16 or 32: about one group of four elements a thread), `pieces` of them per tile.  Rows of no tile have no parts and stay.
 template <class T>
-__global__ void __launch_bounds__(256) k_attn_join(DofAttnBwd B, int pieces) {
+__global__ void __launch_bounds__(256) k_attn_join(DofAttnBwd B, int pieces, int take) {
   const DofAttnFwd& A = B.f;
   const int item = blockIdx.x / A.k_heads, hk = blockIdx.x - item * A.k_heads, tile = item / pieces;
   const DofAttnTile t = A.tiles[tile];
-  const int first = t.row0 + (item - tile * pieces) * kJoinRows, rows = t.lk - first < kJoinRows ? t.lk - first : kJoinRows;
+  const int first = t.row0 + (item - tile * pieces) * take, rows = t.lk - first < take ? t.lk - first : take;
   const int quads = A.dim / 4;
   const float* part = B.part + (blockIdx.y ? B.splits * B.k_rows * A.k_heads * A.dim : 0);
   const int64_t* st = blockIdx.y ? B.dvs : B.dks;
@@ -669,8 +668,8 @@ int dof_launch_attn_dkv(const DofAttnBwd& B, int dtype, int flat, hipStream_t st
     else if (B.f.dim <= 96) launch_dkv<T, 96>(B, flat, stream);
     else launch_dkv<T, 128>(B, flat, stream);
     if (B.splits > 1) {
-      const int pieces = (flat ? kAttnFlat : kAttnTall) / kJoinRows;
-      DOF_LAUNCH((k_attn_join<T>), ((unsigned)((int64_t)B.f.n_tiles * pieces * B.f.k_heads), 2, 1), (256, 1, 1), stream, B, pieces);
+      const int take = B.f.dim > 64 ? 8 : B.f.dim > 32 ? 16 : 32, pieces = (flat ? kAttnFlat : kAttnTall) / take;
+      DOF_LAUNCH((k_attn_join<T>), ((unsigned)((int64_t)B.f.n_tiles * pieces * B.f.k_heads), 2, 1), (256, 1, 1), stream, B, pieces, take);
     }
   });
   return dof_check_launch("k_attn_dkv");
