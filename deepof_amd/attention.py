@@ -196,13 +196,6 @@ class AttentionPlan:
                     "dof_attn_plan_table")
         self.table = host.to(self.device)
 
-    def on_current_stream(self) -> int:
-        """The table's address for a call on the current stream.  The allocator is told of that stream, so that a plan which is
-        dropped gives its memory back only behind the call, also where another stream made it."""
-        if self.table.is_cuda:
-            self.table.record_stream(torch.cuda.current_stream(self.device))
-        return self.table.data_ptr()
-
     @staticmethod
     def _host(name, lengths):
         if isinstance(lengths, torch.Tensor) and lengths.is_cuda:
@@ -225,17 +218,22 @@ class AttentionOps:
         if self.device.type == "cuda" and self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
 
-    def _launch(self, name: str, *args):
+    def _launch(self, name: str, *args, plan: Optional[AttentionPlan] = None):
         """The entry point on the current stream of this object's device; launches go to the current device, so another one is made
-        current for the call."""
+        current for the call.  The allocator is told that the plan's tiles are read there, so that a plan which is dropped gives its
+        memory back only behind the call, also where another stream made it."""
         fn = getattr(self.lib, name)
         if self.device.type != "cuda":
             rc = fn(*args, 0)
-        elif torch.cuda.current_device() == self.device.index:
-            rc = fn(*args, torch.cuda.current_stream(self.device).cuda_stream)
         else:
-            with torch.cuda.device(self.device):
-                rc = fn(*args, torch.cuda.current_stream(self.device).cuda_stream)
+            stream = torch.cuda.current_stream(self.device)
+            if plan is not None:
+                plan.table.record_stream(stream)
+            if torch.cuda.current_device() == self.device.index:
+                rc = fn(*args, stream.cuda_stream)
+            else:
+                with torch.cuda.device(self.device):
+                    rc = fn(*args, stream.cuda_stream)
         if rc:
             _capi.check(self.lib, rc, name)
 
@@ -324,7 +322,7 @@ class AttentionOps:
         """The packing of a batch: document d has ``q_lengths[d]`` query rows and ``k_lengths[d]`` key rows (default: the same),
         one behind the other in the tensors.  ``causal``: the last query row stands at the last key, every row sees the keys up to
         its own; ``prefix``: the first ``prefix[d]`` keys of a document are visible to all its rows besides.  Lengths are host
-        data (lists, arrays, CPU tensors).  Build it once per batch and use it for every layer, forward and backward."""
+        data (lists, arrays, CPU tensors).  Build it once per batch, before any capture, and use it for every layer, forward and backward."""
         return AttentionPlan(self, q_lengths, k_lengths, causal, prefix)
 
     def _attention_args(self, plan, q, k, v, scale, cap, slopes):
@@ -370,8 +368,8 @@ class AttentionOps:
         q, k, v = _wide(q), _wide(k), _wide(v)
         ow = o if _is_wide(o) else o.clone(memory_format=torch.contiguous_format)
         rec = _capi.PACK_ATTENTION.pack(*head, *_st(q), *_st(k), *_st(v), *_st(ow), 0, 0, 0, 0, 0, 0, 0, 0)
-        self._launch("dof_attention_forward", C.byref(plan.record), plan.on_current_stream(), rec, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                     sl, ow.data_ptr(), lse.data_ptr())
+        self._launch("dof_attention_forward", C.byref(plan.record), plan.table.data_ptr(), rec, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                     sl, ow.data_ptr(), lse.data_ptr(), plan=plan)
         if ow is not o:
             o.copy_(ow)
         return o, lse
@@ -379,7 +377,9 @@ class AttentionOps:
     def attention_backward(self, plan, do, q, k, v, o, lse, scale: Optional[float] = None, cap: float = 0.0, slopes=None):
         """-> (dq, dk, dv) from the gradient at ``o`` and the forward's inputs and results; zeros in rows of no document.  The same
         bits on every run.  ``slopes`` are constants: they get no gradient.  float16: the scores' gradients are carried with a power
-        of two of their own, so that gradients of any size keep their precision; dq, dk and dv themselves are float16 numbers."""
+        of two of their own, so that gradients of any size keep their precision; dq, dk and dv themselves are float16 numbers.  What a
+        document's rows hold must be finite: an infinity or NaN of q, k, v or do reaches gradients of that document's other rows, those
+        that do not see it among them (other documents' it does not reach)."""
         head, sl = self._attention_args(plan, q, k, v, scale, cap, slopes)
         for name, t in (("do", do), ("o", o)):
             _rows(name, t, self.device, q.dtype)
@@ -393,8 +393,8 @@ class AttentionOps:
         rec = _capi.PACK_ATTENTION.pack(*head, *_st(q), *_st(k), *_st(v), *_st(o), *_st(do), *_st(dq), *_st(dk), *_st(dv))
         need = self._bytes("dof_attention_workspace_bytes", C.byref(plan.record), rec)
         ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-        self._launch("dof_attention_backward", C.byref(plan.record), plan.on_current_stream(), rec, do.data_ptr(), q.data_ptr(), k.data_ptr(),
-                     v.data_ptr(), sl, o.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(ws))
+        self._launch("dof_attention_backward", C.byref(plan.record), plan.table.data_ptr(), rec, do.data_ptr(), q.data_ptr(), k.data_ptr(),
+                     v.data_ptr(), sl, o.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(ws), plan=plan)
         return dq, dk, dv
 
     # ---- the new frames of live streams ------------------------------------------------------------------------------

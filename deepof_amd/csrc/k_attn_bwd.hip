@@ -5,16 +5,17 @@
 //   dv_j = sum_i p_ij g_i, dk_j = scale sum_i ds_ij q_i   (k_attn_dkv: a workgroup per key tile, walks the query rows that see it,
 //                                                          through all query heads of its group)
 //
-// Every gradient element is summed by one workgroup in a fixed order: no atomics, the same bits on every run.  The price is that S
-// and dP are computed twice (seven products of the size of S instead of five).  Both kernels keep their own rows' operands in
-// registers and stream the other side through LDS (two images); the second products take P and dS straight from the registers the
-// first ones left them in, as in the forward.
+// Every gradient element is summed in a fixed order, by one workgroup or in parts that k_attn_join adds up: no atomics, the same bits on
+// every run.  The price is that S and dP are computed again: heads up to 64 take nine products of the size of S with 16-bit elements (S and dP
+// twice, dv, dq and dk with their rests), larger ones ten (dv has a pass of its own, with S a third time).  The kernels keep their own rows'
+// operands in registers and stream the other side through LDS (two images); the second products take P and dS straight from the
+// registers the first ones left them in, as in the forward.
 //
-// P is rounded to the elements' type for its product with g, as in the forward (dv's error: 1.4 times that of rounding it).  dS goes into its products as two 16-bit numbers, value
-// and rest: rounded once, its error alone would be as large as that of rounding dq and dk themselves (of short documents it came to 1.8
-// times that, together with delta from the rounded o).  The second product costs a fifth: 16384 causal frames, 16 / 4 heads of 128, bf16:
-// dq 1.75 -> 2.28 ms, dk 1.83 -> 2.22 ms.  The dq kernel starts from
-// delta = g.o, sums the unrounded P dP on its way and leaves that delta to the dk kernel.  Everything that is summed is fp32.
+// P is rounded to the elements' type for its product with g, as in the forward (dv's error: 1.4 times that of rounding it).  dS goes into
+// its products as two 16-bit numbers, value and rest: rounded once, its error alone would be as large as that of rounding dq and dk
+// themselves (of short documents it came to 1.8 times that, together with delta from the rounded o).  The second product costs a fifth:
+// 16384 causal frames, 16 / 4 heads of 128, bf16: dq 1.75 -> 2.25 ms, dk 1.83 -> 2.16 ms.  The dq kernel starts from delta = g.o, sums the
+// unrounded P dP on its way and leaves that delta to the dk kernel.  Everything that is summed is fp32.
 // fp16 has 5 exponent bits: there P is carried as 2^12 P (an exact factor, taken out at the end), so that the weights of long
 // documents stay out of its subnormals, and dS with a power of two that follows its largest value (Range): gradients of any size
 // reach dq and dk as they would without the rounding.

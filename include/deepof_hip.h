@@ -531,7 +531,8 @@ int dof_attn_plan_size(int32_t n_docs, const int64_t* q_off, const int64_t* k_of
 int dof_attn_plan_table(const DofAttnPlan* plan, const int64_t* q_off, const int64_t* k_off, const int32_t* prefix, void* table);
 /* head_dim: multiples of 8 from 8 to 128; every tensor and stride a multiple of 16 bytes.  lse (fp32): (query rows, q_heads),
  * natural log.  Backward: g is the gradient at o; o and lse are the forward's; the workspace is 16-byte aligned.  Every gradient is
- * summed in a fixed order (no atomics). */
+ * summed in a fixed order (no atomics).  Forward: infinities and NaN at keys that a row does not see leave it as it is.  Backward: a
+ * document's q, k, v and g must be finite; other documents' infinities and NaN do not reach it. */
 typedef struct {
   int32_t dtype, head_dim, q_heads, k_heads;
   float scale, cap;
