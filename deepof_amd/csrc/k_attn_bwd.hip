@@ -1,4 +1,4 @@
-// Attention over packed documents, backward: two kernels that recompute the probabilities from the forward's log-sum-exp.
+// Attention over packed documents, backward: kernels that recompute the probabilities from the forward's log-sum-exp.
 //
 //   p = exp(s - lse) ; dp_ij = g_i.v_j ; ds = p (dp - delta_i) c_ij, delta_i = sum_d g_id o_id, c = 1 - tanh^2 under a cap, else 1
 //   dq_i = scale sum_j ds_ij k_j        (k_attn_dq:  a workgroup per query tile, walks the keys as the forward does)
