@@ -125,6 +125,7 @@ def _share(a: torch.Tensor, b: torch.Tensor) -> bool:
         a, b, apart = b, a, -apart
     if a.is_contiguous() and apart >= a.nbytes or a.numel() == 0 or b.numel() == 0:
         return False
+    a, b = (t if t.dim() else t.reshape(1) for t in (a, b))
     ea, eb, sa, sb = a.element_size(), b.element_size(), a.stride(), b.stride()
     inner_a, inner_b = ea, eb  # bytes from the first to the last of one row
     for n, s in zip(a.shape[1:], sa[1:]):

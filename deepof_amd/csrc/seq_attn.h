@@ -43,8 +43,8 @@ template <> struct DofSoftmax<DofF16> {
 
 // t[i] = tanh(t[i] mul) of N scores of a lane.  Below 0.6 of the cap, where capped scores mostly lie, an odd polynomial (fitted to
 // tanh(x) / x on [0, 0.6], relative error 1.5e-8) takes 8 instructions, none of them transcendental; from there on
-// 1 - 2 / (1 + 2^(2 log2(e) x)), whose quotient is below 0.47: off by 3 roundings of that and one of the result.  Which of them a score takes depends on it alone: what other
-// rows and hidden keys hold only decides whether the wavefront computes the second at all.
+// 1 - 2 / (1 + 2^(2 log2(e) x)), whose quotient is below 0.47: off by 3 roundings of that and one of the result.  Which of them a
+// score takes depends on it alone: what other rows and hidden keys hold only decides whether the wavefront computes the second at all.
 __device__ __forceinline__ float dof_tanh_near(float x) {
   const float y = x * x;
   float c = fmaf(y, -0.006276387721300125f, 0.021116213873028755f);

@@ -361,6 +361,9 @@ def test_slices_of_one_buffer(device):
         ops.attention(plan, q, q, q, out=o, lse=o.view(-1)[:27].view(9, 3))
     with pytest.raises(ValueError, match="share memory"):
         ops.attention(plan, q, q, q, lse=q.view(-1)[:27].view(9, 3))
+    for bad in (dict(lse=q.view(-1)[5]), dict(out=q.view(-1)[5]), dict(lse=torch.zeros((), device=device)), dict(out=torch.zeros((), device=device))):
+        with pytest.raises(ValueError):
+            ops.attention(plan, q, q, q, **bad)
     kv = torch.randn(6, 8, 4, 16, generator=gen).to(device)
     new, table, lengths = torch.randn(1, 1, 2, 16, device=device), torch.zeros(1, 1, dtype=torch.int32, device=device), torch.zeros(1, dtype=torch.int32, device=device)
     for a, b in ((kv[:4, :, :2], kv[1:5, :, :2]), (kv[:, :, :2], kv[:, :, 1:3])):
