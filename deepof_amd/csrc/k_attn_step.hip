@@ -10,7 +10,9 @@
 // The lengths are device data, so the split is made on the device: every workgroup adds up the streams' lengths, takes the part size
 // that yields about kTarget parts in all and finds the stream its own part lies in.  All parts are then about equally long, whatever the
 // mix of streams, and few workgroups are left without one (a split made on the host for the longest possible stream left most of
-// them empty or the longest stream's for the end: 64 streams of up to 5000 frames 81 us).
+// them empty or the longest stream's for the end: 64 streams of up to 5000 frames 81 us).  Work that every workgroup does for every
+// stream grows with their square: more than kFind streams have a kernel of one workgroup that lists the parts first, and streams
+// that all stay whole need no split.
 //
 // Inside a wavefront the products are transposed as in the forward pass (S^T = K Q^T, O^T = V^T P^T): keys go from memory straight
 // into the operand registers (a lane's 16 bytes are eight elements of one key), values through a wavefront-private LDS tile for the
@@ -36,6 +38,8 @@ constexpr int kMinTiles = 16;   // rounds of a part at least: four per wavefront
 constexpr int kWhole = 32;
 constexpr int kTarget = 1024;   // parts of a call in all: two rounds of two workgroups per CU
 
+constexpr int kFind = 256;      // streams up to which every workgroup finds its part itself: one length per thread
+
 struct Step {
   DofAttnStep d;
   DofScore score;
@@ -47,6 +51,9 @@ struct Step {
   float* part;    // [part][key head][row][dim] unnormalised sums
   float* stat;    // [part][key head][row][2] maximum and sum
   int32_t* sched; // [stream][2] first part and their number
+  int32_t* units; // more than kFind streams in parts: [part] its stream (-1: none), then the part size in tiles
+  int32_t parts;  // workgroups per key head and row block: parts at most; `whole`: streams
+  int32_t whole;  // every stream is one part
   int32_t rows, row_blocks, min_tiles, join_lanes, page_shift;  // page_shift: log2 of the page size, -1 if it is no power of two
 };
 
@@ -71,37 +78,70 @@ __device__ __forceinline__ int tiles_of(const Step& A, int b) {
   return (frames_of(A, b, &len) + kStepKeys - 1) / kStepKeys;
 }
 
-// The stream and the part of it that is number `unit` of all parts, and the part size in tiles; by all 256 threads.
+// tiles of a part, of `all` tiles of the streams
+__device__ __forceinline__ int part_size(const Step& A, int64_t all) {
+  const int64_t share = (all * A.d.k_heads * A.row_blocks + kTarget - 1) / kTarget, most = 1 << 30;  // more than the tiles of any stream
+  return share > most ? (int)most : share > A.min_tiles ? (int)share : A.min_tiles;
+}
+
+// The stream and the part of it that is number `unit` of all parts, and the part size in tiles; by all 256 threads, for kFind streams.
 struct Part { int stream, index, count, per; };
 __device__ __forceinline__ Part find_part(const Step& A, int unit) {
   __shared__ int low[4], high[4], upto_wave[4], found[3];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int mine = tid < A.d.streams ? tiles_of(A, tid) : 0;
-  auto tiles_at = [&](int b0) { return b0 == 0 ? mine : b0 + tid < A.d.streams ? tiles_of(A, b0 + tid) : 0; };
+  const int tiles = tid < A.d.streams ? tiles_of(A, tid) : 0;
   auto wave_sum = [&](int v) {
     for (int k = 32; k > 0; k >>= 1) v += dof_shfl_int(v, lane ^ k);
     return v;
   };
+  const int lo = wave_sum(tiles & 0xFFFF), hi = wave_sum(tiles >> 16);  // in two halves of 16 bits: the sum itself may pass 32
   if (tid == 0) found[0] = -1;
-  int64_t all = 0;
-  for (int b0 = 0; b0 < A.d.streams; b0 += 256) {  // in two halves of 16 bits: the sum itself may pass 32
-    if (b0 > 0) __syncthreads();
-    const int v = tiles_at(b0), lo = wave_sum(v & 0xFFFF), hi = wave_sum(v >> 16);
-    if (lane == 0) {
-      low[wave] = lo;
-      high[wave] = hi;
-    }
-    __syncthreads();
-    all += (int64_t)(low[0] + low[1] + low[2] + low[3]) + ((int64_t)(high[0] + high[1] + high[2] + high[3]) << 16);
+  if (lane == 0) {
+    low[wave] = lo;
+    high[wave] = hi;
   }
-  const int64_t share = (all * A.d.k_heads * A.row_blocks + kTarget - 1) / kTarget;
+  __syncthreads();
   Part p;
-  constexpr int64_t most = 1 << 30;  // more than the tiles of any stream
-  p.per = share > most ? (int)most : share > A.min_tiles ? (int)share : A.min_tiles;
+  p.per = part_size(A, (int64_t)(low[0] + low[1] + low[2] + low[3]) + ((int64_t)(high[0] + high[1] + high[2] + high[3]) << 16));
+  const int n = (tiles + p.per - 1) / p.per;
+  int upto = n;  // inclusive sum over the wavefront
+  for (int k = 1; k < 64; k <<= 1) {
+    const int below = dof_shfl_int(upto, lane >= k ? lane - k : lane);
+    if (lane >= k) upto += below;
+  }
+  if (lane == 63) upto_wave[wave] = upto;
+  __syncthreads();
+  int first = upto - n;
+  for (int w = 0; w < wave; ++w) first += upto_wave[w];
+  if (n > 0 && unit >= first && unit < first + n) {
+    found[0] = tid;
+    found[1] = unit - first;
+    found[2] = n;
+  }
+  __syncthreads();
+  p.stream = found[0];
+  p.index = found[1];
+  p.count = found[2];
+  return p;
+}
+
+// The parts of all streams, by one workgroup: sched and units.
+__global__ void __launch_bounds__(1024) k_attn_step_plan(Step A) {
+  __shared__ int64_t sums[1024];
+  __shared__ int upto_wave[16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int64_t all = 0;
+  for (int b = tid; b < A.d.streams; b += 1024) all += tiles_of(A, b);
+  sums[tid] = all;
+  for (int k = 512; k > 0; k >>= 1) {
+    __syncthreads();
+    if (tid < k) sums[tid] += sums[tid + k];
+  }
+  __syncthreads();
+  const int per = part_size(A, sums[0]);
   int before = 0;
-  for (int b0 = 0; b0 < A.d.streams; b0 += 256) {
-    if (b0 > 0) __syncthreads();
-    const int n = (tiles_at(b0) + p.per - 1) / p.per;
+  for (int b0 = 0; b0 < A.d.streams; b0 += 1024) {
+    const int b = b0 + tid, n = b < A.d.streams ? (tiles_of(A, b) + per - 1) / per : 0;
     int upto = n;  // inclusive sum over the wavefront
     for (int k = 1; k < 64; k <<= 1) {
       const int below = dof_shfl_int(upto, lane >= k ? lane - k : lane);
@@ -111,18 +151,16 @@ __device__ __forceinline__ Part find_part(const Step& A, int unit) {
     __syncthreads();
     int first = before + upto - n;
     for (int w = 0; w < wave; ++w) first += upto_wave[w];
-    if (n > 0 && unit >= first && unit < first + n) {
-      found[0] = b0 + tid;
-      found[1] = unit - first;
-      found[2] = n;
+    for (int w = 0; w < 16; ++w) before += upto_wave[w];
+    if (n > 0) {
+      A.sched[2 * b] = first;
+      A.sched[2 * b + 1] = n;
+      for (int k = 0; k < n; ++k) A.units[first + k] = b;
     }
-    before += upto_wave[0] + upto_wave[1] + upto_wave[2] + upto_wave[3];
+    __syncthreads();  // the next round writes upto_wave
   }
-  __syncthreads();
-  p.stream = found[0];
-  p.index = found[1];
-  p.count = found[2];
-  return p;
+  for (int u = before + tid; u < A.parts; u += 1024) A.units[u] = -1;
+  if (tid == 0) A.units[A.parts] = per;
 }
 
 // Four elements of a row's output: the sums divided by the weights' sum, and with several new frames the infinities and NaN among the
@@ -160,14 +198,25 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && DP > 32 * (3 - RT) + 32
   const int rb = item % A.row_blocks;
   item /= A.row_blocks;
   const int unit = item / A.d.k_heads, hk = item - unit * A.d.k_heads;
-  const Part part = find_part(A, unit);
+  Part part;
+  if (A.whole) {
+    part = {unit, 0, 1, 1 << 30};
+  } else if (A.units) {
+    part.stream = A.units[unit];
+    part.per = A.units[A.parts];
+    part.index = part.stream < 0 ? 0 : unit - A.sched[2 * part.stream];
+    part.count = part.stream < 0 ? 0 : A.sched[2 * part.stream + 1];
+  } else {
+    part = find_part(A, unit);
+  }
   if (part.stream < 0) return;  // uniform: fewer parts than workgroups
   const int b = part.stream;
   int len;
   const int total = frames_of(A, b, &len);
+  if (total == 0) return;  // uniform: idle
   const int tiles = (total + kStepKeys - 1) / kStepKeys;
   const int32_t* table = A.table + (int64_t)b * A.d.max_pages;
-  if (A.sched && part.index == 0 && hk == 0 && rb == 0 && tid == 0) {
+  if (A.sched && !A.units && part.index == 0 && hk == 0 && rb == 0 && tid == 0) {
     A.sched[2 * b] = unit;
     A.sched[2 * b + 1] = part.count;
   }
@@ -572,7 +621,7 @@ extern "C" int64_t dof_attention_step_workspace_bytes(const DofAttnStep* d) {
   if (check(d, "dof_attention_step_workspace_bytes") != DOF_OK) return -1;
   const Shape s = shape_of(d);
   if (!joins(d, s)) return 0;
-  return (part_floats(d, s) + s.parts * d->k_heads * s.rows * 2 + 2 * (int64_t)d->streams) * 4;
+  return (part_floats(d, s) + s.parts * d->k_heads * s.rows * 2 + 2 * (int64_t)d->streams + (d->streams > kFind ? s.parts + 1 : 0)) * 4;
 }
 
 extern "C" int dof_attention_step(const DofAttnStep* d, const void* q, const void* k, const void* v, void* k_cache, void* v_cache,
@@ -620,7 +669,10 @@ extern "C" int dof_attention_step(const DofAttnStep* d, const void* q, const voi
     A.part = static_cast<float*>(workspace);
     A.stat = A.part + part_floats(d, s);
     A.sched = reinterpret_cast<int32_t*>(A.stat + s.parts * d->k_heads * s.rows * 2);
+    if (d->streams > kFind) A.units = A.sched + 2 * (int64_t)d->streams;
   }
+  A.parts = (int32_t)s.parts;
+  A.whole = !joins(d, s);
   A.rows = s.rows;
   A.row_blocks = s.row_blocks;
   A.min_tiles = s.min_tiles;
@@ -631,6 +683,7 @@ extern "C" int dof_attention_step(const DofAttnStep* d, const void* q, const voi
   // the most tiles that the streams' tables let a part have, four wavefronts to share them, kStepKeys / 4 additions each
   const int64_t tiles = ((int64_t)d->max_pages * d->page_size + kStepKeys - 1) / kStepKeys, share = d->streams * tiles * d->k_heads * s.row_blocks / kTarget;
   const bool grows = std::max<int64_t>(s.min_tiles, share) / 4 * (kStepKeys / 2) > kLongTerms;
+  if (A.units) DOF_LAUNCH(k_attn_step_plan, (1, 1, 1), (1024, 1, 1), (hipStream_t)stream, A);
   DOF_SEQ_DISPATCH(d->dtype, T, {
     if (d->head_dim <= 32) launch<T, 32>(A, s.rt, grows, (unsigned)blocks, (hipStream_t)stream);
     else if (d->head_dim <= 64) launch<T, 64>(A, s.rt, grows, (unsigned)blocks, (hipStream_t)stream);

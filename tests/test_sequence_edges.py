@@ -524,3 +524,40 @@ def test_float32_sums_over_many_query_heads(device, heads, n):
     want = torch.cat((size * (1 - 1 / n), (-size / n).expand(n - 1, 1, d)))
     # dS of the other keys is the difference 0 - delta, delta to rel
     assert float((dk / want - 1).abs().max()) <= 3 * rel
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("many,hk,long", [(1500, 1, {3: 1200, 1030: 600, 1499: 900}), (257, 2, {256: 700, 0: 0}), (2, 1100, {0: 1200})])
+def test_step_of_many_streams_or_heads(device, many, hk, long):
+    """More streams than a workgroup finds parts for, idle ones among them; so many heads that long streams stay whole."""
+    ops = make_ops(device)
+    d, page = 8, 16
+    gen = torch.Generator().manual_seed(17)
+    lens = [int(x) for x in torch.randint(0, 40, (many,), generator=gen)]
+    for b, n in long.items():
+        lens[b] = n
+    pages = [-(-(n + 1) // page) for n in lens]
+    table, at = torch.full((many, max(pages)), -1, dtype=torch.int32), 0
+    for b, c in enumerate(pages):
+        table[b, :c] = torch.arange(at, at + c, dtype=torch.int32)
+        at += c
+    kc, vc = (torch.randn(at, page, hk, d, generator=gen) for _ in range(2))
+    q, k, v = (torch.randn(many, 1, hk, d, generator=gen) for _ in range(3))
+    lengths = torch.tensor(lens, dtype=torch.int32)
+    idle = [b for b in (1, 5, 1100) if b < many]
+    lengths[idle] = -1
+    kd, vd, out = kc.to(device), vc.to(device), torch.full((many, 1, hk, d), 7.0, device=device)
+    ops.attention_step(*(x.to(device) for x in (q, k, v)), kd, vd, table.to(device), lengths.to(device), out=out)
+    for b in range(many):
+        if b in idle:
+            assert bool((out[b] == 7).all())
+            continue
+        rows = table[b, :pages[b]].long()
+        K, V = (torch.cat((c[rows].reshape(-1, hk, d)[:lens[b]], x[b])).double() for c, x in ((kc, k), (vc, v)))
+        s = torch.einsum("nhd,hd->hn", K, q[b, 0].double()) * d ** -0.5
+        want = torch.einsum("hn,nhd->hd", torch.softmax(s, 1), V)
+        es = float((K.abs() * q[b].double().abs()).sum(-1).max()) * d ** -0.5 * 16 * U32  # chains of 8 / 8 + 8 roundings
+        bound = (2 * es + (64 + lens[b] / 32) * U32) * float(V.abs().max()) * 1.01
+        assert float((out[b, 0].cpu().double() - want).abs().max()) <= bound
+        kc[table[b, lens[b] // page], lens[b] % page], vc[table[b, lens[b] // page], lens[b] % page] = k[b, 0], v[b, 0]
+    assert torch.equal(kd.cpu(), kc) and torch.equal(vd.cpu(), vc)
