@@ -33,8 +33,9 @@ namespace {
 
 constexpr int kStepKeys = 32;   // frames per wavefront and round
 constexpr int kMinTiles = 16;   // rounds of a part at least: four per wavefront
-// Streams whose table holds no more rounds stay whole, which saves the second kernel for the join.  Eager calls, heads of 64 (8 / 2), one
-// stream, whole against parts: 1024 frames 21 / 25 us, 1536 22 / 25, 2048 27 / 25; 128 streams: 21 / 25, 27 / 31, 32 / 34.
+// Streams whose table holds no more rounds stay whole, which saves the second kernel for the join.  Replayed from a graph (eager calls
+// hide their kernels behind the host), 8 / 2 heads of 64, one stream, whole against parts: 768 frames 11 / 15 us, 1024 13.6 / 14.7,
+// 1536 18.6 / 14.7, 2048 24 / 15; 128 streams: 14 / 20, 17 / 22, 24 / 27, 30 / 37.
 constexpr int kWhole = 32;
 constexpr int kTarget = 1024;   // parts of a call in all: two rounds of two workgroups per CU
 
