@@ -561,3 +561,39 @@ def test_step_of_many_streams_or_heads(device, many, hk, long):
         assert float((out[b, 0].cpu().double() - want).abs().max()) <= bound
         kc[table[b, lens[b] // page], lens[b] % page], vc[table[b, lens[b] // page], lens[b] % page] = k[b, 0], v[b, 0]
     assert torch.equal(kd.cpu(), kc) and torch.equal(vd.cpu(), vc)
+
+
+@pytest.mark.gpu
+def test_graph_of_many_streams_follows_lengths():
+    """300 streams, whose parts a kernel of its own lists: replayed while lengths and idle streams change, the eager results."""
+    ops = make_ops("cuda:0")
+    many, hk, d, page = 300, 2, 16, 16
+    gen = torch.Generator().manual_seed(18)
+    lens = torch.randint(0, 60, (many,), generator=gen, dtype=torch.int32)
+    lens[7], lens[290] = 1500, 900
+    table = torch.zeros(many, 100, dtype=torch.int32)
+    at = 0
+    for b in range(many):
+        c = -(-(int(lens[b]) + 8) // page)
+        table[b, :c] = torch.arange(at, at + c, dtype=torch.int32)
+        at += c
+    caches = [torch.randn(at, page, hk, d, generator=gen) for _ in range(2)]
+    q, k, v = (torch.randn(many, 1, h, d, generator=gen).cuda() for h in (4, hk, hk))
+    (kd, vd), (ke, ve), table = [x.cuda() for x in caches], [x.cuda() for x in caches], table.cuda()
+    ln, out = lens.cuda(), torch.zeros_like(q)
+    ops.attention_step(q, k, v, kd.clone(), vd.clone(), table, ln, out=out.clone())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.attention_step(q, k, v, kd, vd, table, ln, out=out)
+    want = out.clone()
+    for i in range(4):
+        q.mul_(1.1)
+        if i == 2:
+            ln[[7, 20]] = -1
+        le = ln.clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        ops.attention_step(q, k, v, ke, ve, table, le, out=want)
+        assert torch.equal(out, want) and torch.equal(kd, ke) and torch.equal(vd, ve)
+        ln[ln >= 0] += 1
